@@ -414,6 +414,55 @@ T81B200_API int t81b200_tq_to_packed(const uint8_t *blocks, int64_t rows, int64_
 T81B200_API size_t t81b200_gemm_trit_workspace_bytes(int b_dtype, int layout, int c_dtype, int64_t M,
                                          int64_t N, int64_t K);
 
+/* 4-bit weights with group scales ("Q4") — for layers that ternary weights lose too much of (language-model heads, experts).
+ * No counterpart in the reference.  Columns of a row go in groups of 32, 64 or 128 (the last may be shorter).  A group's scale is its
+ * value of largest magnitude (the first of equals) over -8, rounded to five significant bits; a weight's code is the whole
+ * number nearest to weight / scale (ties to even) in -8 .. 7.  code * scale is a bf16 number.  What is no number counts as 0,
+ * magnitudes above 2^126 as that, groups below 2^-100 throughout are 0.
+ *   Codes: tiles of 16 rows x 64 columns, tile (T, c) at byte (T * ceil(cols / 64) + c) * 512; inside, lane l = 4 g + t owns the four
+ *   32-bit words at 16 l; bits 4 r + 16 h .. + 3 of word j hold code + 8 of row 16 T + g + 8 (r % 2), column
+ *   64 c + 32 (j / 2) + 8 t + 4 (j % 2) + 2 (r / 2) + h.  Scales (bf16): those of tile row T and group u at element
+ *   (T * ceil(cols / group) + u) * 16, row r of the tile at 2 (r % 8) + r / 8.  Past the matrix codes and scales are 0.
+ *   q4_bytes / q4_scales: bytes of the codes and number of scales of one matrix, -1 on bad arguments.
+ *   quantize_q4:   `matrices` matrices `matrix_stride` elements apart, row stride ld; their codes and scales lie one behind the other
+ *                  (16-byte aligned).
+ *   dequantize_q4: (matrices, rows, cols) contiguous, exact in fp32 and bf16.
+ *   linear_q4:     C (N, M) = B (N, K) W^T + bias, W (M, K); B as it is where its type is 16-bit, its rows lie on 16-byte boundaries and
+ *                  K % 8 == 0, else through the workspace (linear_q4_workspace_bytes for this very B, 16-byte aligned).  Products are
+ *                  exact and sums fp32; fp32 activations keep all 24 bits.
+ *   experts_q4:    the same with rows sorted by expert: row p is multiplied by matrix e, offsets[e] <= p < offsets[e + 1]; codes, scales
+ *                  and bias (n_experts, M) one expert behind the other; offsets: n_experts + 1 rising numbers on the device,
+ *                  from 0.  Rows at or past offsets[n_experts] become 0. */
+T81B200_API int64_t t81b200_q4_bytes(int64_t rows, int64_t cols);
+T81B200_API int64_t t81b200_q4_scales(int64_t rows, int64_t cols, int group);
+T81B200_API int t81b200_quantize_q4(const void *w, int w_dtype, int64_t matrices, int64_t rows, int64_t cols, int64_t ld, int64_t matrix_stride, int group, uint8_t *codes,
+                                    void *scales, void *stream);
+T81B200_API int t81b200_dequantize_q4(const uint8_t *codes, const void *scales, int64_t matrices, int64_t rows, int64_t cols, int group, void *out, int out_dtype, void *stream);
+T81B200_API size_t t81b200_linear_q4_workspace_bytes(const void *B, int b_dtype, int64_t ldb, int64_t N, int64_t K);
+T81B200_API int t81b200_linear_q4(const uint8_t *codes, const void *scales, const float *bias, void *C, int64_t M, const void *B, int b_dtype, int64_t ldb, int c_dtype, int64_t ldc,
+                                  int64_t N, int64_t K, int group, void *workspace, size_t workspace_bytes, void *stream);
+T81B200_API int t81b200_experts_q4(const uint8_t *codes, const void *scales, const float *bias, void *C, int64_t M, const void *B, int b_dtype, int64_t ldb, int c_dtype, int64_t ldc,
+                                   int64_t N, int64_t K, int group, const int32_t *offsets, int n_experts, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Rows of a mixture of experts.  n = tokens * top (token, slot) pairs, flat index token * top + slot, n < 2^31.  No counterpart in the
+ * reference.
+ *   sort_by_expert: ids (n int32 or int64, id_bytes 4 or 8) to order (n), position (n) and offsets (n_experts + 1): order[p] is the flat
+ *       index of sorted row p, pairs of one expert in their order, -1 past the last; position is the inverse, -1 for ids outside
+ *       0 .. n_experts - 1, which take no part; expert e has the rows offsets[e] .. offsets[e + 1] - 1.  At most 1024 experts.
+ *   gather_rows:  rows (n, width), contiguous: row position[i] = row i / top of x (tokens, width; ld); rows from *kept on are 0.
+ *   combine_rows: y (tokens, width), contiguous: y[t] = sum over slots of weights[t][j] * rows[position[t][j]] (1 where weights is NULL),
+ *       in fp32, in slot order, rounded once; slots without a row take no part, whatever their weight.
+ *   combine_rows_grad: grad_rows[position[i]] = weights[i] * grad_y[i / top], 0 from *kept on; grad_weights[i] = <grad_y[i / top],
+ *       rows[position[i]]>, 0 without a row.  Either may be NULL.
+ * kept: device pointer to the number of rows, offsets + n_experts. */
+T81B200_API int t81b200_sort_by_expert(const void *ids, int id_bytes, int64_t n, int n_experts, int32_t *order, int32_t *position, int32_t *offsets, void *stream);
+T81B200_API int t81b200_gather_rows(const void *x, int dtype, int64_t ld, int64_t tokens, int64_t top, int64_t width, const int32_t *position, const int32_t *kept, void *rows,
+                                    void *stream);
+T81B200_API int t81b200_combine_rows(const void *rows, int dtype, int64_t ld, int64_t tokens, int64_t top, int64_t width, const int32_t *position, const void *weights, int w_dtype,
+                                     void *y, void *stream);
+T81B200_API int t81b200_combine_rows_grad(const void *grad_y, int64_t ld_y, const void *rows, int dtype, int64_t ld, int64_t tokens, int64_t top, int64_t width, const int32_t *position,
+                                          const int32_t *kept, const void *weights, int w_dtype, void *grad_rows, void *grad_weights, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -13,19 +13,25 @@ Kept from the reference: the ``threshold`` / ``keep_biases_bf16`` arguments and 
 to the model, and the ``t81_metadata.json`` side file written by ``save_pretrained_t81`` and read
 back by ``from_pretrained_t81``.  Loading by name goes through ``transformers`` exactly as the
 reference does and needs that package; converting an ``nn.Module`` instance does not.
+
+What ternary weights lose too much of can be kept in 4 bits (``four_bit``: names of modules, with wildcards): an ``nn.Linear`` becomes
+``nn.Q4Linear``, a module that holds a mixture's experts as stacked weights becomes ``nn.Q4Experts``.  The reference has no such
+choice.
 """
 
 from __future__ import annotations
 
 import json
 from dataclasses import dataclass
+from fnmatch import fnmatchcase
 from pathlib import Path
-from typing import Any, Callable, Mapping, Optional
+from typing import Any, Callable, Mapping, Optional, Sequence
 
 import torch
 from torch import nn
 
 from .nn import Linear as TernaryLinear
+from .nn import Q4Experts, Q4Linear
 from . import torch as t81_torch
 
 _METADATA_FILENAME = "t81_metadata.json"
@@ -38,6 +44,8 @@ class ConversionStats:
     ternary_bytes: int = 0
     replaced: int = 0
     packed_on_device: int = 0
+    four_bit: int = 0        # modules that went to 4 bits, not counted in `replaced`
+    four_bit_bytes: int = 0  # their codes and scales
 
 
 def _ternary_byte_count(shape) -> int:
@@ -84,6 +92,58 @@ def _convert_linear_layer(linear: nn.Module, threshold: float, keep_biases_bf16:
     return ternary
 
 
+def _holds_experts(module: nn.Module) -> bool:
+    """A module whose only parameters are stacked experts: ``gate_up_proj`` (experts, 2 ffn, hidden) and ``down_proj`` (experts, hidden,
+    ffn), with their activation in ``act_fn``, called with (hidden_states, top_k_index, top_k_weights)."""
+    names = {name for name, _ in module.named_parameters()}
+    if names != {"gate_up_proj", "down_proj"} or not callable(getattr(module, "act_fn", None)):
+        return False
+    gate_up, down = module.gate_up_proj, module.down_proj
+    return gate_up.ndim == 3 and down.ndim == 3 and gate_up.shape == (down.shape[0], 2 * down.shape[2], down.shape[1])
+
+
+def _named(name: str, patterns: Sequence[str]) -> bool:
+    return any(fnmatchcase(name, pattern) for pattern in patterns)
+
+
+def _four_bit_modules(model: nn.Module, patterns: Sequence[str]) -> "list[str]":
+    """The modules that the names mean, checked before any is replaced."""
+    if isinstance(patterns, str):
+        raise TypeError("four_bit takes a sequence of module names")
+    found = []
+    for name, module in model.named_modules():
+        if not name or not _named(name, patterns):
+            continue
+        if isinstance(module, TernaryLinear) and getattr(module, "_t81_float_released", False):
+            raise ValueError(f"four_bit: the float weight of {name} was released")
+        if isinstance(module, nn.Linear) or _holds_experts(module):
+            weights = [module.weight] if isinstance(module, nn.Linear) else [module.gate_up_proj, module.down_proj]
+            if any(w.is_meta or not w.is_cuda for w in weights):
+                raise ValueError(f"four_bit: the weights of {name} must be on a CUDA device")
+            if any(w.numel() == 0 for w in weights):
+                raise ValueError(f"four_bit: {name} has no weights")
+            found.append(name)
+    for pattern in patterns:
+        if not any(fnmatchcase(name, pattern) for name in found):
+            raise ValueError(f"four_bit: no nn.Linear and no stacked experts are named {pattern!r}")
+    return found
+
+
+def _to_four_bit(model: nn.Module, names: Sequence[str], group: int, keep_biases_bf16: bool, stats: ConversionStats) -> None:
+    for name in names:
+        parent_name, _, leaf = name.rpartition(".")
+        module, parent = model.get_submodule(name), model.get_submodule(parent_name) if parent_name else model
+        if isinstance(module, nn.Linear):
+            new = Q4Linear.from_linear(module, group)
+            if not keep_biases_bf16 and new.bias is not None and new.bias.dtype == torch.bfloat16:
+                new.bias = nn.Parameter(new.bias.detach().to(torch.float32), requires_grad=new.bias.requires_grad)
+        else:
+            new = Q4Experts.from_float(module.gate_up_proj, module.down_proj, module.act_fn, group).train(module.training)
+        setattr(parent, leaf, new)
+        stats.four_bit += 1
+        stats.four_bit_bytes += sum(b.numel() * b.element_size() for b in new.buffers())
+
+
 def _walk_and_replace(module: nn.Module, threshold: float, keep_biases_bf16: bool, rule: str, pack_now: bool,
                       release_float: bool, stats: ConversionStats) -> None:
     """t81/convert.py:142-153."""
@@ -104,7 +164,7 @@ def _report_stats(stats: ConversionStats) -> None:
     print(f"t81.convert: replaced {stats.replaced} nn.Linear modules, "
           f"compressed {stats.float_bytes / mib:.2f} MiB -> {stats.ternary_bytes / mib:.2f} MiB "
           f"(ratio {ratio:.2f}), estimated VRAM savings {(stats.float_bytes - stats.ternary_bytes) / mib:.2f} MiB; "
-          f"{stats.packed_on_device} packed on the device")
+          f"{stats.packed_on_device} packed on the device" + (f"; {stats.four_bit} modules in 4 bits, {stats.four_bit_bytes / mib:.2f} MiB" if stats.four_bit else ""))
 
 
 def _load_model(model_id_or_path: str, device_map, torch_dtype):
@@ -126,13 +186,24 @@ def _load_model(model_id_or_path: str, device_map, torch_dtype):
 
 
 def convert_module(model: nn.Module, threshold: float = 0.45, keep_biases_bf16: bool = True, *, rule: str = "fixed",
-                   pack_now: bool = True, release_float: bool = False, verbose: bool = True) -> ConversionStats:
+                   pack_now: bool = True, release_float: bool = False, verbose: bool = True,
+                   four_bit: Sequence[str] = (), q4_group: int = 128) -> ConversionStats:
     """Ternarise every ``nn.Linear`` below ``model`` in place (t81/convert.py:214-221) and return the
     statistics.  With ``pack_now`` weights that live on a CUDA device are quantised and packed there
     immediately; others are packed lazily by the first eval forward, like the reference.  ``release_float``
     drops the float weight of every layer packed here (inference only: such a layer cannot train, and its
-    ``state_dict`` no longer holds the float weight)."""
+    ``state_dict`` no longer holds the float weight).
+
+    ``four_bit`` names modules (``"lm_head"``, ``"layers.*.mlp.experts"``) that go to 4-bit weights with a scale per ``q4_group``
+    columns instead: each ``nn.Linear`` and each module of stacked experts so named, whose weights must be on a CUDA device and whose
+    float weights are given up."""
     stats = ConversionStats()
+    if q4_group not in (32, 64, 128):
+        raise ValueError(f"groups of 32, 64 or 128 columns, not {q4_group}")
+    if four_bit:
+        _to_four_bit(model, _four_bit_modules(model, four_bit), q4_group, keep_biases_bf16, stats)
+        setattr(model, "_t81_four_bit", list(four_bit))
+        setattr(model, "_t81_q4_group", q4_group)
     _walk_and_replace(model, threshold, keep_biases_bf16, rule, pack_now, release_float, stats)
     setattr(model, "_t81_threshold", threshold)
     setattr(model, "_t81_keep_biases_bf16", keep_biases_bf16)
@@ -146,7 +217,7 @@ def convert_module(model: nn.Module, threshold: float = 0.45, keep_biases_bf16: 
 def convert(model_id_or_path, threshold: float = 0.45, keep_biases_bf16: bool = True,
             device_map: "str | Mapping[str, Any] | None" = "auto", torch_dtype: Optional[torch.dtype] = None, *,
             inplace: bool = False, force_cpu_device_map: bool = False, rule: str = "fixed", pack_now: bool = True,
-            release_float: bool = False) -> nn.Module:
+            release_float: bool = False, four_bit: Sequence[str] = (), q4_group: int = 128) -> nn.Module:
     """t81/convert.py:224-264.  A checkpoint name or path is loaded through ``transformers``; a model instance
     is converted as it is and, as in the reference, needs ``inplace=True``."""
     if isinstance(model_id_or_path, nn.Module):
@@ -159,7 +230,7 @@ def convert(model_id_or_path, threshold: float = 0.45, keep_biases_bf16: bool = 
         if isinstance(effective_device_map, str) and effective_device_map.strip().lower() == "none":
             effective_device_map = None
         model = _load_model(str(model_id_or_path), effective_device_map, torch_dtype)
-    convert_module(model, threshold, keep_biases_bf16, rule=rule, pack_now=pack_now, release_float=release_float)
+    convert_module(model, threshold, keep_biases_bf16, rule=rule, pack_now=pack_now, release_float=release_float, four_bit=four_bit, q4_group=q4_group)
     spec: dict = {"device_map": effective_device_map, "torch_dtype": torch_dtype, "threshold": threshold,
                   "keep_biases_bf16": keep_biases_bf16, "rule": rule}
     if isinstance(model_id_or_path, (str, Path)):
@@ -185,7 +256,7 @@ def save_pretrained_t81(model: nn.Module, save_directory, *, threshold: Optional
     directory.mkdir(parents=True, exist_ok=True)
     if call_save_pretrained:
         if any(getattr(m, "_t81_float_released", False) for m in model.modules()):
-            raise RuntimeError("float weights were released at conversion (release_float=True); nothing to save")
+            raise RuntimeError("float weights were released at conversion (release_float=True or four_bit); nothing to save")
         saver = save_fn or getattr(type(model), "__t81_original_save_pretrained__", None)
         if saver is not None:
             saver(model, directory, **kwargs)
@@ -198,6 +269,8 @@ def save_pretrained_t81(model: nn.Module, save_directory, *, threshold: Optional
         "keep_biases_bf16": keep_biases_bf16 if keep_biases_bf16 is not None else getattr(model, "_t81_keep_biases_bf16", True),
         "rule": getattr(model, "_t81_rule", "fixed"),
     }
+    if getattr(model, "_t81_four_bit", None):
+        metadata |= {"four_bit": model._t81_four_bit, "q4_group": model._t81_q4_group}
     with _metadata_path(directory).open("w", encoding="utf-8") as handle:
         json.dump(metadata, handle)
 
@@ -224,7 +297,8 @@ def from_pretrained_t81(cls, pretrained_model_name_or_path, *model_args: Any, th
     else:
         model = cls.from_pretrained(pretrained_model_name_or_path, *model_args, trust_remote_code=trust_remote_code,
                                     device_map=device_map, torch_dtype=torch_dtype, **model_kwargs)
-    convert_module(model, threshold, keep_biases_bf16, rule=metadata.get("rule", "fixed"), verbose=False)
+    convert_module(model, threshold, keep_biases_bf16, rule=metadata.get("rule", "fixed"), verbose=False,
+                   four_bit=metadata.get("four_bit", ()), q4_group=metadata.get("q4_group", 128))
     return model
 
 

@@ -1,0 +1,50 @@
+// The 4-bit weight format ("Q4") and what the kernels that read it share.
+//
+// Columns of a row go in groups of 32, 64 or 128.  A weight is code * scale, code in -8 .. 7, scale a bf16 number of five significant
+// bits per row and group; so the weight itself is a bf16 number (3 + 5 bits), and kernels that multiply codes and scale the sums give
+// the same products as ones that multiply the weights.
+//
+// Codes lie in tiles of 16 rows x 64 columns, 512 bytes, tile (T, c) at (T * ceil(cols / 64) + c) * 512, in the order of the mma.sync
+// m16n8k16 A fragments: lane l = 4 g + t owns the four words at 16 l; word j holds in bits 4 r + 16 h (four of them) code + 8 of
+//     row 16 T + g + 8 (r % 2),  column 64 c + 32 (j / 2) + 8 t + 4 (j % 2) + 2 (r / 2) + h.
+// Words 0, 1 are columns 0 .. 31 and words 2, 3 columns 32 .. 63, so that no multiply mixes two groups, and a lane's eight columns of either
+// half are 16 bytes of an activation row or of an operand tile.  Scales of tile row T and group u: 16 bf16 numbers at
+// (T * ceil(cols / group) + u) * 16, row r of the tile at 2 (r % 8) + r / 8: a lane's two rows are one word.
+// Rows and columns past the matrix have code 0 (bits 8) and scale 0.
+#pragma once
+
+#include "common.cuh"
+
+namespace t81b200 {
+
+constexpr int kQ4TileBytes = 512;
+
+__host__ __device__ inline int64_t q4_row_tiles(int64_t rows) { return (rows + 15) / 16; }
+__host__ __device__ inline int64_t q4_col_tiles(int64_t cols) { return (cols + 63) / 64; }
+__host__ __device__ inline int64_t q4_groups(int64_t cols, int group) { return (cols + group - 1) / group; }
+
+inline bool q4_group_ok(int group) { return group == 32 || group == 64 || group == 128; }
+
+// Register r of a word as a pair of exact numbers -8 .. 7.  The four bits go to where the units 1 to 8 lie in the mantissa of 16 (bf16: bit
+// 3, fp16: bit 6), which gives 16 + code + 8; one packed FMA takes the 24 away.
+template <typename T> struct Q4Decode;
+template <> struct Q4Decode<__nv_bfloat16> {
+    template <int R> static __device__ __forceinline__ uint32_t biased(uint32_t w) {
+        const uint32_t x = R == 0 ? w << 3 : w >> (4 * R - 3);
+        return (x & 0x00780078u) | 0x41804180u;
+    }
+    static __device__ __forceinline__ uint32_t minus24(uint32_t v) { return fma_bf16x2(v, 0x3F803F80u, 0xC1C0C1C0u); }
+};
+template <> struct Q4Decode<__half> {
+    template <int R> static __device__ __forceinline__ uint32_t biased(uint32_t w) {
+        const uint32_t x = R < 2 ? w << (6 - 4 * R) : w >> (4 * R - 6);
+        return (x & 0x03C003C0u) | 0x4C004C00u;
+    }
+    static __device__ __forceinline__ uint32_t minus24(uint32_t v) {
+        uint32_t d;
+        asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(v), "r"(0xCE00CE00u));
+        return d;
+    }
+};
+
+}  // namespace t81b200

@@ -553,6 +553,361 @@ PyObject *gemm_trit(PyObject *, PyObject *const *args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---- 4-bit weights with group scales ----
+
+// codes and scales hold `matrices` rows x k matrices with groups of `group` columns.
+bool holds_q4(const Tensor &codes, const Tensor &scales, int64_t matrices, int64_t rows, int64_t k, int64_t group) {
+    return codes.is_cuda() && codes.scalar_type() == at::kByte && codes.is_contiguous() && codes.numel() == matrices * t81b200_q4_bytes(rows, k) &&
+           scales.device() == codes.device() && scales.scalar_type() == at::kBFloat16 && scales.is_contiguous() &&
+           scales.numel() == matrices * t81b200_q4_scales(rows, k, (int)group);
+}
+
+Tensor product_q4(const Tensor &codes, const Tensor &scales, int64_t rows, int64_t k, int64_t group, const float *bias, const Rows &x, c10::IntArrayRef shape,
+                  at::ScalarType out_type, const int32_t *offsets, int64_t n_experts) {
+    const c10::Device device = codes.device();
+    OnDevice on(device);
+    Tensor y = at::empty(shape, at::TensorOptions().dtype(out_type).device(device));
+    if (y.numel() == 0) return y;
+    const size_t need = t81b200_linear_q4_workspace_bytes(x.data, x.dtype, x.ld, x.tokens, k);
+    Tensor ws;
+    if (need) ws = at::empty({(int64_t)need}, at::TensorOptions().dtype(at::kByte).device(device));
+    void *const scratch = need ? ws.mutable_data_ptr() : nullptr;
+    const auto *c = codes.const_data_ptr<uint8_t>();
+    const void *const s = scales.const_data_ptr();
+    if (offsets)
+        check(t81b200_experts_q4(c, s, bias, y.mutable_data_ptr(), rows, x.data, x.dtype, x.ld, dtype_code(out_type), rows, x.tokens, k, (int)group, offsets, (int)n_experts, scratch, need,
+                                 stream_of(device)));
+    else
+        check(t81b200_linear_q4(c, s, bias, y.mutable_data_ptr(), rows, x.data, x.dtype, x.ld, dtype_code(out_type), rows, x.tokens, k, (int)group, scratch, need, stream_of(device)));
+    return y;
+}
+
+// Q4Product(codes, scales, rows, k, group): called with (x, bias=None, out_dtype=None) like Product.
+struct Q4ProductObject {
+    PyObject_HEAD
+    vectorcallfunc call;
+    Tensor *codes, *scales;
+    int64_t rows, k, group;
+};
+
+PyObject *q4_product_call(PyObject *self, PyObject *const *args, size_t nargsf, PyObject *kwnames) {
+    HANDLE_TH_ERRORS
+    auto *p = reinterpret_cast<Q4ProductObject *>(self);
+    const Py_ssize_t n = PyVectorcall_NARGS(nargsf);
+    if (kwnames && PyTuple_GET_SIZE(kwnames)) {
+        PyErr_SetString(PyExc_TypeError, "Q4Product takes positional arguments (x, bias, out_dtype)");
+        return nullptr;
+    }
+    if (n < 1 || !plain_tensor(args[0])) Py_RETURN_NONE;
+    const Tensor &x = THPVariable_Unpack(args[0]);
+    const c10::Device device = p->codes->device();
+    Rows rows;
+    if (x.device() != device || x.layout() != at::kStrided || x.is_neg() || !as_rows(x, p->k, rows)) Py_RETURN_NONE;
+    const bool grad = at::GradMode::is_enabled();
+    if (grad && x.requires_grad()) Py_RETURN_NONE;
+    const float *bias = nullptr;
+    if (n > 1 && args[1] != Py_None) {
+        if (!plain_tensor(args[1])) Py_RETURN_NONE;
+        const Tensor &b = THPVariable_Unpack(args[1]);
+        if ((grad && b.requires_grad()) || !float_vector(b, device, p->rows)) Py_RETURN_NONE;
+        bias = b.const_data_ptr<float>();
+    }
+    at::ScalarType out_type = x.scalar_type();
+    if (n > 2 && args[2] != Py_None) {
+        if (!THPDtype_Check(args[2])) Py_RETURN_NONE;
+        out_type = reinterpret_cast<THPDtype *>(args[2])->scalar_type;
+        if (dtype_code(out_type) < 0) Py_RETURN_NONE;
+    }
+    int64_t shape[3] = {x.size(0), x.dim() == 3 ? x.size(1) : p->rows, p->rows};
+    try {
+        return THPVariable_Wrap(product_q4(*p->codes, *p->scales, p->rows, p->k, p->group, bias, rows, c10::IntArrayRef(shape, x.dim()), out_type, nullptr, 0));
+    } catch (const LibraryError &e) {
+        return raise_library_error(e.code);
+    }
+    END_HANDLE_TH_ERRORS
+}
+
+PyObject *q4_product_new(PyTypeObject *type, PyObject *args, PyObject *) {
+    HANDLE_TH_ERRORS
+    PyObject *codes, *scales;
+    long long rows, k, group;
+    if (!PyArg_ParseTuple(args, "OOLLL", &codes, &scales, &rows, &k, &group)) return nullptr;
+    TORCH_CHECK_VALUE(plain_tensor(codes) && plain_tensor(scales), "Q4Product: expected tensors");
+    TORCH_CHECK_VALUE(rows > 0 && k > 0 && holds_q4(THPVariable_Unpack(codes), THPVariable_Unpack(scales), 1, rows, k, group),
+                      "Q4Product: codes and scales do not hold a rows x k matrix");
+    auto *self = reinterpret_cast<Q4ProductObject *>(type->tp_alloc(type, 0));
+    if (!self) return nullptr;
+    self->call = q4_product_call;
+    self->codes = new Tensor(THPVariable_Unpack(codes));
+    self->scales = new Tensor(THPVariable_Unpack(scales));
+    self->rows = rows;
+    self->k = k;
+    self->group = group;
+    return reinterpret_cast<PyObject *>(self);
+    END_HANDLE_TH_ERRORS
+}
+
+void q4_product_dealloc(PyObject *o) {
+    auto *self = reinterpret_cast<Q4ProductObject *>(o);
+    delete self->codes;
+    delete self->scales;
+    Py_TYPE(o)->tp_free(o);
+}
+
+PyTypeObject Q4ProductType = {PyVarObject_HEAD_INIT(nullptr, 0)};
+
+PyObject *pair_of(const Tensor &a, const Tensor &b) {
+    PyObject *result = PyTuple_New(2);
+    if (!result) return nullptr;
+    PyTuple_SET_ITEM(result, 0, THPVariable_Wrap(a));
+    PyTuple_SET_ITEM(result, 1, THPVariable_Wrap(b));
+    return result;
+}
+
+// quantize_q4(w, group) -> (codes, scales); w (rows, cols) or (matrices, rows, cols)
+PyObject *quantize_q4(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 2) return PyErr_Format(PyExc_TypeError, "quantize_q4 takes 2 arguments");
+    Tensor w = tensor_of(args[0]);
+    const int64_t group = PyLong_AsLongLong(args[1]);
+    if (PyErr_Occurred()) return nullptr;
+    TORCH_CHECK_VALUE(w.dim() == 2 || w.dim() == 3, "quantize_q4 expects a 2D matrix or a 3D stack of them");
+    TORCH_CHECK_VALUE(w.is_cuda(), "w must be a CUDA tensor (there is no CPU path)");
+    const int dtype = dtype_code(w.scalar_type());
+    TORCH_CHECK_VALUE(dtype >= 0, "w must be float32, bfloat16 or float16, got ", w.dtype());
+    TORCH_CHECK_VALUE(group == 32 || group == 64 || group == 128, "groups of 32, 64 or 128 columns, not ", group);
+    const int64_t d = w.dim(), matrices = d == 3 ? w.size(0) : 1, rows = w.size(d - 2), cols = w.size(d - 1);
+    const c10::Device device = w.device();
+    OnDevice on(device);
+    if (w.is_neg() || (w.numel() > 0 && ((cols > 1 && w.stride(d - 1) != 1) || (rows > 1 && w.stride(d - 2) < cols)))) w = w.resolve_neg().contiguous();
+    const auto options = at::TensorOptions().device(device);
+    Tensor codes = at::empty({matrices * t81b200_q4_bytes(rows, cols)}, options.dtype(at::kByte));
+    Tensor scales = at::empty({matrices * t81b200_q4_scales(rows, cols, (int)group)}, options.dtype(at::kBFloat16));
+    try {
+        check(t81b200_quantize_q4(w.const_data_ptr(), dtype, matrices, rows, cols, rows > 1 ? w.stride(d - 2) : cols, matrices > 1 ? w.stride(0) : rows * cols, (int)group,
+                                  codes.mutable_data_ptr<uint8_t>(), scales.mutable_data_ptr(), stream_of(device)));
+    } catch (const LibraryError &e) {
+        return raise_library_error(e.code);
+    }
+    return pair_of(codes, scales);
+    END_HANDLE_TH_ERRORS
+}
+
+// dequantize_q4(codes, scales, matrices, rows, cols, group, dtype) -> (matrices, rows, cols)
+PyObject *dequantize_q4(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 7) return PyErr_Format(PyExc_TypeError, "dequantize_q4 takes 7 arguments");
+    const Tensor &codes = tensor_of(args[0]), &scales = tensor_of(args[1]);
+    const int64_t matrices = PyLong_AsLongLong(args[2]), rows = PyLong_AsLongLong(args[3]), cols = PyLong_AsLongLong(args[4]), group = PyLong_AsLongLong(args[5]);
+    if (PyErr_Occurred()) return nullptr;
+    TORCH_CHECK_TYPE(THPDtype_Check(args[6]), "dtype must be a torch.dtype");
+    const at::ScalarType type = reinterpret_cast<THPDtype *>(args[6])->scalar_type;
+    TORCH_CHECK_VALUE(dtype_code(type) >= 0, "dtype must be float32, bfloat16 or float16");
+    TORCH_CHECK_VALUE(matrices >= 0 && rows >= 0 && cols >= 0 && holds_q4(codes, scales, matrices, rows, cols, group), "codes and scales do not hold such matrices");
+    const c10::Device device = codes.device();
+    OnDevice on(device);
+    Tensor out = at::empty({matrices, rows, cols}, at::TensorOptions().dtype(type).device(device));
+    try {
+        check(t81b200_dequantize_q4(codes.const_data_ptr<uint8_t>(), scales.const_data_ptr(), matrices, rows, cols, (int)group, out.mutable_data_ptr(), dtype_code(type), stream_of(device)));
+    } catch (const LibraryError &e) {
+        return raise_library_error(e.code);
+    }
+    return THPVariable_Wrap(out);
+    END_HANDLE_TH_ERRORS
+}
+
+// linear_q4(codes, scales, rows, k, group, x, bias or None, out_dtype or None, offsets or None, n_experts): x (tokens, k) with unit column
+// stride; with offsets (n_experts + 1 int32) the rows are sorted by expert and the weights hold n_experts matrices, the bias (n_experts, rows).
+PyObject *linear_q4(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 10) return PyErr_Format(PyExc_TypeError, "linear_q4 takes 10 arguments");
+    const Tensor &codes = tensor_of(args[0]), &scales = tensor_of(args[1]), &x = tensor_of(args[5]);
+    const int64_t rows = PyLong_AsLongLong(args[2]), k = PyLong_AsLongLong(args[3]), group = PyLong_AsLongLong(args[4]), experts = PyLong_AsLongLong(args[9]);
+    const std::optional<Tensor> bias = optional_tensor(args[6]), offsets = optional_tensor(args[8]);
+    if (PyErr_Occurred()) return nullptr;
+    at::ScalarType out_type = x.scalar_type();
+    if (args[7] != Py_None) {
+        TORCH_CHECK_TYPE(THPDtype_Check(args[7]), "out_dtype must be a torch.dtype");
+        out_type = reinterpret_cast<THPDtype *>(args[7])->scalar_type;
+    }
+    const int64_t matrices = offsets ? experts : 1;
+    TORCH_CHECK_VALUE(rows >= 0 && k >= 0 && matrices >= 1 && holds_q4(codes, scales, matrices, rows, k, group), "linear_q4: codes and scales do not hold such matrices");
+    Rows r;
+    TORCH_CHECK_VALUE(x.dim() == 2 && x.device() == codes.device() && as_rows(x, k, r) && dtype_code(out_type) >= 0,
+                      "linear_q4: x must be (tokens, K) float32, bfloat16 or float16 rows on the weight's device");
+    TORCH_CHECK_VALUE(!bias || float_vector(*bias, codes.device(), matrices * rows), "linear_q4: bias must be float32, contiguous, of the results' width on the weight's device");
+    TORCH_CHECK_VALUE(!offsets || (offsets->scalar_type() == at::kInt && offsets->device() == codes.device() && offsets->is_contiguous() && offsets->numel() == matrices + 1),
+                      "linear_q4: offsets must be int32 (n_experts + 1,) on the weight's device");
+    try {
+        return THPVariable_Wrap(product_q4(codes, scales, rows, k, group, float_ptr(bias), r, {r.tokens, rows}, out_type, offsets ? offsets->const_data_ptr<int32_t>() : nullptr, matrices));
+    } catch (const LibraryError &e) {
+        return raise_library_error(e.code);
+    }
+    END_HANDLE_TH_ERRORS
+}
+
+// ---- rows of a mixture of experts ----
+
+// sort_by_expert(ids, n_experts) -> (order, position, offsets)
+PyObject *sort_by_expert(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 2) return PyErr_Format(PyExc_TypeError, "sort_by_expert takes 2 arguments");
+    Tensor ids = tensor_of(args[0]);
+    const int64_t experts = PyLong_AsLongLong(args[1]);
+    if (PyErr_Occurred()) return nullptr;
+    TORCH_CHECK_VALUE(ids.is_cuda(), "experts must be a CUDA tensor (there is no CPU path)");
+    TORCH_CHECK_VALUE(ids.dim() == 2 && ids.size(1) > 0 && (ids.scalar_type() == at::kLong || ids.scalar_type() == at::kInt), "experts must be int64 or int32 (tokens, slots)");
+    TORCH_CHECK_VALUE(experts >= 1 && experts <= 0x7FFFFFFF, "the number of experts must be positive");
+    const c10::Device device = ids.device();
+    OnDevice on(device);
+    ids = ids.contiguous();
+    const auto options = at::TensorOptions().dtype(at::kInt).device(device);
+    Tensor order = at::empty({ids.numel()}, options), position = at::empty(ids.sizes(), options), offsets = at::empty({experts + 1}, options);
+    try {
+        check(t81b200_sort_by_expert(ids.const_data_ptr(), (int)ids.element_size(), ids.numel(), (int)experts, order.mutable_data_ptr<int32_t>(), position.mutable_data_ptr<int32_t>(),
+                                     offsets.mutable_data_ptr<int32_t>(), stream_of(device)));
+    } catch (const LibraryError &e) {
+        return raise_library_error(e.code);
+    }
+    PyObject *result = PyTuple_New(3);
+    if (!result) return nullptr;
+    PyTuple_SET_ITEM(result, 0, THPVariable_Wrap(order));
+    PyTuple_SET_ITEM(result, 1, THPVariable_Wrap(position));
+    PyTuple_SET_ITEM(result, 2, THPVariable_Wrap(offsets));
+    return result;
+    END_HANDLE_TH_ERRORS
+}
+
+const int32_t *kept_ptr(const Tensor &offsets) { return offsets.const_data_ptr<int32_t>() + (offsets.numel() - 1); }
+
+Tensor gather(const Tensor &x, const Tensor &position, const Tensor &offsets) {
+    OnDevice on(x.device());
+    const Tensor r = with_unit_columns(x);
+    Tensor rows = at::empty({position.numel(), x.size(1)}, x.options());
+    if (rows.numel()) check(t81b200_gather_rows(r.const_data_ptr(), dtype_code(r.scalar_type()), r.size(0) > 1 ? r.stride(0) : r.size(1), r.size(0), position.size(1), r.size(1),
+                                                position.const_data_ptr<int32_t>(), kept_ptr(offsets), rows.mutable_data_ptr(), stream_of(x.device())));
+    return rows;
+}
+
+Tensor combine(const Tensor &rows, const std::optional<Tensor> &weights, const Tensor &position) {
+    OnDevice on(rows.device());
+    const Tensor r = with_unit_columns(rows);
+    Tensor y = at::empty({position.size(0), rows.size(1)}, rows.options());
+    if (y.numel()) check(t81b200_combine_rows(r.const_data_ptr(), dtype_code(r.scalar_type()), r.size(0) > 1 ? r.stride(0) : r.size(1), position.size(0), position.size(1), r.size(1),
+                                              position.const_data_ptr<int32_t>(), weights ? weights->const_data_ptr() : nullptr, weights ? dtype_code(weights->scalar_type()) : T81B200_F32,
+                                              y.mutable_data_ptr(), stream_of(rows.device())));
+    return y;
+}
+
+// Gradients that torch's operations have to compute: those that are differentiated again, and batches under vmap.
+bool recorded(const Tensor &g) { return at::GradMode::is_enabled() || !g.has_storage() || g.is_neg(); }
+
+// The rows of each slot, (tokens, slots, width), zero where a slot has none; differentiable in `rows`.
+Tensor slots_of(const Tensor &rows, const Tensor &position) {
+    const Tensor at = position.clamp_min(0).to(at::kLong).view({-1});
+    const Tensor slots = rows.index_select(0, at).reshape({position.size(0), position.size(1), rows.size(-1)});
+    return at::where((position >= 0).unsqueeze(-1), slots, at::zeros({}, rows.options()));
+}
+
+void check_routing(const Tensor &position, const Tensor &offsets, const c10::Device &device) {
+    TORCH_CHECK_VALUE(position.device() == device && position.scalar_type() == at::kInt && position.dim() == 2 && position.size(1) > 0 && position.is_contiguous() &&
+                          offsets.device() == device && offsets.scalar_type() == at::kInt && offsets.is_contiguous() && offsets.numel() > 1,
+                      "position must be int32 (tokens, slots) and offsets int32 (experts + 1,), both on the rows' device");
+}
+
+struct GatherRows : public torch::autograd::Function<GatherRows> {
+    using Context = torch::autograd::AutogradContext;
+    static Tensor forward(Context *ctx, const Tensor &x, const Tensor &position, const Tensor &offsets) {
+        ctx->save_for_backward({position, offsets});
+        return gather(x, position, offsets);
+    }
+    static torch::autograd::variable_list backward(Context *ctx, torch::autograd::variable_list grads) {
+        return as_python_error([&]() -> torch::autograd::variable_list {
+            const auto saved = ctx->get_saved_variables();  // hooks on saved tensors may hand them back elsewhere and laid out otherwise
+            const Tensor position = saved[0].contiguous();
+            check_routing(position, saved[1].contiguous(), grads[0].device());
+            if (recorded(grads[0])) return {slots_of(grads[0], position).to(at::kFloat).sum(1).to(grads[0].scalar_type()), Tensor(), Tensor()};
+            return {combine(grads[0], std::nullopt, position), Tensor(), Tensor()};
+        });
+    }
+};
+
+struct CombineRows : public torch::autograd::Function<CombineRows> {
+    using Context = torch::autograd::AutogradContext;
+    static Tensor forward(Context *ctx, const Tensor &rows, const std::optional<Tensor> &weights, const Tensor &position, const Tensor &offsets) {
+        ctx->save_for_backward({rows, weights ? *weights : Tensor(), position, offsets});
+        ctx->saved_data["rows"] = rows.requires_grad();
+        ctx->saved_data["weights"] = weights && weights->requires_grad();
+        return combine(rows, weights, position);
+    }
+    static torch::autograd::variable_list backward(Context *ctx, torch::autograd::variable_list grads) {
+        return as_python_error([&] { return gradients(ctx, grads[0]); });
+    }
+    static torch::autograd::variable_list gradients(Context *ctx, const Tensor &grad) {
+        const auto saved = ctx->get_saved_variables();
+        const Tensor position = saved[2].contiguous(), offsets = saved[3].contiguous();
+        check_routing(position, offsets, grad.device());
+        const Tensor rows = with_unit_columns(saved[0]), weights = saved[1].defined() ? saved[1].contiguous() : Tensor();
+        TORCH_CHECK_VALUE(rows.device() == grad.device() && rows.scalar_type() == grad.scalar_type() && rows.size(0) == position.numel() &&
+                              (!weights.defined() || (weights.device() == grad.device() && weights.sizes() == position.sizes() && dtype_code(weights.scalar_type()) >= 0)),
+                          "saved tensors of the combination came back as others");
+        const bool want_rows = ctx->saved_data["rows"].toBool(), want_weights = ctx->saved_data["weights"].toBool();
+        Tensor grad_rows, grad_weights;
+        if (recorded(grad)) {
+            const Tensor kept = position >= 0, g = grad.to(at::kFloat).unsqueeze(1);
+            if (want_rows) {
+                const Tensor none = at::zeros({}, g.options());
+                const Tensor share = weights.defined() ? saved[1].to(at::kFloat) : at::ones(position.sizes(), g.options());
+                const Tensor shares = at::where(kept.unsqueeze(-1), share.unsqueeze(-1) * g, none).reshape({rows.size(0), rows.size(1)});
+                const Tensor at = position.clamp_min(0).to(at::kLong).view({-1});
+                grad_rows = at::zeros({rows.size(0), rows.size(1)}, g.options()).index_add(0, at, shares).to(rows.scalar_type());
+            }
+            if (want_weights) grad_weights = (slots_of(saved[0], position).to(at::kFloat) * g).sum(-1).to(weights.scalar_type());
+            return {grad_rows, grad_weights, Tensor(), Tensor()};
+        }
+        OnDevice on(grad.device());
+        const Tensor g = with_unit_columns(grad);
+        if (want_rows) grad_rows = at::empty({rows.size(0), rows.size(1)}, rows.options());
+        if (want_weights) grad_weights = at::empty(position.sizes(), weights.options());
+        check(t81b200_combine_rows_grad(g.const_data_ptr(), g.size(0) > 1 ? g.stride(0) : g.size(1), rows.const_data_ptr(), dtype_code(rows.scalar_type()),
+                                        rows.size(0) > 1 ? rows.stride(0) : rows.size(1), position.size(0), position.size(1), rows.size(1), position.const_data_ptr<int32_t>(),
+                                        kept_ptr(offsets), weights.defined() ? weights.const_data_ptr() : nullptr, weights.defined() ? dtype_code(weights.scalar_type()) : T81B200_F32,
+                                        want_rows ? grad_rows.mutable_data_ptr() : nullptr, want_weights ? grad_weights.mutable_data_ptr() : nullptr, stream_of(g.device())));
+        return {grad_rows, grad_weights, Tensor(), Tensor()};
+    }
+};
+
+// gather_rows(x, position, offsets), combine_rows(rows, weights or None, position, offsets): recorded for autograd.
+PyObject *gather_rows(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 3) return PyErr_Format(PyExc_TypeError, "gather_rows takes 3 arguments");
+    const Tensor &x = tensor_of(args[0]), &position = tensor_of(args[1]), &offsets = tensor_of(args[2]);
+    TORCH_CHECK_VALUE(x.is_cuda(), "x must be a CUDA tensor (there is no CPU path)");
+    check_routing(position, offsets, x.device());
+    TORCH_CHECK_VALUE(x.dim() == 2 && x.size(0) == position.size(0), "gather_rows: x must have one row per token");
+    TORCH_CHECK_VALUE(dtype_code(x.scalar_type()) >= 0, "x must be float32, bfloat16 or float16, got ", x.dtype());
+    return THPVariable_Wrap(as_python_error([&] { return GatherRows::apply(x.is_neg() ? x.resolve_neg() : x, position, offsets); }));
+    END_HANDLE_TH_ERRORS
+}
+
+PyObject *combine_rows(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 4) return PyErr_Format(PyExc_TypeError, "combine_rows takes 4 arguments");
+    const Tensor &rows = tensor_of(args[0]), &position = tensor_of(args[2]), &offsets = tensor_of(args[3]);
+    std::optional<Tensor> weights = optional_tensor(args[1]);
+    TORCH_CHECK_VALUE(rows.is_cuda(), "rows must be a CUDA tensor (there is no CPU path)");
+    check_routing(position, offsets, rows.device());
+    TORCH_CHECK_VALUE(rows.dim() == 2 && rows.size(0) == position.numel(), "combine_rows: rows must have one row per (token, slot) pair");
+    TORCH_CHECK_VALUE(dtype_code(rows.scalar_type()) >= 0, "rows must be float32, bfloat16 or float16, got ", rows.dtype());
+    if (weights) {
+        TORCH_CHECK_VALUE(weights->sizes() == position.sizes() && weights->device() == rows.device() && dtype_code(weights->scalar_type()) >= 0,
+                          "combine_rows: weights must be float32, bfloat16 or float16 (tokens, slots) on the rows' device");
+        weights = weights->resolve_neg().contiguous();
+    }
+    return THPVariable_Wrap(as_python_error([&] { return CombineRows::apply(rows.is_neg() ? rows.resolve_neg() : rows, weights, position, offsets); }));
+    END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef methods[] = {
     {"quantize_pack", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(quantize_pack)), METH_FASTCALL, nullptr},
     {"tensor_body", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(tensor_body)), METH_FASTCALL, nullptr},
@@ -562,6 +917,12 @@ PyMethodDef methods[] = {
     {"qat_linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(qat_linear)), METH_FASTCALL, nullptr},
     {"linear_t2", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(linear_t2)), METH_FASTCALL, nullptr},
     {"qat_weight_grad", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(qat_weight_grad)), METH_FASTCALL, nullptr},
+    {"quantize_q4", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(quantize_q4)), METH_FASTCALL, nullptr},
+    {"dequantize_q4", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(dequantize_q4)), METH_FASTCALL, nullptr},
+    {"linear_q4", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(linear_q4)), METH_FASTCALL, nullptr},
+    {"sort_by_expert", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(sort_by_expert)), METH_FASTCALL, nullptr},
+    {"gather_rows", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(gather_rows)), METH_FASTCALL, nullptr},
+    {"combine_rows", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(combine_rows)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_t81_torch", nullptr, -1, methods};
@@ -577,9 +938,19 @@ PyMODINIT_FUNC PyInit__t81_torch() {
     ProductType.tp_call = PyVectorcall_Call;
     ProductType.tp_vectorcall_offset = offsetof(ProductObject, call);
     if (PyType_Ready(&ProductType) < 0) return nullptr;
+    Q4ProductType.tp_name = "t81lib_b200._t81_torch.Q4Product";
+    Q4ProductType.tp_basicsize = sizeof(Q4ProductObject);
+    Q4ProductType.tp_flags = Py_TPFLAGS_DEFAULT | Py_TPFLAGS_HAVE_VECTORCALL;
+    Q4ProductType.tp_new = q4_product_new;
+    Q4ProductType.tp_dealloc = q4_product_dealloc;
+    Q4ProductType.tp_call = PyVectorcall_Call;
+    Q4ProductType.tp_vectorcall_offset = offsetof(Q4ProductObject, call);
+    if (PyType_Ready(&Q4ProductType) < 0) return nullptr;
     PyObject *m = PyModule_Create(&module);
     if (!m) return nullptr;
     Py_INCREF(&ProductType);
     PyModule_AddObject(m, "Product", reinterpret_cast<PyObject *>(&ProductType));
+    Py_INCREF(&Q4ProductType);
+    PyModule_AddObject(m, "Q4Product", reinterpret_cast<PyObject *>(&Q4ProductType));
     return m;
 }

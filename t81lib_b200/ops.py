@@ -374,3 +374,48 @@ def qat_weight_grad(grad: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, s
     """``(grad^T x) * slope`` in float32 for token-major ``grad`` (tokens, rows) and ``x`` (tokens, cols) of one dtype;
     slope is 2 where ``|weight / scale| < 0.5`` and 0 elsewhere (t81/qat.py:28-57)."""
     return _capi.native.qat_weight_grad(grad, x, weight, scale)
+
+
+def quantize_q4(w: torch.Tensor, group: int = 128) -> Tuple[torch.Tensor, torch.Tensor]:
+    """A (rows, cols) matrix or a (matrices, rows, cols) stack of them -> 4-bit codes and group scales in the products' order:
+    ``(codes uint8, scales bfloat16)``, both flat.  ``group``: 32, 64 or 128 columns that share a scale."""
+    return _capi.native.quantize_q4(w, group)
+
+
+def dequantize_q4(codes: torch.Tensor, scales: torch.Tensor, rows: int, cols: int, group: int, matrices: int = 1,
+                  dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """The weights that the codes stand for, (matrices, rows, cols); exact in float32 and bfloat16."""
+    return _capi.native.dequantize_q4(codes, scales, matrices, rows, cols, group, dtype)
+
+
+def linear_q4(codes: torch.Tensor, scales: torch.Tensor, M: int, x: torch.Tensor, K: int, group: int, bias: Optional[torch.Tensor] = None,
+              out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """``x @ W.T + bias`` for one 4-bit (M, K) matrix and (tokens, K) activations with unit column stride on its device; ``bias`` is
+    contiguous float32 (M,) or None."""
+    return _capi.native.linear_q4(codes, scales, M, K, group, x, bias, out_dtype, None, 1)
+
+
+def experts_q4(codes: torch.Tensor, scales: torch.Tensor, M: int, x: torch.Tensor, K: int, group: int, offsets: torch.Tensor,
+               bias: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """``linear_q4`` for rows sorted by expert: rows ``offsets[e]`` to ``offsets[e + 1] - 1`` are multiplied by matrix ``e`` of the stack
+    (and get row ``e`` of the bias, (experts, M)); rows from ``offsets[-1]`` on come out as 0.  ``offsets``: int32, on the device,
+    rising from 0, as ``sort_by_expert`` gives it."""
+    return _capi.native.linear_q4(codes, scales, M, K, group, x, bias, out_dtype, offsets, offsets.numel() - 1)
+
+
+def sort_by_expert(experts: torch.Tensor, n_experts: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(tokens, slots) expert ids -> ``(order, position, offsets)``, int32: ``order[p]`` is the flat index (token * slots + slot) of sorted
+    row ``p`` (-1 past the last), ``position`` (tokens, slots) its inverse, and expert ``e`` has the rows ``offsets[e]`` to
+    ``offsets[e + 1] - 1``.  The sort is stable; ids outside 0 .. n_experts - 1 take no part (position -1)."""
+    return _capi.native.sort_by_expert(experts, n_experts)
+
+
+def gather_rows(x: torch.Tensor, position: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
+    """(tokens, width) -> (tokens * slots, width): each token's row at the positions of its slots, 0 from ``offsets[-1]`` on.  Differentiable."""
+    return _capi.native.gather_rows(x, position, offsets)
+
+
+def combine_rows(rows: torch.Tensor, weights: Optional[torch.Tensor], position: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
+    """(tokens * slots, width) -> (tokens, width): the sum over a token's slots of weight times row, in float32, rounded once.  Slots without
+    a position take no part.  Differentiable in ``rows`` and ``weights``."""
+    return _capi.native.combine_rows(rows, weights, position, offsets)

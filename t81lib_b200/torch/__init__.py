@@ -384,4 +384,6 @@ def remove_patches() -> None:
 
 install_patches()
 
-__all__ = ["trit", "TernaryTensor", "TritDtype", "install_patches", "remove_patches"]
+from .q4 import Q4Tensor, Routing, route  # noqa: E402
+
+__all__ = ["trit", "TernaryTensor", "TritDtype", "Q4Tensor", "Routing", "route", "install_patches", "remove_patches"]
