@@ -422,7 +422,8 @@ T81B200_API size_t t81b200_gemm_trit_workspace_bytes(int b_dtype, int layout, in
  *   Codes: tiles of 16 rows x 64 columns, tile (T, c) at byte (T * ceil(cols / 64) + c) * 512; inside, lane l = 4 g + t owns the four
  *   32-bit words at 16 l; bits 4 r + 16 h .. + 3 of word j hold code + 8 of row 16 T + g + 8 (r % 2), column
  *   64 c + 32 (j / 2) + 8 t + 4 (j % 2) + 2 (r / 2) + h.  Scales (bf16): those of tile row T and group u at element
- *   (T * ceil(cols / group) + u) * 16, row r of the tile at 2 (r % 8) + r / 8.  Past the matrix codes and scales are 0.
+ *   (T * (groups + 1) + u) * 16, row r of the tile at 2 (r % 8) + r / 8, groups = ceil(cols / group); block u = groups holds the
+ *   largest magnitude of a row's scales.  Past the matrix codes and scales are 0.
  *   q4_bytes / q4_scales: bytes of the codes and number of scales of one matrix, -1 on bad arguments.
  *   quantize_q4:   `matrices` matrices `matrix_stride` elements apart, row stride ld; their codes and scales lie one behind the other
  *                  (16-byte aligned).

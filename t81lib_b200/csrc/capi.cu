@@ -87,6 +87,7 @@ int gemm_trit_tc_launch(int fmt, int fp32_planes, const uint8_t *A, const float 
 
 int gemm_trit_tc_status(int reset);
 int gemm_wgrad_status(int reset);
+int gemm_q4_tc_status(int reset);
 int gemv_trit_status(int reset);
 int gemv_trit_lut_status(int reset);
 int quantize_pack_status(int reset);
@@ -105,7 +106,9 @@ extern "C" int t81b200_kernel_status(int reset) {
     const int lut = gemv_trit_lut_status(reset);
     const int qp = quantize_pack_status(reset);
     const int wg = gemm_wgrad_status(reset);
+    const int q4 = gemm_q4_tc_status(reset);
     if (wg != 0) return wg;
+    if (q4 != 0) return q4;
     return tc != 0 ? tc : (gv != 0 ? gv : (lut != 0 ? lut : qp));
 }
 

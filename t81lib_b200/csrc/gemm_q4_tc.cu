@@ -1,0 +1,616 @@
+// Products of 4-bit weights (q4.cuh) on the 5th-generation tensor cores (tcgen05), for more activation rows than the streaming kernel
+// serves well: 16-bit activations, one matrix or rows sorted by expert.
+//
+//   D[o][t] = sum_k W[o][k] * x[t][k]     o: output feature (256 per CTA pair, 128 per CTA), t: row of x (up to 256 per tile)
+//
+// The form is gemm_trit_tc.cu's: a pair of CTAs (cta_group::2) works on one tile, each expands its own 128 weight rows into its shared memory
+// and loads half of the tile's activation rows by TMA; the even CTA issues the MMAs, and each CTA keeps its 128 accumulator rows in
+// TMEM (2 x 256 columns, in turn).  What bounds it is shared memory: a 64-deep step writes and reads 16 KB of expanded weights per CTA and
+// writes and reads its half of the activations.
+//
+// Weights: 128 columns (a chunk) of 128 rows are 8 KB of codes and up to 1 KB of scales, one TMA load each; a converter warp per 16 rows
+// turns them into operands of 128-byte rows.  A pair of codes is a shift, an AND-OR and one packed FMA, v * s - 24 s on v = 16 + code + 8, which
+// is exact: a code times its scale is a bf16 number.  Beside fp16 activations the scales of a row are first divided by the power of
+// two in the row's largest, which the result is multiplied by: fp16 holds all of a row's weights then but those 2^-20 below its
+// largest, which lose places that the sums do not have.
+//
+// Rows sorted by expert: every CTA turns the experts' row counts into a list of tiles of its own (a sum over experts in shared memory) and the
+// persistent clusters take tiles of it in turn.  An expert's rows are split evenly into tiles of whole 32 rows; rows of a tile past
+// the expert's last are multiplied and not stored.
+//
+// Few tiles: the contraction is split over S = 2 to 4 pairs of a cluster, whose sums meet in shared memory and are added in rank order.
+//
+// 15 warps per CTA: 0 activations   1 MMA issuer (even CTA), TMEM allocation   2-5 epilogue   6-13 converters   14 codes and scales.
+// Every mbarrier wait is bounded; on expiry the role records a status code and all roles fall through to the common teardown.
+#include "common.cuh"
+#include "launch_order.cuh"
+#include "q4.cuh"
+#include "tma.cuh"
+#include "umma.cuh"
+
+#include <atomic>
+#include <cstring>
+#include <type_traits>
+
+namespace t81b200 {
+
+namespace {
+
+constexpr int BM = 128, BK = 64, CHUNK = 128;
+constexpr int A_ATOM_BYTES = BM * BK * 2, A_CHUNK_BYTES = 2 * A_ATOM_BYTES;  // 16 and 32 KB
+constexpr int RAW_CODES = 8 * 1024, RAW_BYTES = RAW_CODES + 1024;            // a chunk's codes and scales
+constexpr int A_STAGES = 3, RAW_STAGES = 3, B_MAX = 12, MAX_SPLITS = 4;
+constexpr int NUM_THREADS = 15 * 32, EPILOGUE_WARP0 = 2, CONVERTER_WARP0 = 6, CONVERTERS = 8, RAW_WARP = 14;
+constexpr int BARRIER_BYTES = 512, MOST_EXPERTS = 1024;
+constexpr int SMEM_LIMIT = 227 * 1024;
+
+enum { STATUS_PRODUCER = 1, STATUS_MMA = 2, STATUS_EPILOGUE = 3, STATUS_CONVERTER = 4 };
+
+__device__ int g_q4_status = 0;
+
+struct Q4TcParams {
+    const __nv_bfloat16 *scales;
+    const float *bias;
+    void *C;
+    const int32_t *offsets;
+    int64_t ldc;
+    int M, N;                   // output features (of an expert), rows of x
+    int n_experts, row_tiles;   // 16-row tiles of an expert
+    int groups;
+    int m_tiles, n_tiles;       // 256-row pair tiles; tiles of bn rows of x (one matrix)
+    int bn, box_rows;           // most rows of x a tile, a multiple of 32; rows of a TMA box
+    int n_atoms, n_chunks;
+    int splits, b_stages, one_tile, out_bytes;
+    int vec;                    // 16-byte stores are possible
+};
+
+// What a tile is: its expert, first output feature, rows [tok, end) and their number rounded up to 32.
+struct Tile {
+    int expert, row0, tok, end, n;
+};
+
+template <bool EXPERTS> struct TileList;
+template <> struct TileList<false> {
+    __device__ __forceinline__ int build(const Q4TcParams &p) { return p.m_tiles * p.n_tiles; }
+    __device__ __forceinline__ Tile tile(const Q4TcParams &p, int i, int half) const {
+        const int tok = i / p.m_tiles * p.bn;
+        return {0, (i % p.m_tiles * 2 + half) * BM, tok, min(tok + p.bn, p.N), p.bn};
+    }
+};
+template <> struct TileList<true> {
+    int32_t *first, *before;  // [experts + 1] in shared memory: an expert's first row, tiles of experts ahead (in n)
+    // Whole CTA; the offsets are held to rising numbers within the rows whatever they say.
+    __device__ __forceinline__ int build(const Q4TcParams &p) {
+        if (threadIdx.x < 32) {
+            int sum = 0, last = 0;
+            for (int e0 = 0; e0 <= p.n_experts; e0 += 32) {
+                const int e = e0 + (int)threadIdx.x;
+                int at = e <= p.n_experts ? min(max(p.offsets[e], 0), p.N) : 0;
+#pragma unroll
+                for (int d = 1; d < 32; d <<= 1) {
+                    const int o = __shfl_up_sync(0xffffffffu, at, d);
+                    if ((int)threadIdx.x >= d) at = max(at, o);
+                }
+                at = max(at, last);
+                last = __shfl_sync(0xffffffffu, at, 31);
+                if (e <= p.n_experts) first[e] = at;
+            }
+            __syncwarp();
+            for (int e0 = 0; e0 <= p.n_experts; e0 += 32) {
+                const int e = e0 + (int)threadIdx.x, tiles = e < p.n_experts ? (first[e + 1] - first[e] + p.bn - 1) / p.bn : 0;
+                int scan = tiles;
+#pragma unroll
+                for (int d = 1; d < 32; d <<= 1) {
+                    const int o = __shfl_up_sync(0xffffffffu, scan, d);
+                    if ((int)threadIdx.x >= d) scan += o;
+                }
+                if (e <= p.n_experts) before[e] = sum + scan - tiles;
+                sum += __shfl_sync(0xffffffffu, scan, 31);
+            }
+        }
+        __syncthreads();
+        return before[p.n_experts] * p.m_tiles;
+    }
+    __device__ __forceinline__ Tile tile(const Q4TcParams &p, int i, int half) const {
+        const int at = i / p.m_tiles;
+        int lo = 0, hi = p.n_experts;  // the last expert with before[e] <= at that has a tile
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (before[mid] <= at) lo = mid;
+            else hi = mid;
+        }
+        const int tiles = before[lo + 1] - before[lo], rows = first[lo + 1] - first[lo];
+        const int width = ((rows + tiles - 1) / tiles + 31) / 32 * 32;
+        const int tok = first[lo] + (at - before[lo]) * width, end = min(tok + width, first[lo + 1]);
+        return {lo, (i % p.m_tiles * 2 + half) * BM, tok, end, max((end - tok + 31) / 32 * 32, 32)};
+    }
+};
+
+__device__ __forceinline__ bool epilogue_all(bool pred) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 q, %1, 0;\n\t"
+        "barrier.cta.red.and.pred p, 2, 128, q;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(r)
+        : "r"((uint32_t)pred)
+        : "memory");
+    return r != 0;
+}
+
+// One warp's 32 features x 32 rows of x: rows of the result through a buffer of the warp's, 16 bytes a lane, or element by element.
+template <typename CT>
+__device__ __forceinline__ void emit(const Q4TcParams &p, const uint32_t (&v)[32], int feature0, int lane, float scale, float bias, int tok0, int end, CT *stage) {
+    CT *const C = static_cast<CT *>(p.C);
+    if (p.vec && feature0 + 32 <= p.M) {
+        constexpr int PER = 16 / (int)sizeof(CT), PIECES = 32 / PER;  // of a row
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) stage[i * 32 + lane] = from_float<CT>(fmaf(__uint_as_float(v[i]), scale, bias));
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const int at = i * 32 + lane, tok = tok0 + at / PIECES;
+            if (tok < end) *reinterpret_cast<uint4 *>(C + (int64_t)tok * p.ldc + feature0 + at % PIECES * PER) = reinterpret_cast<const uint4 *>(stage)[at];
+        }
+    } else if (feature0 + lane < p.M) {
+        CT *dst = C + (int64_t)tok0 * p.ldc + feature0 + lane;
+#pragma unroll
+        for (int i = 0; i < 32; ++i, dst += p.ldc)
+            if (tok0 + i < end) *dst = from_float<CT>(fmaf(__uint_as_float(v[i]), scale, bias));
+    }
+}
+
+// The power of two in a row's largest scale (1 for a row of zeros), as the exponent bits of a float.
+__device__ __forceinline__ uint32_t row_exponent(const __nv_bfloat16 *scales, int64_t tile, int groups, int r) {
+    const uint32_t bits = (uint32_t)__ldg(reinterpret_cast<const unsigned short *>(scales) + (tile * (groups + 1) + groups) * 16 + 2 * (r & 7) + (r >> 3)) & 0x7F80u;
+    return bits ? bits << 16 : 0x3F800000u;
+}
+
+template <typename T, int GROUP, typename CT, bool EXPERTS>
+__global__ void __launch_bounds__(NUM_THREADS, 1)
+gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_constant__ CUtensorMap map_scales, const __grid_constant__ CUtensorMap map_x,
+                  const __grid_constant__ Q4TcParams p) {
+    constexpr bool F16 = std::is_same<T, __half>::value;
+    constexpr int PER = CHUNK / GROUP;
+    constexpr uint32_t RAW_TX = RAW_CODES + 8 * PER * 32;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ int32_t list[EXPERTS ? 2 * (MOST_EXPERTS + 1) : 1];
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t *gen_base = smem_raw + (base - smem_u32(smem_raw));
+    const uint32_t b_stage_bytes = (uint32_t)p.bn * (BK * 2 / 2);  // this CTA's half of the rows
+    const uint32_t b_off = A_STAGES * A_CHUNK_BYTES, raw_off = b_off + (uint32_t)p.b_stages * b_stage_bytes, out_off = raw_off + RAW_STAGES * RAW_BYTES;
+    const uint32_t bars = base + out_off + (uint32_t)p.out_bytes;
+    auto a_full = [&](int s) { return bars + 8u * s; };
+    auto a_empty = [&](int s) { return bars + 8u * (A_STAGES + s); };
+    auto raw_full = [&](int s) { return bars + 8u * (2 * A_STAGES + s); };
+    auto raw_empty = [&](int s) { return bars + 8u * (2 * A_STAGES + RAW_STAGES + s); };
+    auto acc_full = [&](int s) { return bars + 8u * (2 * A_STAGES + 2 * RAW_STAGES + s); };
+    auto acc_empty = [&](int s) { return bars + 8u * (2 * A_STAGES + 2 * RAW_STAGES + 2 + s); };
+    auto b_full = [&](int s) { return bars + 8u * (2 * A_STAGES + 2 * RAW_STAGES + 4 + s); };
+    auto b_empty = [&](int s) { return bars + 8u * (2 * A_STAGES + 2 * RAW_STAGES + 4 + B_MAX + s); };
+    const uint32_t tmem_slot = bars + 8u * (2 * A_STAGES + 2 * RAW_STAGES + 4 + 2 * B_MAX);
+
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();
+    const int half = (int)(rank & 1u), slice = (int)(rank >> 1);
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < A_STAGES; ++s) { mbar_init(a_full(s), 2 * CONVERTERS); mbar_init(a_empty(s), 1); }
+        for (int s = 0; s < RAW_STAGES; ++s) { mbar_init(raw_full(s), 1); mbar_init(raw_empty(s), CONVERTERS); }
+        for (int s = 0; s < 2; ++s) { mbar_init(acc_full(s), 1); mbar_init(acc_empty(s), 8); }
+        for (int s = 0; s < B_MAX; ++s) { mbar_init(b_full(s), 1); mbar_init(b_empty(s), 1); }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        prefetch_map(&map_codes);
+        prefetch_map(&map_scales);
+        prefetch_map(&map_x);
+    }
+    __syncthreads();
+    if (warp == 1) tmem_alloc_pair(tmem_slot);
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    cluster_barrier();  // the other CTAs' barriers are initialised before anything arrives on them
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    // everything up to here overlaps the end of the kernel ahead; no thread touches global memory before this
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t *>(gen_base + (tmem_slot - base));
+
+    TileList<EXPERTS> tiles;
+    if constexpr (EXPERTS) {
+        tiles.first = list;
+        tiles.before = list + MOST_EXPERTS + 1;
+    }
+    const int total_tiles = tiles.build(p);
+    const int n_clusters = (int)gridDim.x / (2 * p.splits), cluster_id = (int)blockIdx.x / (2 * p.splits);
+    const int c0 = p.n_chunks * slice / p.splits, c1 = p.n_chunks * (slice + 1) / p.splits;
+    const uint16_t pair_mask = (uint16_t)(3u << (rank & ~1u));
+
+    if constexpr (EXPERTS) {  // rows of no expert: a warp each
+        const int kept = tiles.first[p.n_experts];
+        for (int64_t row = (int64_t)kept + blockIdx.x * (NUM_THREADS / 32) + warp; row < p.N; row += (int64_t)gridDim.x * (NUM_THREADS / 32)) {
+            CT *dst = static_cast<CT *>(p.C) + row * p.ldc;
+            if (p.vec && p.M % 8 == 0)
+                for (int i = lane; i < p.M * (int)sizeof(CT) / 16; i += 32) reinterpret_cast<uint4 *>(dst)[i] = make_uint4(0u, 0u, 0u, 0u);
+            else
+                for (int i = lane; i < p.M; i += 32) dst[i] = from_float<CT>(0.0f);
+        }
+        __syncwarp();
+    }
+    // factor of the sums and bias of a feature
+    auto factor_of = [&](const Tile &t, int r) {
+        if (!F16 || t.row0 + r >= p.M) return 1.0f;
+        return __uint_as_float(row_exponent(p.scales, (int64_t)t.expert * p.row_tiles + ((t.row0 + r) >> 4), p.groups, r & 15));
+    };
+    auto bias_of = [&](const Tile &t, int r) { return p.bias && t.row0 + r < p.M ? __ldg(p.bias + (int64_t)t.expert * p.M + t.row0 + r) : 0.0f; };
+
+    if (warp == 0) {
+        // ---------------- this CTA's half of a tile's rows of x ----------------
+        Ring b;
+        bool ok = true;
+        int chunks = 0;
+        for (int i = cluster_id; i < total_tiles && ok; i += n_clusters) {
+            const Tile t = tiles.tile(p, i, half);
+            const int boxes = (t.n / 2 + p.box_rows - 1) / p.box_rows, row = t.tok + half * (t.n / 2);
+            const uint32_t box_bytes = (uint32_t)p.box_rows * (BK * 2);
+            for (int c = c0; c < c1 && ok; ++c, ++chunks) {
+                const int a1 = min(2 * c + 2, p.n_atoms);
+                for (int a = 2 * c; a < a1; ++a) {
+                    ok = mbar_wait(b_empty(b.stage), b.phase ^ 1);
+                    if (!ok) break;
+                    if (elect_one()) {
+                        if (half == 0) mbar_arrive_expect_tx(b_full(b.stage), 2u * (uint32_t)boxes * box_bytes);
+                        const uint32_t dst = base + b_off + (uint32_t)b.stage * b_stage_bytes;
+                        for (int k = 0; k < boxes; ++k) tma_load_2d_pair(dst + (uint32_t)k * box_bytes, &map_x, a * BK, row + k * p.box_rows, b_full(b.stage));
+                    }
+                    __syncwarp();
+                    b.advance(p.b_stages);
+                }
+            }
+        }
+        // The last commits' arrivals come from the pair's issuing CTA; this CTA may not end before they have landed.
+        for (int i = 0; i < p.b_stages && ok; ++i) {
+            ok = mbar_wait(b_empty(b.stage), b.phase ^ 1);
+            b.advance(p.b_stages);
+        }
+        for (int i = chunks; i < chunks + A_STAGES && ok; ++i) ok = mbar_wait(a_empty(i % A_STAGES), ((uint32_t)(i / A_STAGES) & 1u) ^ 1u);
+        if (!ok) give_up(&g_q4_status, STATUS_PRODUCER);
+    } else if (warp == RAW_WARP) {
+        // ---------------- codes and scales ----------------
+        Ring raw;
+        bool ok = true;
+        for (int i = cluster_id; i < total_tiles && ok; i += n_clusters) {
+            const Tile t = tiles.tile(p, i, half);
+            const int y = t.expert * p.row_tiles + (t.row0 >> 4);
+            for (int c = c0; c < c1; ++c) {
+                ok = mbar_wait(raw_empty(raw.stage), raw.phase ^ 1);
+                if (!ok) break;
+                if (elect_one()) {
+                    mbar_arrive_expect_tx(raw_full(raw.stage), RAW_TX);
+                    const uint32_t dst = base + raw_off + (uint32_t)raw.stage * RAW_BYTES;
+                    tma_load_2d(dst, &map_codes, c * 256, y, raw_full(raw.stage));
+                    tma_load_2d(dst + RAW_CODES, &map_scales, c * PER * 16, y, raw_full(raw.stage));
+                }
+                __syncwarp();
+                raw.advance(RAW_STAGES);
+            }
+        }
+        if (!ok) give_up(&g_q4_status, STATUS_PRODUCER);
+    } else if (warp == 1) {
+        // ---------------- MMA issuer ----------------
+        if (half == 0) {
+            Ring a, b;
+            bool ok = true;
+            int it = 0;
+            for (int i = cluster_id; i < total_tiles && ok; i += n_clusters, ++it) {
+                const Tile t = tiles.tile(p, i, half);
+                const int buf = it & 1;
+                const uint32_t idesc = umma_instr_desc(t.n, F16);
+                ok = mbar_wait(acc_empty(buf), ((uint32_t)(it >> 1) & 1u) ^ 1u);
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t d_tmem = tmem_base + (uint32_t)buf * 256u;
+                for (int c = c0; c < c1 && ok; ++c) {
+                    ok = mbar_wait(a_full(a.stage), a.phase);
+                    if (!ok) break;
+                    const int atoms = min(p.n_atoms - 2 * c, 2);
+                    for (int j = 0; j < atoms; ++j) {
+                        ok = mbar_wait(b_full(b.stage), b.phase);
+                        if (!ok) break;
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        if (elect_one()) {
+                            const uint64_t bd = umma_desc_k(base + b_off + (uint32_t)b.stage * b_stage_bytes);
+                            const uint64_t ad = umma_desc_k(base + (uint32_t)a.stage * A_CHUNK_BYTES + (uint32_t)j * A_ATOM_BYTES);
+#pragma unroll
+                            for (int k = 0; k < BK / 16; ++k)
+                                umma_pair(d_tmem, ad + (uint64_t)(2 * k), bd + (uint64_t)(2 * k), idesc, c > c0 || j > 0 || k > 0 ? 1u : 0u);
+                            umma_commit_pair(b_empty(b.stage), pair_mask);
+                        }
+                        __syncwarp();
+                        b.advance(p.b_stages);
+                    }
+                    if (!ok) break;
+                    if (elect_one()) umma_commit_pair(a_empty(a.stage), pair_mask);
+                    __syncwarp();
+                    a.advance(A_STAGES);
+                }
+                if (ok && elect_one()) umma_commit_pair(acc_full(buf), pair_mask);
+                __syncwarp();
+            }
+            if (!ok) give_up(&g_q4_status, STATUS_MMA);
+        }
+    } else if (warp < CONVERTER_WARP0) {
+        // ---------------- epilogue of all but one-tile launches, which are finished below ----------------
+        const int quarter = warp & 3;
+        CT *stage = reinterpret_cast<CT *>(gen_base + out_off) + quarter * 1024;
+        bool ok = true;
+        int it = 0;
+        for (int i = cluster_id; i < total_tiles && ok; i += n_clusters, ++it) {
+            const Tile t = tiles.tile(p, i, half);
+            const int buf = it & 1, r = quarter * 32 + lane;
+            const float factor = p.one_tile ? 1.0f : factor_of(t, r), bias = p.one_tile ? 0.0f : bias_of(t, r);
+            ok = epilogue_all(mbar_wait(acc_full(buf), (uint32_t)(it >> 1) & 1u));
+            if (!ok || p.one_tile) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll 1
+            for (int b = 0; b < t.n / 32; ++b) {
+                uint32_t v[32];
+                tmem_ld32(tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * 256 + b * 32), v);
+                emit<CT>(p, v, t.row0 + quarter * 32, lane, factor, bias, t.tok + b * 32, t.end, stage);
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive_leader(acc_empty(buf));
+        }
+        if (!ok) give_up(&g_q4_status, STATUS_EPILOGUE);
+    } else {
+        // ---------------- converters: 16 rows of a chunk each ----------------
+        const int cw = warp - CONVERTER_WARP0, g = lane >> 2, t4 = lane & 3;
+        const uint32_t swap = (uint32_t)(g & 1);  // lanes of odd rows store their second 32 columns first: eight lanes cover all banks
+        uint32_t off[2];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) off[s] = (uint32_t)(cw * 16 + g) * 128u + (uint32_t)((4 * (s ^ (int)swap) + t4) ^ g) * 16u;
+        Ring a, raw;
+        bool ok = true;
+        for (int i = cluster_id; i < total_tiles && ok; i += n_clusters) {
+            float shrink[2] = {1.0f, 1.0f};
+            if constexpr (F16) {
+                const Tile t = tiles.tile(p, i, half);
+                const int64_t tile = (int64_t)t.expert * p.row_tiles + (t.row0 >> 4) + cw;
+#pragma unroll
+                for (int r = 0; r < 2; ++r)
+                    if (t.row0 + cw * 16 < p.M) shrink[r] = __uint_as_float(0x7F000000u - row_exponent(p.scales, tile, p.groups, g + 8 * r));  // 2^-e
+            }
+            for (int c = c0; c < c1; ++c) {
+                ok = __all_sync(0xffffffffu, mbar_wait(raw_full(raw.stage), raw.phase));
+                if (!ok) break;
+                const uint8_t *src = gen_base + raw_off + raw.stage * RAW_BYTES;
+                uint4 q[2];
+                uint32_t s[PER];
+#pragma unroll
+                for (int k = 0; k < 2; ++k) q[k] = *reinterpret_cast<const uint4 *>(src + cw * 1024 + k * 512 + lane * 16);
+#pragma unroll
+                for (int u = 0; u < PER; ++u) s[u] = *reinterpret_cast<const uint32_t *>(src + RAW_CODES + (cw * PER + u) * 32 + g * 4);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(raw_empty(raw.stage));
+                raw.advance(RAW_STAGES);
+                // a row's scale twice in a word, and -24 times it
+                uint32_t s2[2][PER], n2[2][PER];
+#pragma unroll
+                for (int u = 0; u < PER; ++u)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        if constexpr (F16) {
+                            const __half h = __float2half_rn(__uint_as_float(r ? s[u] & 0xFFFF0000u : s[u] << 16) * shrink[r]);
+                            const __half2 hh(h, h), nn = __hmul2(hh, __half2(__float2half_rn(-24.0f), __float2half_rn(-24.0f)));
+                            s2[r][u] = *reinterpret_cast<const uint32_t *>(&hh);
+                            n2[r][u] = *reinterpret_cast<const uint32_t *>(&nn);
+                        } else {
+                            s2[r][u] = __byte_perm(s[u], s[u], r ? 0x3232 : 0x1010);
+                            n2[r][u] = fma_bf16x2(s2[r][u], 0xC1C0C1C0u, 0x80008000u);
+                        }
+                    }
+                ok = __all_sync(0xffffffffu, mbar_wait(a_empty(a.stage), a.phase ^ 1));
+                if (!ok) break;
+                uint8_t *dst = gen_base + a.stage * A_CHUNK_BYTES;
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const uint32_t w[4] = {swap ? q[k].z : q[k].x, swap ? q[k].w : q[k].y, swap ? q[k].x : q[k].z, swap ? q[k].y : q[k].w};
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)  // the lane's first and second half to be stored
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            uint32_t sc, nc;
+                            if constexpr (GROUP == 32) {
+                                sc = swap ? s2[r][2 * k + 1 - h] : s2[r][2 * k + h];
+                                nc = swap ? n2[r][2 * k + 1 - h] : n2[r][2 * k + h];
+                            } else {
+                                sc = s2[r][GROUP == 64 ? k : 0];
+                                nc = n2[r][GROUP == 64 ? k : 0];
+                            }
+                            uint32_t o[4];
+#pragma unroll
+                            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                                for (int pr = 0; pr < 2; ++pr) {
+                                    const uint32_t x = w[2 * h + j];
+                                    const uint32_t v = r == 0 ? (pr == 0 ? Q4Decode<T>::template biased<0>(x) : Q4Decode<T>::template biased<2>(x))
+                                                              : (pr == 0 ? Q4Decode<T>::template biased<1>(x) : Q4Decode<T>::template biased<3>(x));
+                                    o[2 * j + pr] = Q4Decode<T>::scaled(v, sc, nc);
+                                }
+                            *reinterpret_cast<uint4 *>(dst + k * A_ATOM_BYTES + off[h] + r * 1024) = make_uint4(o[0], o[1], o[2], o[3]);
+                        }
+                }
+                // generic-proxy writes must be visible to the tensor core's async proxy
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive_leader(a_full(a.stage));
+                a.advance(A_STAGES);
+            }
+        }
+        if (!ok) give_up(&g_q4_status, STATUS_CONVERTER);
+    }
+    __syncwarp();
+
+    if (p.one_tile) {
+        // Three groups of four warps take the tile's 32-row blocks in turn; what they stage goes into the activation ring, idle by now.  With
+        // splits > 1 block b is finished by slice b % splits, the others write theirs into its shared memory first (the weight ring).
+        const int group = (warp - EPILOGUE_WARP0) >> 2, quarter = warp & 3, S = p.splits, blocks = p.bn / 32;
+        const bool worker = warp >= EPILOGUE_WARP0 && warp < RAW_WARP;
+        const Tile t = tiles.tile(p, cluster_id, half);
+        const uint32_t r = (uint32_t)(quarter * 32 + lane);
+        const uint32_t t_lane = tmem_base + ((uint32_t)(quarter * 32) << 16);
+        const float factor = factor_of(t, (int)r), bias = bias_of(t, (int)r);
+        __syncthreads();
+        if (S > 1) cluster_barrier();
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (S > 1) {
+            if (worker)
+                for (int b = group; b < blocks; b += 3) {
+                    const int to = b % S;
+                    if (to == slice) continue;
+                    uint32_t v[32];
+                    tmem_ld32(t_lane + (uint32_t)(b * 32), v);
+                    push_partial(v, base + partial_slot(b, S, slice, to) * 16384u + r * 4u, (uint32_t)(2 * to + half));
+                }
+            __syncthreads();
+            cluster_barrier();
+        }
+        if (worker) {
+            CT *stage = reinterpret_cast<CT *>(gen_base + b_off) + (group * 4 + quarter) * 1024;
+            for (int b = slice + S * group; b < blocks; b += 3 * S) {
+                uint32_t v[32];
+                tmem_ld32(t_lane + (uint32_t)(b * 32), v);
+                if (S > 1) fold_partials(v, gen_base, b, S, slice, r);
+                emit<CT>(p, v, t.row0 + quarter * 32, lane, factor, bias, t.tok + b * 32, t.end, stage);
+            }
+        }
+    }
+    // ---------------- teardown: no CTA leaves while its peer may still arrive on its barriers or read its operands ----------------
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    cluster_barrier();
+    if (warp == 1) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        tmem_free_pair(tmem_base);
+    }
+}
+
+// Time of a 64-deep step at n columns, in units of 1.7 ns (gemm_trit_tc.cu's figures).
+double step_cost(int n) {
+    constexpr double cost[8] = {115, 119, 122, 125, 130, 153, 169, 187};  // 32, 64, .. 256 columns
+    return cost[n / 32 - 1];
+}
+
+template <typename T, int GROUP, typename CT, bool EXPERTS>
+int launch(const CUtensorMap &mc, const CUtensorMap &ms, const CUtensorMap &mx, const Q4TcParams &p, int clusters, size_t smem, cudaStream_t st) {
+    auto kern = gemm_q4_tc_kernel<T, GROUP, CT, EXPERTS>;
+    constexpr int most = SMEM_LIMIT - (EXPERTS ? 2 * (MOST_EXPERTS + 1) * 4 + 256 : 64);
+    static std::atomic<bool> configured[64];
+    int dev = 0;
+    T81_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64 || !configured[dev].load(std::memory_order_acquire)) {
+        T81_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+        if (dev >= 0 && dev < 64) configured[dev].store(true, std::memory_order_release);
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(clusters * 2 * p.splits));
+    cfg.blockDim = dim3(NUM_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)(2 * p.splits);
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    T81_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, mc, ms, mx, p));
+    return T81B200_OK;
+}
+
+}  // namespace
+
+int gemm_q4_tc_status(int reset) {
+    int v = 0;
+    if (cudaMemcpyFromSymbol(&v, g_q4_status, sizeof v) != cudaSuccess) return T81B200_ECUDA;
+    if (reset && v != 0) {
+        const int zero = 0;
+        if (cudaMemcpyToSymbol(g_q4_status, &zero, sizeof zero) != cudaSuccess) return T81B200_ECUDA;
+    }
+    return v;
+}
+
+// x: 16-bit rows on 16-byte boundaries, kx >= K columns of them readable (zeros past K), N rows.  Arguments are checked by the caller.
+int gemm_q4_tc_launch(const uint8_t *codes, const void *scales, const float *bias, void *C, int64_t M, const void *x, bool f16, int64_t ldx, int c_dtype, int64_t ldc, int64_t N,
+                      int64_t K, int group, const int32_t *offsets, int n_experts, cudaStream_t st) {
+    Q4TcParams p;
+    memset(&p, 0, sizeof p);
+    const int experts = offsets ? n_experts : 1;
+    p.scales = static_cast<const __nv_bfloat16 *>(scales); p.bias = bias; p.C = C; p.offsets = offsets; p.ldc = ldc;
+    p.M = (int)M; p.N = (int)N; p.n_experts = experts;
+    p.row_tiles = (int)q4_row_tiles(M); p.groups = (int)q4_groups(K, group);
+    p.m_tiles = (int)((M + 255) / 256);
+    p.n_atoms = (int)((K + BK - 1) / BK); p.n_chunks = (int)((K + CHUNK - 1) / CHUNK);
+    p.splits = 1;
+    p.vec = reinterpret_cast<uintptr_t>(C) % 16 == 0 && ldc * (int64_t)dtype_size(c_dtype) % 16 == 0;
+    const int resident = resident_pair_clusters(1);
+    int clusters;
+    if (offsets) {
+        // rows of an expert go evenly into tiles of at most 256
+        p.bn = 256;
+        p.box_rows = 16;
+        const int64_t most = (N / p.bn + (N < experts ? N : experts)) * p.m_tiles;
+        clusters = (int)(most < resident ? (most < 1 ? 1 : most) : resident);
+    } else {
+        const int64_t least = (N + 255) / 256, most = least + 8;
+        double best_t = 1e30;
+        for (int64_t want = least; want <= most && want <= (N + 31) / 32; ++want) {
+            const int bn = (int)(((N + want - 1) / want + 31) / 32 * 32);
+            const int64_t n_tiles = (N + bn - 1) / bn, tiles = p.m_tiles * n_tiles;
+            for (int s = 1; s <= MAX_SPLITS; ++s) {
+                const int fit = resident_pair_clusters(s);
+                if (s > p.n_chunks || (s > 1 && tiles > fit)) continue;
+                const double t = (double)((tiles + fit - 1) / fit) * (2.0 * (double)((p.n_chunks + s - 1) / s) * step_cost(bn) + 400.0) + 3.0 * bn + (s > 1 ? 1300.0 + 3.0 * bn : 0.0);
+                if (t < best_t) { best_t = t; p.bn = bn; p.n_tiles = (int)n_tiles; p.splits = s; }
+            }
+        }
+        p.box_rows = p.bn / 2;
+        const int tiles = p.m_tiles * p.n_tiles;
+        p.one_tile = p.splits > 1 || tiles <= resident ? 1 : 0;
+        clusters = p.one_tile ? tiles : resident;
+    }
+    p.out_bytes = p.one_tile ? 0 : 4 * 1024 * (int)dtype_size(c_dtype);
+    const int limit = SMEM_LIMIT - (offsets ? 2 * (MOST_EXPERTS + 1) * 4 + 256 : 64);
+    const int fixed = A_STAGES * A_CHUNK_BYTES + RAW_STAGES * RAW_BYTES + p.out_bytes + BARRIER_BYTES + 1024, stage = p.bn * BK;
+    const int fit = (limit - fixed) / stage;
+    p.b_stages = fit > B_MAX ? B_MAX : fit;
+    const size_t smem = (size_t)fixed + (size_t)p.b_stages * stage;
+    CUtensorMap mc, ms, mx;
+    const int64_t tiles16 = (int64_t)experts * p.row_tiles, ktiles = q4_col_tiles(K);
+    if (int rc = make_map_2d(&mc, CU_TENSOR_MAP_DATA_TYPE_UINT32, codes, (uint64_t)ktiles * 128, (uint64_t)tiles16, (uint64_t)ktiles * kQ4TileBytes, 256, 8, CU_TENSOR_MAP_SWIZZLE_NONE)) return rc;
+    if (int rc = make_map_2d(&ms, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, scales, (uint64_t)(p.groups + 1) * 16, (uint64_t)tiles16, (uint64_t)(p.groups + 1) * 32, (uint32_t)(CHUNK / group) * 16, 8,
+                             CU_TENSOR_MAP_SWIZZLE_NONE))
+        return rc;
+    if (int rc = make_map_2d(&mx, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, x, (uint64_t)K, (uint64_t)N, (uint64_t)ldx * 2, BK, (uint32_t)p.box_rows,
+                             CU_TENSOR_MAP_SWIZZLE_128B))
+        return rc;
+    auto go = [&](auto t, auto g, auto ct, auto e) { return launch<decltype(t), decltype(g)::value, decltype(ct), decltype(e)::value>(mc, ms, mx, p, clusters, smem, st); };
+    auto by_experts = [&](auto t, auto g, auto ct) { return offsets ? go(t, g, ct, std::true_type{}) : go(t, g, ct, std::false_type{}); };
+    auto by_out = [&](auto t, auto g) {
+        switch (c_dtype) {
+            case T81B200_F32: return by_experts(t, g, float{});
+            case T81B200_BF16: return by_experts(t, g, __nv_bfloat16{});
+            default: return by_experts(t, g, __half{});
+        }
+    };
+    auto by_group = [&](auto t) {
+        if (group == 32) return by_out(t, std::integral_constant<int, 32>{});
+        if (group == 64) return by_out(t, std::integral_constant<int, 64>{});
+        return by_out(t, std::integral_constant<int, 128>{});
+    };
+    return f16 ? by_group(__half{}) : by_group(__nv_bfloat16{});
+}
+
+}  // namespace t81b200

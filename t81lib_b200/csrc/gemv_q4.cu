@@ -19,6 +19,10 @@
 
 namespace t81b200 {
 
+// gemm_q4_tc.cu
+int gemm_q4_tc_launch(const uint8_t *codes, const void *scales, const float *bias, void *C, int64_t M, const void *x, bool f16, int64_t ldx, int c_dtype, int64_t ldc, int64_t N,
+                      int64_t K, int group, const int32_t *offsets, int n_experts, cudaStream_t st);
+
 namespace {
 
 struct Q4Params {
@@ -132,7 +136,7 @@ __global__ void __launch_bounds__(512) gemv_q4_kernel(const __grid_constant__ Q4
                     q[r][c] = there && 2 * unit + c < p.col_tiles ? load_codes(codes + ((tile0 + r) * p.col_tiles + 2 * unit + c) * kQ4TileBytes + lane * 16) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
                 for (int i = 0; i < PER; ++i)
-                    s[r][i] = there && unit * PER + i < p.groups ? load_scales(scales + ((tile0 + r) * p.groups + unit * PER + i) * 16 + 2 * g) : 0u;
+                    s[r][i] = there && unit * PER + i < p.groups ? load_scales(scales + ((tile0 + r) * (p.groups + 1) + unit * PER + i) * 16 + 2 * g) : 0u;
             }
         };
         uint4 q[RT][2], q_next[RT][2];
@@ -283,6 +287,8 @@ int product_q4(const char *name, const uint8_t *codes, const void *scales, const
         p.ldx = p.kx = staged_row(K);
         p.plane_elems = N * p.ldx;
     }
+    if (b_dtype != T81B200_F32 && K > 0 && n_experts <= 1024 && N >= (offsets ? 8 * (int64_t)n_experts : 33))
+        return gemm_q4_tc_launch(codes, scales, bias, C, M, p.x, b_dtype == T81B200_F16, p.ldx, c_dtype, ldc, N, K, group, offsets, n_experts, st);
     if (b_dtype == T81B200_F32) return launch_shape<__nv_bfloat16, 3>(p, group, c_dtype, st);
     return b_dtype == T81B200_BF16 ? launch_shape<__nv_bfloat16, 1>(p, group, c_dtype, st) : launch_shape<__half, 1>(p, group, c_dtype, st);
 }

@@ -9,7 +9,8 @@
 //     row 16 T + g + 8 (r % 2),  column 64 c + 32 (j / 2) + 8 t + 4 (j % 2) + 2 (r / 2) + h.
 // Words 0, 1 are columns 0 .. 31 and words 2, 3 columns 32 .. 63, so that no multiply mixes two groups, and a lane's eight columns of either
 // half are 16 bytes of an activation row or of an operand tile.  Scales of tile row T and group u: 16 bf16 numbers at
-// (T * ceil(cols / group) + u) * 16, row r of the tile at 2 (r % 8) + r / 8: a lane's two rows are one word.
+// (T * (groups + 1) + u) * 16, row r of the tile at 2 (r % 8) + r / 8: a lane's two rows are one word.  Behind the groups' come the
+// rows' largest magnitudes of a scale: kernels that hold weights in fp16 divide a row by the power of two in it.
 // Rows and columns past the matrix have code 0 (bits 8) and scale 0.
 #pragma once
 
@@ -34,6 +35,8 @@ template <> struct Q4Decode<__nv_bfloat16> {
         return (x & 0x00780078u) | 0x41804180u;
     }
     static __device__ __forceinline__ uint32_t minus24(uint32_t v) { return fma_bf16x2(v, 0x3F803F80u, 0xC1C0C1C0u); }
+    // (v - 24) s for n = -24 s (7 bits): one rounding, of an exact result
+    static __device__ __forceinline__ uint32_t scaled(uint32_t v, uint32_t s, uint32_t n) { return fma_bf16x2(v, s, n); }
 };
 template <> struct Q4Decode<__half> {
     template <int R> static __device__ __forceinline__ uint32_t biased(uint32_t w) {
@@ -43,6 +46,11 @@ template <> struct Q4Decode<__half> {
     static __device__ __forceinline__ uint32_t minus24(uint32_t v) {
         uint32_t d;
         asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(v), "r"(0xCE00CE00u));
+        return d;
+    }
+    static __device__ __forceinline__ uint32_t scaled(uint32_t v, uint32_t s, uint32_t n) {
+        uint32_t d;
+        asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(v), "r"(s), "r"(n));
         return d;
     }
 };

@@ -72,74 +72,90 @@ __device__ __forceinline__ uint32_t code_of(float w, float s, float inverse) {
     return (uint32_t)(__float2int_rn(fminf(fmaxf(q, -8.0f), 7.0f)) + 8);
 }
 
+// A block takes 16 rows, its warps units of 128 columns in turn.
 template <typename T, int GROUP, bool VEC>
 __global__ void __launch_bounds__(kThreads) quantize_q4_kernel(const T *__restrict__ w, int64_t rows, int64_t cols, int64_t ld, int64_t matrix_stride,
                                                                uint4 *__restrict__ codes, __nv_bfloat16 *__restrict__ scales) {
+    __shared__ float most[kWarps][16];
     const int64_t row_tiles = q4_row_tiles(rows), col_tiles = q4_col_tiles(cols), groups = q4_groups(cols, GROUP), units = (cols + 127) / 128;
-    const int64_t warp = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5), per_matrix = row_tiles * units;
-    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int64_t matrix = blockIdx.y, T16 = warp / units, unit = warp % units;
-    if (warp >= per_matrix) return;
-    const int64_t out_tile = matrix * row_tiles + T16;
-    float v[2][2][2][8];  // [tile][half of its columns][row of the lane]
-#pragma unroll
-    for (int c = 0; c < 2; ++c)
-#pragma unroll
-        for (int half = 0; half < 2; ++half)
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const int64_t row = 16 * T16 + g + 8 * r, col = unit * 128 + 64 * c + 32 * half + 8 * t;
-                load8<T, VEC>(w + matrix * matrix_stride + row * ld + col, row < rows ? cols - col : 0, v[c][half][r]);
-            }
-    float m[2][2][2];
-#pragma unroll
-    for (int c = 0; c < 2; ++c)
-#pragma unroll
-        for (int half = 0; half < 2; ++half)
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                float most = v[c][half][r][0];
-#pragma unroll
-                for (int i = 1; i < 8; ++i) most = larger(most, v[c][half][r][i]);
-                m[c][half][r] = largest_of_lanes(most, t);
-            }
-    float s[2][2][2];
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-        if (GROUP >= 64)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) m[c][0][r] = m[c][1][r] = larger(m[c][0][r], m[c][1][r]);
-        if (GROUP == 128) m[0][0][r] = m[0][1][r] = m[1][0][r] = m[1][1][r] = larger(m[0][0][r], m[1][0][r]);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int64_t matrix = blockIdx.y, T16 = blockIdx.x, out_tile = matrix * row_tiles + T16;
+    float largest[2] = {0.0f, 0.0f};  // of the lane's rows
+    for (int64_t unit = warp; unit < units; unit += kWarps) {
+        float v[2][2][2][8];  // [tile][half of its columns][row of the lane]
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
-            for (int half = 0; half < 2; ++half) s[c][half][r] = scale_of(m[c][half][r]);
-    }
-    constexpr int PER = 128 / GROUP;  // groups of the 128 columns; lane t == 0 of a row writes them
-    if (t == 0) {
+            for (int half = 0; half < 2; ++half)
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int64_t u = unit * PER + i;
-            if (u >= groups) break;
-            const int c = i * GROUP / 64, half = i * GROUP % 64 / 32;
-            const __nv_bfloat162 pair(__float2bfloat16_rn(s[c][half][0]), __float2bfloat16_rn(s[c][half][1]));
-            *reinterpret_cast<uint32_t *>(scales + (out_tile * groups + u) * 16 + 2 * g) = bf162_bits(pair);
+                for (int r = 0; r < 2; ++r) {
+                    const int64_t row = 16 * T16 + g + 8 * r, col = unit * 128 + 64 * c + 32 * half + 8 * t;
+                    load8<T, VEC>(w + matrix * matrix_stride + row * ld + col, row < rows ? cols - col : 0, v[c][half][r]);
+                }
+        float m[2][2][2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    float x = v[c][half][r][0];
+#pragma unroll
+                    for (int i = 1; i < 8; ++i) x = larger(x, v[c][half][r][i]);
+                    m[c][half][r] = largest_of_lanes(x, t);
+                }
+        float s[2][2][2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            if (GROUP >= 64)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) m[c][0][r] = m[c][1][r] = larger(m[c][0][r], m[c][1][r]);
+            if (GROUP == 128) m[0][0][r] = m[0][1][r] = m[1][0][r] = m[1][1][r] = larger(m[0][0][r], m[1][0][r]);
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    s[c][half][r] = scale_of(m[c][half][r]);
+                    largest[r] = fmaxf(largest[r], fabsf(s[c][half][r]));
+                }
+        }
+        constexpr int PER = 128 / GROUP;  // groups of the 128 columns; lane t == 0 of a row writes them
+        if (t == 0) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const int64_t u = unit * PER + i;
+                if (u >= groups) break;
+                const int c = i * GROUP / 64, half = i * GROUP % 64 / 32;
+                const __nv_bfloat162 pair(__float2bfloat16_rn(s[c][half][0]), __float2bfloat16_rn(s[c][half][1]));
+                *reinterpret_cast<uint32_t *>(scales + (out_tile * (groups + 1) + u) * 16 + 2 * g) = bf162_bits(pair);
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            if (unit * 2 + c >= col_tiles) break;
+            uint32_t word[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const float scale = s[c][half][r], inverse = scale != 0.0f ? 1.0f / scale : 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)  // column 4 (j % 2) + 2 (register / 2) + h of the lane's eight
+                        word[2 * half + (i >> 2)] |= (scale != 0.0f ? code_of(v[c][half][r][i], scale, inverse) : 8u) << (4 * (r + 2 * ((i >> 1) & 1)) + 16 * (i & 1));
+                }
+            codes[(out_tile * col_tiles + unit * 2 + c) * 32 + lane] = make_uint4(word[0], word[1], word[2], word[3]);
         }
     }
+    if (t == 0) {
+        most[warp][2 * g] = largest[0];
+        most[warp][2 * g + 1] = largest[1];
+    }
+    __syncthreads();
+    if (threadIdx.x < 16) {
+        float x = most[0][threadIdx.x];
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-        if (unit * 2 + c >= col_tiles) break;
-        uint32_t word[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
-        for (int half = 0; half < 2; ++half)
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const float scale = s[c][half][r], inverse = scale != 0.0f ? 1.0f / scale : 0.0f;
-#pragma unroll
-                for (int i = 0; i < 8; ++i)  // column 4 (j % 2) + 2 (register / 2) + h of the lane's eight
-                    word[2 * half + (i >> 2)] |= (scale != 0.0f ? code_of(v[c][half][r][i], scale, inverse) : 8u) << (4 * (r + 2 * ((i >> 1) & 1)) + 16 * (i & 1));
-            }
-        codes[(out_tile * col_tiles + unit * 2 + c) * 32 + lane] = make_uint4(word[0], word[1], word[2], word[3]);
+        for (int i = 1; i < kWarps; ++i) x = fmaxf(x, most[i][threadIdx.x]);
+        scales[(out_tile * (groups + 1) + groups) * 16 + threadIdx.x] = __float2bfloat16_rn(x);
     }
 }
 
@@ -159,7 +175,7 @@ __global__ void __launch_bounds__(kThreads) dequantize_q4_kernel(const uint4 *__
     for (int half = 0; half < 2; ++half) {
         const int64_t col = 64 * c + 32 * half + 8 * t;
         if (col >= cols) continue;
-        const uint32_t pair = *reinterpret_cast<const uint32_t *>(scales + (all_T * groups + col / group) * 16 + 2 * g);
+        const uint32_t pair = *reinterpret_cast<const uint32_t *>(scales + (all_T * (groups + 1) + col / group) * 16 + 2 * g);
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
             const int64_t row = 16 * T16 + g + 8 * r;
@@ -183,7 +199,7 @@ __global__ void __launch_bounds__(kThreads) dequantize_q4_kernel(const uint4 *__
 
 template <typename T>
 int launch_quantize(const void *w, int64_t matrices, int64_t rows, int64_t cols, int64_t ld, int64_t matrix_stride, int group, uint8_t *codes, void *scales, cudaStream_t st) {
-    const int64_t blocks = (q4_row_tiles(rows) * ((cols + 127) / 128) + kWarps - 1) / kWarps;
+    const int64_t blocks = q4_row_tiles(rows);
     if (blocks > 0x7FFFFFFF || matrices > 65535) return fail(T81B200_ELIMIT, "quantize_q4: matrix too large");
     const bool vec = reinterpret_cast<uintptr_t>(w) % 16 == 0 && ld * sizeof(T) % 16 == 0 && matrix_stride * sizeof(T) % 16 == 0;
     const dim3 grid((unsigned)blocks, (unsigned)matrices);
@@ -219,7 +235,7 @@ extern "C" int64_t t81b200_q4_bytes(int64_t rows, int64_t cols) {
 
 extern "C" int64_t t81b200_q4_scales(int64_t rows, int64_t cols, int group) {
     if (rows < 0 || cols < 0 || !q4_group_ok(group)) return -1;
-    return q4_row_tiles(rows) * q4_groups(cols, group) * 16;
+    return q4_row_tiles(rows) * (q4_groups(cols, group) + 1) * 16;
 }
 
 extern "C" int t81b200_quantize_q4(const void *w, int w_dtype, int64_t matrices, int64_t rows, int64_t cols, int64_t ld, int64_t matrix_stride, int group, uint8_t *codes,

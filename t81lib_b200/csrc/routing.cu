@@ -110,9 +110,6 @@ __global__ void __launch_bounds__(kSortThreads, 1) sort_by_expert_kernel(const I
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 
-// `bytes` bytes of a row by one warp, in pieces of P.
-template <typename P> __device__ __forceinline__ P zero_piece() { return P{}; }
-
 // Tokens first (row t of x to its slots), then the rows past the last expert's, which are zero.
 template <typename P>
 __global__ void __launch_bounds__(kThreads) gather_rows_kernel(const uint8_t *__restrict__ x, int64_t ld, int64_t tokens, int top, int64_t pieces, const int32_t *__restrict__ position,
@@ -127,7 +124,7 @@ __global__ void __launch_bounds__(kThreads) gather_rows_kernel(const uint8_t *__
             if (p >= 0 && p < n) reinterpret_cast<P *>(rows)[p * pieces + chunk] = v;
         }
     }
-    for (int64_t p = (int64_t)max(*kept, 0) + blockIdx.x; p < n; p += gridDim.x) reinterpret_cast<P *>(rows)[p * pieces + chunk] = zero_piece<P>();
+    for (int64_t p = (int64_t)max(*kept, 0) + blockIdx.x; p < n; p += gridDim.x) reinterpret_cast<P *>(rows)[p * pieces + chunk] = P{};
 }
 
 template <typename T, int N> struct alignas(sizeof(T) * N) Piece { T v[N]; };

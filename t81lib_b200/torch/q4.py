@@ -55,7 +55,8 @@ class Q4Tensor:
     def group_scales(self) -> torch.Tensor:
         """bfloat16 (..., rows, groups)."""
         rows, cols = self.shape[-2:]
-        s = self.scales.view(*self.shape[:-2], (rows + 15) // 16, (cols + self.group - 1) // self.group, 8, 2)
+        groups = (cols + self.group - 1) // self.group
+        s = self.scales.view(*self.shape[:-2], (rows + 15) // 16, groups + 1, 8, 2)[..., :groups, :, :]
         # row r of a tile lies at [r % 8, r / 8]
         return s.movedim((-1, -2), (-3, -2)).flatten(-4, -2)[..., :rows, :].contiguous()
 

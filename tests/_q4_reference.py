@@ -24,7 +24,7 @@ def pack(codes, scales, group):
     """One matrix as the header states the layout: 32-bit words of codes (as int64) and the bf16 scales."""
     rows, cols = codes.shape
     tiles, wide, groups = (rows + 15) // 16, (cols + 63) // 64, (cols + group - 1) // group
-    out, out_scales = torch.full((tiles * wide * 128,), 0x88888888, dtype=torch.int64), torch.zeros(tiles * groups * 16, dtype=torch.float64)
+    out, out_scales = torch.full((tiles * wide * 128,), 0x88888888, dtype=torch.int64), torch.zeros(tiles * (groups + 1) * 16, dtype=torch.float64)
     r, k = torch.meshgrid(torch.arange(rows), torch.arange(cols), indexing="ij")
     rr, kk = r % 16, k % 64
     t, j, pair, h = kk % 32 // 8, 2 * (kk // 32) + kk % 8 // 4, kk % 4 // 2, kk % 2
@@ -35,7 +35,9 @@ def pack(codes, scales, group):
     flips = ((8 ^ (codes.cpu() + 8)) << shift).flatten()
     out ^= torch.zeros_like(out).index_add_(0, word.flatten(), flips)  # distinct bits of a word add up
     r, u = torch.meshgrid(torch.arange(rows), torch.arange(groups), indexing="ij")
-    out_scales[((r // 16) * groups + u) * 16 + 2 * (r % 8) + r % 16 // 8] = scales.cpu()
+    out_scales[((r // 16) * (groups + 1) + u) * 16 + 2 * (r % 8) + r % 16 // 8] = scales.cpu()
+    r = torch.arange(rows)
+    out_scales[((r // 16) * (groups + 1) + groups) * 16 + 2 * (r % 8) + r % 16 // 8] = scales.cpu().abs().amax(1)
     return out, out_scales.to(torch.bfloat16)
 
 

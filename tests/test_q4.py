@@ -12,7 +12,8 @@ import _q4_reference as ref
 def dev(lib_built):
     from t81lib_b200 import _capi
     assert _capi.device_available(), _capi.last_error()
-    return torch.device("cuda", 0)
+    yield torch.device("cuda", 0)
+    assert _capi.kernel_status(reset=True) == 0  # no bounded wait of a kernel ran out
 
 
 # ---- on the CPU ----
@@ -24,7 +25,7 @@ def test_refusals_need_no_device(lib_built):
     from t81lib_b200.nn import Q4Experts, Q4Linear
     lib = _capi.lib
     assert lib.t81b200_q4_bytes(17, 65) == 2 * 2 * 512 and lib.t81b200_q4_bytes(-1, 4) == -1
-    assert lib.t81b200_q4_scales(17, 65, 32) == 2 * 3 * 16 and lib.t81b200_q4_scales(17, 65, 33) == -1
+    assert lib.t81b200_q4_scales(17, 65, 32) == 2 * 4 * 16 and lib.t81b200_q4_scales(17, 65, 33) == -1
     buf = ctypes.create_string_buffer(64)
     assert lib.t81b200_quantize_q4(buf, 0, 1, 4, 8, 4, 0, 32, buf, buf, None) == _capi.EINVAL      # ld below cols
     assert lib.t81b200_quantize_q4(buf, 0, 1, 4, 8, 8, 0, 48, buf, buf, None) == _capi.EINVAL      # group
@@ -44,7 +45,7 @@ def test_refusals_need_no_device(lib_built):
         t81_torch.Q4Tensor(torch.zeros(512, dtype=torch.uint8), torch.zeros(16, dtype=torch.bfloat16), (17, 64), 64)
     with pytest.raises(ValueError, match="experts must be"):
         Q4Experts.from_float(torch.zeros(2, 8, 4), torch.zeros(2, 4, 3))
-    q = t81_torch.Q4Tensor(torch.zeros(512, dtype=torch.uint8), torch.zeros(16, dtype=torch.bfloat16), (16, 64), 64)
+    q = t81_torch.Q4Tensor(torch.zeros(512, dtype=torch.uint8), torch.zeros(32, dtype=torch.bfloat16), (16, 64), 64)
     with pytest.raises(ValueError, match="2D activations"):
         q.matmul_input(torch.zeros(64))
     with pytest.raises(ValueError, match="width"):

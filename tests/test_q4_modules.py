@@ -69,7 +69,8 @@ def test_convert_refusals_leave_the_model_alone(lib_built, tmp_path):
 def dev(lib_built):
     from t81lib_b200 import _capi
     assert _capi.device_available(), _capi.last_error()
-    return torch.device("cuda", 0)
+    yield torch.device("cuda", 0)
+    assert _capi.kernel_status(reset=True) == 0  # no bounded wait of a kernel ran out
 
 
 @pytest.mark.gpu

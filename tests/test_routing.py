@@ -16,7 +16,8 @@ pytestmark = pytest.mark.gpu
 def dev(lib_built):
     from t81lib_b200 import _capi
     assert _capi.device_available(), _capi.last_error()
-    return torch.device("cuda", 0)
+    yield torch.device("cuda", 0)
+    assert _capi.kernel_status(reset=True) == 0  # no bounded wait of a kernel ran out
 
 
 @pytest.mark.parametrize("tokens,top,experts", [(1, 1, 1), (1, 6, 64), (16, 6, 64), (33, 1, 3), (100, 8, 8), (512, 2, 60), (513, 2, 1024), (1500, 4, 100), (3000, 7, 33), (40, 3, 1024)])
