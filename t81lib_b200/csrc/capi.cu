@@ -88,6 +88,7 @@ int gemm_trit_tc_launch(int fmt, int fp32_planes, const uint8_t *A, const float 
 int gemm_trit_tc_status(int reset);
 int gemm_wgrad_status(int reset);
 int gemm_q4_tc_status(int reset);
+int gemv_q4_status(int reset);
 int gemv_trit_status(int reset);
 int gemv_trit_lut_status(int reset);
 int quantize_pack_status(int reset);
@@ -106,7 +107,7 @@ extern "C" int t81b200_kernel_status(int reset) {
     const int lut = gemv_trit_lut_status(reset);
     const int qp = quantize_pack_status(reset);
     const int wg = gemm_wgrad_status(reset);
-    const int q4 = gemm_q4_tc_status(reset);
+    const int q4_tc = gemm_q4_tc_status(reset), q4_gemv = gemv_q4_status(reset), q4 = q4_tc != 0 ? q4_tc : q4_gemv;
     if (wg != 0) return wg;
     if (q4 != 0) return q4;
     return tc != 0 ? tc : (gv != 0 ? gv : (lut != 0 ? lut : qp));

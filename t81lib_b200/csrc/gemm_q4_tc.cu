@@ -370,6 +370,7 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_co
         uint32_t off[2];
 #pragma unroll
         for (int s = 0; s < 2; ++s) off[s] = (uint32_t)(cw * 16 + g) * 128u + (uint32_t)((4 * (s ^ (int)swap) + t4) ^ g) * 16u;
+        const Q4Decode<T> decode;
         Ring a, raw;
         bool ok = true;
         for (int i = cluster_id; i < total_tiles && ok; i += n_clusters) {
@@ -434,8 +435,8 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_co
 #pragma unroll
                                 for (int pr = 0; pr < 2; ++pr) {
                                     const uint32_t x = w[2 * h + j];
-                                    const uint32_t v = r == 0 ? (pr == 0 ? Q4Decode<T>::template biased<0>(x) : Q4Decode<T>::template biased<2>(x))
-                                                              : (pr == 0 ? Q4Decode<T>::template biased<1>(x) : Q4Decode<T>::template biased<3>(x));
+                                    const uint32_t v = r == 0 ? (pr == 0 ? decode.template biased<0>(x) : decode.template biased<2>(x))
+                                                              : (pr == 0 ? decode.template biased<1>(x) : decode.template biased<3>(x));
                                     o[2 * j + pr] = Q4Decode<T>::scaled(v, sc, nc);
                                 }
                             *reinterpret_cast<uint4 *>(dst + k * A_ATOM_BYTES + off[h] + r * 1024) = make_uint4(o[0], o[1], o[2], o[3]);

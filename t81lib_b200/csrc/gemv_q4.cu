@@ -1,21 +1,28 @@
 // Products of 4-bit weights (q4.cuh) for few activation rows: y[t][o] = sum_k x[t][k] code[o][k] scale[o][k / group] (+ bias[o]).
 //
-// Bound by reading the weights (half a byte each and two bytes a group).  A warp streams 16-row tiles: a lane's 16 bytes of a tile are the
-// A fragments of four mma.sync m16n8k16, the codes as exact numbers -8 .. 7, and its eight columns of an activation row are the B
-// fragments of two of them, read where the row lies (L1 holds the few rows that a CTA's warps share; weights pass it by).  Sums of a
-// group are scaled and added in fp32.  The warps of a CTA take units of 128 columns in turn and their sums meet in shared memory, in
-// warp order: results do not depend on the schedule.
+// Bound by reading the weights (half a byte each and two bytes a group).  Every warp streams them through a ring of its own in shared memory:
+// TMA copies of the 128 columns (a unit) of RT row tiles, 1 KB each, and their scales, kStages units ahead, across rows and
+// experts: some 70 KB under way per SM, which the bandwidth times the latency wants (loads to registers two units ahead in 16 warps an
+// SM were 16 KB, and 65536 x 4096 with 8 tokens took 69 us).  A warp waits for and refills its own stages only.
+// A lane's 16 bytes of a tile are the A fragments of four mma.sync m16n8k16, the codes as exact numbers -8 .. 7, and its eight columns of an
+// activation row are the B fragments of two of them, read where the row lies (L1 holds the few rows that an SM's warps share).
+// Sums of a group are scaled and added in fp32.  A block's warps take the units of its rows in turn and their sums meet in shared
+// memory, in warp order: results do not depend on the schedule.
 //
 // float32 activations come as three bf16 planes (all 24 bits, stage_planes), each multiplied exactly; the first has sums of its own, since the
 // tensor core cuts small terms beside large ones off.
 //
-// The same kernel multiplies rows sorted by expert (`offsets`): a block finds the expert of its number among those that have rows and
-// takes that expert's rows; the blocks of the last number write zeros to rows behind the last expert's.
+// The same kernel multiplies rows sorted by expert (`offsets`): blocks go through the experts that have rows; rows behind the last
+// expert's become zero.
 #include "common.cuh"
 #include "launch_order.cuh"
 #include "q4.cuh"
 #include "tma.cuh"
 #include "umma.cuh"
+
+#include <atomic>
+#include <cstring>
+#include <type_traits>
 
 namespace t81b200 {
 
@@ -25,6 +32,11 @@ int gemm_q4_tc_launch(const uint8_t *codes, const void *scales, const float *bia
 
 namespace {
 
+constexpr int kWarps = 8, kThreads = kWarps * 32, kStages = 4, kMostExperts = 1024, kBlocksPerSm = 2;
+enum { STATUS_CONSUMER = 6 };
+
+__device__ int g_gemv_q4_status = 0;
+
 struct Q4Params {
     const uint8_t *codes;
     const __nv_bfloat16 *scales;
@@ -32,12 +44,14 @@ struct Q4Params {
     const void *x;
     void *y;
     int64_t ldx, ldy, plane_elems;  // elements
-    int64_t M, K, kx;               // kx: columns of x that may be read, a multiple of 8 (zeros past K)
+    int64_t M, kx;                  // kx: columns of x that may be read, a multiple of 8 (zeros past K)
     int64_t rows;                   // of x
-    int64_t code_stride, scale_stride, bias_stride;  // from one expert to the next
+    int64_t bias_stride;            // from one expert to the next
     const int32_t *offsets;         // n_experts + 1, or null: one matrix for all rows
     int n_experts;
-    int col_tiles, groups, units;
+    int col_tiles, groups, units;   // of a row
+    int row_tiles, row_items;       // 16-row tiles, and blocks' shares of them (RT * k_split-wise rows)
+    int k_warps;                    // warps that share a row tile's units
 };
 
 template <typename T> __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
@@ -52,126 +66,146 @@ template <> __device__ __forceinline__ void mma_16816<__half>(float (&c)[4], con
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Weights are read once: past L1.
-__device__ __forceinline__ uint4 load_codes(const uint8_t *p) {
-    uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    return v;
-}
-__device__ __forceinline__ uint32_t load_scales(const void *p) {
-    uint32_t v;
-    asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(v) : "l"(p));
-    return v;
+template <typename T>
+__device__ __forceinline__ void fragments(const Q4Decode<T> &decode, uint32_t w, uint32_t (&a)[4]) {
+    a[0] = decode.code(decode.template biased<0>(w));
+    a[1] = decode.code(decode.template biased<1>(w));
+    a[2] = decode.code(decode.template biased<2>(w));
+    a[3] = decode.code(decode.template biased<3>(w));
 }
 
-template <typename T>
-__device__ __forceinline__ void fragments(uint32_t w, uint32_t (&a)[4]) {
-    a[0] = Q4Decode<T>::minus24(Q4Decode<T>::template biased<0>(w));
-    a[1] = Q4Decode<T>::minus24(Q4Decode<T>::template biased<1>(w));
-    a[2] = Q4Decode<T>::minus24(Q4Decode<T>::template biased<2>(w));
-    a[3] = Q4Decode<T>::minus24(Q4Decode<T>::template biased<3>(w));
-}
+// Where a warp is: a block's share `item` of the row tiles (of an expert), and a pass over TOK of its rows of x.
+template <int TOK> struct Walk {
+    int item, expert, tile0;
+    int64_t tok, end;
+    __device__ __forceinline__ void open(const Q4Params &p, const int16_t *active, int items, int tiles_per_item, int tile_of_item) {
+        if (item >= items) return;
+        int share = item;
+        expert = 0;
+        tok = 0;
+        end = p.rows;
+        if (p.offsets) {
+            const int at = item / p.row_items;
+            share = item - at * p.row_items;
+            expert = active[at];
+            tok = max(p.offsets[expert], 0);
+            end = min((int64_t)p.offsets[expert + 1], p.rows);  // whatever the offsets say, nothing lies outside the rows
+        }
+        tile0 = share * tiles_per_item + tile_of_item;
+    }
+    // True where the next pass starts other rows of the weights.
+    __device__ __forceinline__ bool next(const Q4Params &p, const int16_t *active, int items, int tiles_per_item, int tile_of_item) {
+        tok += TOK;
+        if (tok < end) return false;
+        item += (int)gridDim.x;
+        open(p, active, items, tiles_per_item, tile_of_item);
+        return true;
+    }
+};
+
+template <int RT, int GROUP> constexpr int kStageBytes = RT * 1024 + (RT * (128 / GROUP) * 32 + 127) / 128 * 128;
 
 // T: type of the operands; PLANES: 1, or 3 of float32 activations; RT: row tiles a warp; NT: blocks of 8 rows of x at a time.
 template <typename T, int PLANES, int RT, int NT, int GROUP, typename CT>
-__global__ void __launch_bounds__(512) gemv_q4_kernel(const __grid_constant__ Q4Params p) {
-    extern __shared__ float part[];  // [warps][RT * 16 rows][8 NT rows of x]
-    constexpr int PER = 128 / GROUP, SUMS = PLANES == 1 ? 1 : 2, TOK = 8 * NT;
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm) gemv_q4_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_constant__ CUtensorMap map_scales, const __grid_constant__ Q4Params p) {
+    constexpr int PER = 128 / GROUP, SUMS = PLANES == 1 ? 1 : 2, TOK = 8 * NT, SCALES = PER * 32, CODES = RT * 1024, STAGE = kStageBytes<RT, GROUP>;
+    extern __shared__ __align__(128) uint8_t ring[];  // [warps][stages][RT units of codes, RT of scales], then part
+    __shared__ __align__(8) uint64_t full[kWarps][kStages];
+    __shared__ int16_t active[kMostExperts];
+    __shared__ int n_active, failed;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int kw = warp % p.k_warps, row_warps = kWarps / p.k_warps, rw = warp / p.k_warps;
+    float *part = reinterpret_cast<float *>(ring + kWarps * kStages * STAGE);  // [warps][TOK][RT * 16 + 1]
+    if (lane < kStages) mbar_init(smem_u32(&full[warp][lane]), 1);
+    if (threadIdx.x == 0) {
+        failed = 0;
+        prefetch_map(&map_codes);
+        prefetch_map(&map_scales);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     wait_for_kernel_ahead();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5, g = lane >> 2, t = lane & 3;
-    const int64_t tile0 = (int64_t)blockIdx.x * RT, row_tiles = (p.M + 15) >> 4;
-    int64_t first = 0, end = p.rows;
-    int expert = 0;
+    int items = p.row_items;
     if (p.offsets) {
-        // this block's expert: number blockIdx.y of those with rows
-        __shared__ int found[3];
         if (warp == 0) {
-            int seen = 0, expert_here = -1;
+            int seen = 0;
             for (int e0 = 0; e0 < p.n_experts; e0 += 32) {
                 const int e = e0 + lane;
-                const bool some = e < p.n_experts && p.offsets[e + 1] > p.offsets[e];
+                const bool some = e < p.n_experts && min((int64_t)p.offsets[e + 1], p.rows) > max(p.offsets[e], 0);
                 const uint32_t ballot = __ballot_sync(0xffffffffu, some);
-                const int n = __popc(ballot);
-                if (seen + n > (int)blockIdx.y) {
-                    const int nth = (int)__fns(ballot, 0, (int)blockIdx.y - seen + 1);
-                    expert_here = e0 + nth;
-                    break;
-                }
-                seen += n;
+                if (some) active[seen + __popc(ballot & ((1u << lane) - 1u))] = (int16_t)e;
+                seen += __popc(ballot);
             }
-            if (lane == 0) {
-                found[0] = expert_here;
-                if (expert_here >= 0) {
-                    found[1] = p.offsets[expert_here];
-                    found[2] = p.offsets[expert_here + 1];
-                }
-            }
+            if (lane == 0) n_active = seen;
         }
-        __syncthreads();
-        expert = found[0];
-        if (blockIdx.y == gridDim.y - 1) {  // rows of no expert
-            const int64_t kept = p.offsets[p.n_experts] > 0 ? p.offsets[p.n_experts] : 0;
-            for (int64_t i = threadIdx.x; i < (p.rows - kept) * (RT * 16); i += blockDim.x) {
-                const int64_t row = tile0 * 16 + i % (RT * 16), tok = kept + i / (RT * 16);
-                if (row < p.M) static_cast<CT *>(p.y)[tok * p.ldy + row] = from_float<CT>(0.0f);
-            }
-            return;
-        }
-        if (expert < 0) return;
-        first = found[1] > 0 ? found[1] : 0;
-        end = found[2] < p.rows ? found[2] : p.rows;  // whatever the offsets say, nothing lies outside the rows
+        const int64_t kept = max(p.offsets[p.n_experts], 0);  // rows of no expert: a warp each
+        for (int64_t row = kept + blockIdx.x * kWarps + warp; row < p.rows; row += (int64_t)gridDim.x * kWarps)
+            for (int64_t i = lane; i < p.M; i += 32) static_cast<CT *>(p.y)[row * p.ldy + i] = from_float<CT>(0.0f);
     }
-    const uint8_t *codes = p.codes + expert * p.code_stride;
-    const __nv_bfloat16 *scales = p.scales + expert * p.scale_stride;
-    const T *x = static_cast<const T *>(p.x);
+    __syncthreads();
+    if (p.offsets) items = n_active * p.row_items;
 
-    for (int64_t tok0 = first + (int64_t)blockIdx.z * TOK; tok0 < end; tok0 += (int64_t)gridDim.z * TOK) {
+    const uint32_t my_ring = smem_u32(ring) + (uint32_t)warp * kStages * STAGE, my_full = smem_u32(&full[warp][0]);
+    const int per_item = row_warps * RT, last_unit = p.units - 1;
+    Walk<TOK> fill, use;
+    fill.item = use.item = (int)blockIdx.x;
+    fill.open(p, active, items, per_item, rw * RT);
+    use.open(p, active, items, per_item, rw * RT);
+    // ---- copies (what lies past the matrix arrives as zeros, or is the next expert's rows) ----
+    int fill_unit = kw, fill_row = fill.expert * p.row_tiles + fill.tile0;
+    uint32_t slot = 0;
+    auto issue = [&]() {
+        if (fill.item >= items) return;
+        if (elect_one()) {
+            const uint32_t bar = my_full + 8u * slot, dst = my_ring + slot * STAGE;
+            mbar_arrive_expect_tx(bar, (uint32_t)(CODES + RT * SCALES));
+            tma_load_2d(dst, &map_codes, fill_unit * 256, fill_row, bar);
+            tma_load_2d(dst + CODES, &map_scales, fill_unit * (PER * 16), fill_row, bar);
+        }
+        __syncwarp();
+        slot = slot + 1 == kStages ? 0 : slot + 1;
+        fill_unit += p.k_warps;
+        if (fill_unit > last_unit) {
+            fill_unit = kw;
+            if (fill.next(p, active, items, per_item, rw * RT)) fill_row = fill.expert * p.row_tiles + fill.tile0;
+        }
+    };
+    if (p.units > 0)
+        for (int i = 0; i < kStages; ++i) issue();
+    const Q4Decode<T> decode;
+    Ring at;
+    bool ok = true;
+    while (use.item < items) {
+        const int tile0 = use.tile0;
         float sum[RT][NT][SUMS][4] = {};
-        auto read = [&](int unit, uint4 (&q)[RT][2], uint32_t (&s)[RT][PER]) {
+        // this lane's eight columns of a row of x for the B fragments; rows past the last are some other row's, and not stored
+        const T *src_x[NT];
 #pragma unroll
-            for (int r = 0; r < RT; ++r) {
-                const bool there = tile0 + r < row_tiles && unit < p.units;
-#pragma unroll
-                for (int c = 0; c < 2; ++c)
-                    q[r][c] = there && 2 * unit + c < p.col_tiles ? load_codes(codes + ((tile0 + r) * p.col_tiles + 2 * unit + c) * kQ4TileBytes + lane * 16) : make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-                for (int i = 0; i < PER; ++i)
-                    s[r][i] = there && unit * PER + i < p.groups ? load_scales(scales + ((tile0 + r) * (p.groups + 1) + unit * PER + i) * 16 + 2 * g) : 0u;
-            }
-        };
-        uint4 q[RT][2], q_next[RT][2];
-        uint32_t s[RT][PER], s_next[RT][PER];
-        read(warp, q_next, s_next);
-        for (int unit = warp; unit < p.units; unit += warps) {
-#pragma unroll
-            for (int r = 0; r < RT; ++r) {
-                q[r][0] = q_next[r][0];
-                q[r][1] = q_next[r][1];
-#pragma unroll
-                for (int i = 0; i < PER; ++i) s[r][i] = s_next[r][i];
-            }
+        for (int n = 0; n < NT; ++n) src_x[n] = static_cast<const T *>(p.x) + min(use.tok + 8 * n + g, use.end - 1) * p.ldx + kw * 128 + 8 * t;
+        auto multiply = [&](int unit, auto is_last) {
+            constexpr bool LAST = decltype(is_last)::value;
             uint4 b[PLANES][NT][4];  // [.. 32 columns]
 #pragma unroll
             for (int pl = 0; pl < PLANES; ++pl)
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const int64_t tok = tok0 + 8 * n + g;
-                    const T *src = x + pl * p.plane_elems + tok * p.ldx + (int64_t)unit * 128 + 8 * t;
+                for (int n = 0; n < NT; ++n)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        b[pl][n][i] = tok < end && (int64_t)unit * 128 + 32 * i + 8 * t < p.kx ? __ldg(reinterpret_cast<const uint4 *>(src + 32 * i)) : make_uint4(0u, 0u, 0u, 0u);
-                }
-            read(unit + warps, q_next, s_next);
+                        b[pl][n][i] = !LAST || (int64_t)unit * 128 + 32 * i + 8 * t < p.kx ? __ldg(reinterpret_cast<const uint4 *>(src_x[n] + pl * p.plane_elems + 32 * i)) : make_uint4(0u, 0u, 0u, 0u);
+            ok = __all_sync(0xffffffffu, mbar_wait(my_full + 8u * at.stage, at.phase));
+            if (!ok) return;
+            const uint8_t *src = ring + (warp * kStages + at.stage) * STAGE;
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
-                const uint32_t word[8] = {q[r][0].x, q[r][0].y, q[r][0].z, q[r][0].w, q[r][1].x, q[r][1].y, q[r][1].z, q[r][1].w};
+                // (what lies past the last column meets zeros of x, rows past the last are not stored)
+                const uint4 q0 = *reinterpret_cast<const uint4 *>(src + r * 1024 + lane * 16), q1 = *reinterpret_cast<const uint4 *>(src + r * 1024 + 512 + lane * 16);
+                const uint32_t word[8] = {q0.x, q0.y, q0.z, q0.w, q1.x, q1.y, q1.z, q1.w};
 #pragma unroll
                 for (int i = 0; i < PER; ++i) {
                     float c[NT][SUMS][4] = {};
 #pragma unroll
                     for (int j = i * (8 / PER); j < (i + 1) * (8 / PER); ++j) {
                         uint32_t a[4];
-                        fragments<T>(word[j], a);
+                        fragments<T>(decode, word[j], a);
 #pragma unroll
                         for (int pl = 0; pl < PLANES; ++pl)
 #pragma unroll
@@ -180,7 +214,8 @@ __global__ void __launch_bounds__(512) gemv_q4_kernel(const __grid_constant__ Q4
                                 mma_16816<T>(c[n][pl > 0 ? SUMS - 1 : 0], a, j & 1 ? v.z : v.x, j & 1 ? v.w : v.y);
                             }
                     }
-                    const float lo = __uint_as_float(s[r][i] << 16), hi = __uint_as_float(s[r][i] & 0xFFFF0000u);
+                    const uint32_t s = !LAST || unit * PER + i < p.groups ? *reinterpret_cast<const uint32_t *>(src + CODES + r * SCALES + i * 32 + 4 * g) : 0u;
+                    const float lo = __uint_as_float(s << 16), hi = __uint_as_float(s & 0xFFFF0000u);
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -192,10 +227,17 @@ __global__ void __launch_bounds__(512) gemv_q4_kernel(const __grid_constant__ Q4
                         }
                 }
             }
-        }
-        // part[warp][row of x][row of the tiles]
+            __syncwarp();
+            issue();  // into the stage just read
+            at.advance(kStages);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) src_x[n] += p.k_warps * 128;
+        };
+        int unit = kw;
+        for (; unit < last_unit && ok; unit += p.k_warps) multiply(unit, std::false_type{});
+        if (unit == last_unit && ok) multiply(unit, std::true_type{});
+        if (!ok && lane == 0) failed = 1;
         constexpr int WIDTH = RT * 16 + 1;
-        if (tok0 != first + (int64_t)blockIdx.z * TOK) __syncthreads();
 #pragma unroll
         for (int r = 0; r < RT; ++r)
 #pragma unroll
@@ -206,52 +248,74 @@ __global__ void __launch_bounds__(512) gemv_q4_kernel(const __grid_constant__ Q4
                     part[(warp * TOK + 8 * n + 2 * t + (i & 1)) * WIDTH + r * 16 + g + 8 * (i >> 1)] = v;
                 }
         __syncthreads();
-        for (int i = threadIdx.x; i < TOK * RT * 16; i += blockDim.x) {
-            const int tok = i / (RT * 16), r = i % (RT * 16);
-            const int64_t row = tile0 * 16 + r;
-            if (tok0 + tok >= end || row >= p.M) continue;
+        if (failed) break;  // the same for all: it is set before the barrier only
+        for (int i = threadIdx.x; i < TOK * row_warps * RT * 16; i += kThreads) {
+            const int r = i % (RT * 16), share = i / (RT * 16) % row_warps, tok = i / (RT * 16 * row_warps);
+            const int64_t row = (int64_t)(tile0 - rw * RT + share * RT) * 16 + r;
+            if (use.tok + tok >= use.end || row >= p.M) continue;
             float v = 0.0f;
-            for (int w = 0; w < warps; ++w) v += part[(w * TOK + tok) * WIDTH + r];
-            if (p.bias) v += p.bias[expert * p.bias_stride + row];
-            static_cast<CT *>(p.y)[(tok0 + tok) * p.ldy + row] = from_float<CT>(v);
+            for (int w = 0; w < p.k_warps; ++w) v += part[((share * p.k_warps + w) * TOK + tok) * WIDTH + r];
+            if (p.bias) v += p.bias[use.expert * p.bias_stride + row];
+            static_cast<CT *>(p.y)[(use.tok + tok) * p.ldy + row] = from_float<CT>(v);
         }
+        __syncthreads();
+        use.next(p, active, items, per_item, rw * RT);
     }
+    if (failed) give_up(&g_gemv_q4_status, STATUS_CONSUMER);
 }
 
 template <typename T, int PLANES, int RT, int NT, int GROUP, typename CT>
-int launch(const Q4Params &p, int warps, cudaStream_t st) {
-    const int64_t blocks = (((p.M + 15) / 16) + RT - 1) / RT, passes = (p.rows + 8 * NT - 1) / (8 * NT);
-    const dim3 grid((unsigned)blocks, p.offsets ? (unsigned)((p.rows < p.n_experts ? p.rows : p.n_experts) + 1) : 1u, p.offsets ? 1u : (unsigned)(passes < 65535 ? passes : 65535));
-    const size_t smem = (size_t)warps * 8 * NT * (RT * 16 + 1) * sizeof(float);
+int launch(Q4Params &p, cudaStream_t st) {
+    const int row_warps = kWarps / p.k_warps;
+    p.row_items = (p.row_tiles + RT * row_warps - 1) / (RT * row_warps);
+    const int64_t items = (int64_t)p.row_items * (p.offsets ? (p.rows < p.n_experts ? p.rows : p.n_experts) : 1), most = (int64_t)sm_count() * kBlocksPerSm;
+    constexpr size_t smem = (size_t)kWarps * (kStages * kStageBytes<RT, GROUP> + 8 * NT * (RT * 16 + 1) * sizeof(float));
+    CUtensorMap mc, ms;
+    memset(&mc, 0, sizeof mc);
+    memset(&ms, 0, sizeof ms);
+    if (p.units > 0) {
+        const uint64_t tiles = (uint64_t)p.row_tiles * (p.offsets ? p.n_experts : 1), scale_row = (uint64_t)(p.groups + 1) * 16;
+        if (int rc = make_map_2d(&mc, CU_TENSOR_MAP_DATA_TYPE_UINT32, p.codes, (uint64_t)p.col_tiles * 128, tiles, (uint64_t)p.col_tiles * kQ4TileBytes, 256, RT, CU_TENSOR_MAP_SWIZZLE_NONE)) return rc;
+        if (int rc = make_map_2d(&ms, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p.scales, scale_row, tiles, scale_row * 2, 128 / GROUP * 16, RT, CU_TENSOR_MAP_SWIZZLE_NONE)) return rc;
+    }
     auto kernel = gemv_q4_kernel<T, PLANES, RT, NT, GROUP, CT>;
-    if (smem > 48 * 1024) T81_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    T81_CUDA_TRY(launch_behind(kernel, grid, dim3(warps * 32), smem, st, p));
+    static std::atomic<bool> configured[64];  // the shared-memory limit is an attribute of the function on a device
+    int dev = 0;
+    T81_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64 || !configured[dev].load(std::memory_order_acquire)) {
+        T81_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        if (dev >= 0 && dev < 64) configured[dev].store(true, std::memory_order_release);
+    }
+    T81_CUDA_TRY(launch_behind(kernel, dim3((unsigned)(items < most ? items : most)), dim3(kThreads), smem, st, mc, ms, p));
     return T81B200_OK;
 }
 
 template <typename T, int PLANES, int RT, int NT, int GROUP>
-int launch_ct(const Q4Params &p, int c_dtype, int warps, cudaStream_t st) {
+int launch_ct(Q4Params &p, int c_dtype, cudaStream_t st) {
     switch (c_dtype) {
-        case T81B200_F32: return launch<T, PLANES, RT, NT, GROUP, float>(p, warps, st);
-        case T81B200_BF16: return launch<T, PLANES, RT, NT, GROUP, __nv_bfloat16>(p, warps, st);
-        case T81B200_F16: return launch<T, PLANES, RT, NT, GROUP, __half>(p, warps, st);
+        case T81B200_F32: return launch<T, PLANES, RT, NT, GROUP, float>(p, st);
+        case T81B200_BF16: return launch<T, PLANES, RT, NT, GROUP, __nv_bfloat16>(p, st);
+        case T81B200_F16: return launch<T, PLANES, RT, NT, GROUP, __half>(p, st);
     }
     return fail(T81B200_EINVAL, "linear_q4: unknown output dtype %d", c_dtype);
 }
 
 template <typename T, int PLANES, int RT, int NT>
-int launch_group(const Q4Params &p, int group, int c_dtype, int warps, cudaStream_t st) {
-    if (group == 32) return launch_ct<T, PLANES, RT, NT, 32>(p, c_dtype, warps, st);
-    if (group == 64) return launch_ct<T, PLANES, RT, NT, 64>(p, c_dtype, warps, st);
-    return launch_ct<T, PLANES, RT, NT, 128>(p, c_dtype, warps, st);
+int launch_group(Q4Params &p, int group, int c_dtype, cudaStream_t st) {
+    if (group == 32) return launch_ct<T, PLANES, RT, NT, 32>(p, c_dtype, st);
+    if (group == 64) return launch_ct<T, PLANES, RT, NT, 64>(p, c_dtype, st);
+    return launch_ct<T, PLANES, RT, NT, 128>(p, c_dtype, st);
 }
 
 template <typename T, int PLANES>
-int launch_shape(const Q4Params &p, int group, int c_dtype, cudaStream_t st) {
-    const int warps = p.units >= 16 ? 16 : (p.units >= 8 ? 8 : 4);
+int launch_shape(Q4Params &p, int group, int c_dtype, cudaStream_t st) {
+    p.k_warps = p.units >= 8 ? 8 : (p.units >= 4 ? 4 : (p.units >= 2 ? 2 : 1));
+    // two row tiles a warp read each piece of an activation row once for both, where that leaves every block a share
+    const int64_t shares = (int64_t)p.row_tiles * p.k_warps / kWarps * (p.offsets ? (p.rows < p.n_experts ? p.rows : p.n_experts) : 1);
+    const bool wide = shares >= 2 * (int64_t)sm_count() * kBlocksPerSm;
     if constexpr (PLANES == 1)
-        if (p.rows > 8) return launch_group<T, PLANES, 1, 2>(p, group, c_dtype, warps, st);
-    return launch_group<T, PLANES, 1, 1>(p, group, c_dtype, warps, st);  // three planes of 16 rows do not fit the registers
+        if (p.rows > 8 && !p.offsets) return wide ? launch_group<T, PLANES, 2, 2>(p, group, c_dtype, st) : launch_group<T, PLANES, 1, 2>(p, group, c_dtype, st);
+    return wide ? launch_group<T, PLANES, 2, 1>(p, group, c_dtype, st) : launch_group<T, PLANES, 1, 1>(p, group, c_dtype, st);  // three planes of 16 rows do not fit the registers
 }
 
 // Rows that the kernels read where they are: 16-bit, on 16-byte boundaries, whole pieces of eight columns.
@@ -265,7 +329,8 @@ int product_q4(const char *name, const uint8_t *codes, const void *scales, const
     if (M < 0 || N < 0 || K < 0 || ldb < K || ldc < M || n_experts < 0) return fail(T81B200_EINVAL, "%s: bad dimensions", name);
     if (!q4_group_ok(group)) return fail(T81B200_EINVAL, "%s: groups of 32, 64 or 128 columns, not %d", name, group);
     if (dtype_size(b_dtype) == 0 || b_dtype < 0 || b_dtype > T81B200_F16 || c_dtype < 0 || c_dtype > T81B200_F16) return fail(T81B200_EINVAL, "%s: unknown dtype", name);
-    if (M >= (1ll << 31) || N >= (1ll << 31) || K >= (1ll << 31) || n_experts > 65534) return fail(T81B200_ELIMIT, "%s: dimension too large", name);
+    if (M >= (1ll << 31) || N >= (1ll << 31) || K >= (1ll << 31) || n_experts > kMostExperts || q4_row_tiles(M) * (n_experts > 0 ? n_experts : 1) >= (1ll << 31))
+        return fail(T81B200_ELIMIT, "%s: dimension too large (at most %d experts)", name, kMostExperts);
     if (int rc = check_device()) return rc;
     if (M == 0 || N == 0) return T81B200_OK;
     if (!C || (K > 0 && (!B || !codes || !scales))) return fail(T81B200_EINVAL, "%s: null pointer", name);
@@ -274,10 +339,11 @@ int product_q4(const char *name, const uint8_t *codes, const void *scales, const
     p.codes = codes; p.scales = static_cast<const __nv_bfloat16 *>(scales); p.bias = bias;
     p.x = B; p.ldx = ldb; p.kx = K;
     p.y = C; p.ldy = ldc;
-    p.M = M; p.K = K; p.rows = N;
+    p.M = M; p.rows = N;
     p.offsets = offsets; p.n_experts = n_experts;
-    p.code_stride = t81b200_q4_bytes(M, K); p.scale_stride = t81b200_q4_scales(M, K, group); p.bias_stride = M;
-    p.col_tiles = (int)q4_col_tiles(K); p.groups = (int)q4_groups(K, group); p.units = (int)((K + 127) / 128);
+    p.bias_stride = M;
+    p.col_tiles = (int)q4_col_tiles(K); p.groups = (int)q4_groups(K, group); p.units = (int)((K + 127) / 128); p.row_tiles = (int)q4_row_tiles(M);
+
     if (K > 0 && !in_place(B, b_dtype, ldb, K)) {
         const size_t need = (size_t)(b_dtype == T81B200_F32 ? 3 : 1) * N * staged_row(K) * 2;
         if (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
@@ -287,13 +353,24 @@ int product_q4(const char *name, const uint8_t *codes, const void *scales, const
         p.ldx = p.kx = staged_row(K);
         p.plane_elems = N * p.ldx;
     }
-    if (b_dtype != T81B200_F32 && K > 0 && n_experts <= 1024 && N >= (offsets ? 8 * (int64_t)n_experts : 33))
+    if (b_dtype != T81B200_F32 && K > 0 && N >= (offsets ? 8 * (int64_t)n_experts : 33))
         return gemm_q4_tc_launch(codes, scales, bias, C, M, p.x, b_dtype == T81B200_F16, p.ldx, c_dtype, ldc, N, K, group, offsets, n_experts, st);
     if (b_dtype == T81B200_F32) return launch_shape<__nv_bfloat16, 3>(p, group, c_dtype, st);
     return b_dtype == T81B200_BF16 ? launch_shape<__nv_bfloat16, 1>(p, group, c_dtype, st) : launch_shape<__half, 1>(p, group, c_dtype, st);
 }
 
 }  // namespace
+
+int gemv_q4_status(int reset) {
+    int v = 0;
+    if (cudaMemcpyFromSymbol(&v, g_gemv_q4_status, sizeof v) != cudaSuccess) return T81B200_ECUDA;
+    if (reset && v != 0) {
+        const int zero = 0;
+        if (cudaMemcpyToSymbol(g_gemv_q4_status, &zero, sizeof zero) != cudaSuccess) return T81B200_ECUDA;
+    }
+    return v;
+}
+
 }  // namespace t81b200
 
 using namespace t81b200;

@@ -27,25 +27,40 @@ __host__ __device__ inline int64_t q4_groups(int64_t cols, int group) { return (
 inline bool q4_group_ok(int group) { return group == 32 || group == 64 || group == 128; }
 
 // Register r of a word as a pair of exact numbers -8 .. 7.  The four bits go to where the units 1 to 8 lie in the mantissa of 16 (bf16: bit
-// 3, fp16: bit 6), which gives 16 + code + 8; one packed FMA takes the 24 away.
+// 3, fp16: bit 6), which gives 16 + code + 8; one packed add takes the 24 away, or one packed FMA with a scale s and -24 s.
+// The constants are made opaque: known ones are made again for every use where registers are short, which doubled the instructions of
+// the streaming kernel.
+__device__ __forceinline__ uint32_t opaque(uint32_t v) {
+    uint32_t r;
+    asm volatile("mov.b32 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t d;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+    return d;
+}
+
 template <typename T> struct Q4Decode;
 template <> struct Q4Decode<__nv_bfloat16> {
-    template <int R> static __device__ __forceinline__ uint32_t biased(uint32_t w) {
-        const uint32_t x = R == 0 ? w << 3 : w >> (4 * R - 3);
-        return (x & 0x00780078u) | 0x41804180u;
+    uint32_t mask, sixteen, minus24;
+    __device__ __forceinline__ Q4Decode() : mask(opaque(0x00780078u)), sixteen(opaque(0x41804180u)), minus24(opaque(0xC1C0C1C0u)) {}
+    template <int R> __device__ __forceinline__ uint32_t biased(uint32_t w) const { return and_or(R == 0 ? w << 3 : w >> (4 * R - 3), mask, sixteen); }
+    __device__ __forceinline__ uint32_t code(uint32_t v) const {
+        uint32_t d;
+        asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(v), "r"(minus24));
+        return d;
     }
-    static __device__ __forceinline__ uint32_t minus24(uint32_t v) { return fma_bf16x2(v, 0x3F803F80u, 0xC1C0C1C0u); }
     // (v - 24) s for n = -24 s (7 bits): one rounding, of an exact result
     static __device__ __forceinline__ uint32_t scaled(uint32_t v, uint32_t s, uint32_t n) { return fma_bf16x2(v, s, n); }
 };
 template <> struct Q4Decode<__half> {
-    template <int R> static __device__ __forceinline__ uint32_t biased(uint32_t w) {
-        const uint32_t x = R < 2 ? w << (6 - 4 * R) : w >> (4 * R - 6);
-        return (x & 0x03C003C0u) | 0x4C004C00u;
-    }
-    static __device__ __forceinline__ uint32_t minus24(uint32_t v) {
+    uint32_t mask, sixteen, minus24;
+    __device__ __forceinline__ Q4Decode() : mask(opaque(0x03C003C0u)), sixteen(opaque(0x4C004C00u)), minus24(opaque(0xCE00CE00u)) {}
+    template <int R> __device__ __forceinline__ uint32_t biased(uint32_t w) const { return and_or(R < 2 ? w << (6 - 4 * R) : w >> (4 * R - 6), mask, sixteen); }
+    __device__ __forceinline__ uint32_t code(uint32_t v) const {
         uint32_t d;
-        asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(v), "r"(0xCE00CE00u));
+        asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(v), "r"(minus24));
         return d;
     }
     static __device__ __forceinline__ uint32_t scaled(uint32_t v, uint32_t s, uint32_t n) {
