@@ -20,7 +20,8 @@
 //
 // Few tiles: the contraction is split over S = 2 to 4 pairs of a cluster, whose sums meet in shared memory and are added in rank order.
 //
-// 15 warps per CTA: 0 activations   1 MMA issuer (even CTA), TMEM allocation   2-5 epilogue   6-13 converters   14 codes and scales.
+// 23 warps per CTA: 0 activations   1 MMA issuer (even CTA), TMEM allocation   2-5 epilogue   6-21 converters (two groups of eight that take
+// alternate chunks)   22 codes and scales.
 // Every mbarrier wait is bounded; on expiry the role records a status code and all roles fall through to the common teardown.
 #include "common.cuh"
 #include "launch_order.cuh"
@@ -39,8 +40,9 @@ namespace {
 constexpr int BM = 128, BK = 64, CHUNK = 128;
 constexpr int A_ATOM_BYTES = BM * BK * 2, A_CHUNK_BYTES = 2 * A_ATOM_BYTES;  // 16 and 32 KB
 constexpr int RAW_CODES = 8 * 1024, RAW_BYTES = RAW_CODES + 1024;            // a chunk's codes and scales
-constexpr int A_STAGES = 3, RAW_STAGES = 3, B_MAX = 12, MAX_SPLITS = 4;
-constexpr int NUM_THREADS = 15 * 32, EPILOGUE_WARP0 = 2, CONVERTER_WARP0 = 6, CONVERTERS = 8, RAW_WARP = 14;
+constexpr int A_STAGES = 3, RAW_STAGES = 4, B_MAX = 12, MAX_SPLITS = 4;
+constexpr int NUM_THREADS = 23 * 32, EPILOGUE_WARP0 = 2, CONVERTER_WARP0 = 6, CONVERTERS = 8, RAW_WARP = 22;
+constexpr int FINISHERS = (RAW_WARP - EPILOGUE_WARP0) / 4;  // groups of four warps that finish a tile alone in its launch
 constexpr int BARRIER_BYTES = 512, MOST_EXPERTS = 1024;
 constexpr int SMEM_LIMIT = 227 * 1024;
 
@@ -364,16 +366,22 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_co
         }
         if (!ok) give_up(&g_q4_status, STATUS_EPILOGUE);
     } else {
-        // ---------------- converters: 16 rows of a chunk each ----------------
-        const int cw = warp - CONVERTER_WARP0, g = lane >> 2, t4 = lane & 3;
+        // ---------------- converters: 16 rows of a chunk each, the two groups take the chunks of the CTA's sequence in turn ----------------
+        const int cw = (warp - CONVERTER_WARP0) & 7, group = (warp - CONVERTER_WARP0) >> 3, g = lane >> 2, t4 = lane & 3;
         const uint32_t swap = (uint32_t)(g & 1);  // lanes of odd rows store their second 32 columns first: eight lanes cover all banks
         uint32_t off[2];
 #pragma unroll
         for (int s = 0; s < 2; ++s) off[s] = (uint32_t)(cw * 16 + g) * 128u + (uint32_t)((4 * (s ^ (int)swap) + t4) ^ g) * 16u;
         const Q4Decode<T> decode;
+        // Slots of the raw ring (four) stay with a group.  Those of the operand ring (three) change hands: a group waits for the MMAs of the slot's
+        // last chunk, k - 3.  It has seen those of k - 5 end when it took its own last chunk, and MMAs end in order, so those of k - 6, the
+        // slot's use before, have ended too, and the wait cannot be a whole use behind.
         Ring a, raw;
+        if (group == 1) { a.advance(A_STAGES); raw.advance(RAW_STAGES); }
         bool ok = true;
-        for (int i = cluster_id; i < total_tiles && ok; i += n_clusters) {
+        const int span = c1 - c0;
+        int c = group;  // of the tile's span
+        for (int i = cluster_id; i < total_tiles && ok; i += n_clusters, c -= span) {
             float shrink[2] = {1.0f, 1.0f};
             if constexpr (F16) {
                 const Tile t = tiles.tile(p, i, half);
@@ -382,7 +390,7 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_co
                 for (int r = 0; r < 2; ++r)
                     if (t.row0 + cw * 16 < p.M) shrink[r] = __uint_as_float(0x7F000000u - row_exponent(p.scales, tile, p.groups, g + 8 * r));  // 2^-e
             }
-            for (int c = c0; c < c1; ++c) {
+            for (; c < span; c += 2) {
                 ok = __all_sync(0xffffffffu, mbar_wait(raw_full(raw.stage), raw.phase));
                 if (!ok) break;
                 const uint8_t *src = gen_base + raw_off + raw.stage * RAW_BYTES;
@@ -392,9 +400,6 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_co
                 for (int k = 0; k < 2; ++k) q[k] = *reinterpret_cast<const uint4 *>(src + cw * 1024 + k * 512 + lane * 16);
 #pragma unroll
                 for (int u = 0; u < PER; ++u) s[u] = *reinterpret_cast<const uint32_t *>(src + RAW_CODES + (cw * PER + u) * 32 + g * 4);
-                __syncwarp();
-                if (lane == 0) mbar_arrive(raw_empty(raw.stage));
-                raw.advance(RAW_STAGES);
                 // a row's scale twice in a word, and -24 times it
                 uint32_t s2[2][PER], n2[2][PER];
 #pragma unroll
@@ -445,7 +450,15 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_co
                 // generic-proxy writes must be visible to the tensor core's async proxy
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive_leader(a_full(a.stage));
+                // The codes are handed back only now that they have been used: an arrival overtakes loads of shared memory that are still on their way
+                // (16 warps' stores ahead of them), and the next copy overwrote what they were to read.
+                if (lane == 0) {
+                    mbar_arrive_leader(a_full(a.stage));
+                    mbar_arrive(raw_empty(raw.stage));
+                }
+                raw.advance(RAW_STAGES);
+                raw.advance(RAW_STAGES);
+                a.advance(A_STAGES);
                 a.advance(A_STAGES);
             }
         }
@@ -454,7 +467,7 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_co
     __syncwarp();
 
     if (p.one_tile) {
-        // Three groups of four warps take the tile's 32-row blocks in turn; what they stage goes into the activation ring, idle by now.  With
+        // Groups of four warps take the tile's 32-row blocks in turn; what they stage goes into the activation ring, idle by now.  With
         // splits > 1 block b is finished by slice b % splits, the others write theirs into its shared memory first (the weight ring).
         const int group = (warp - EPILOGUE_WARP0) >> 2, quarter = warp & 3, S = p.splits, blocks = p.bn / 32;
         const bool worker = warp >= EPILOGUE_WARP0 && warp < RAW_WARP;
@@ -467,7 +480,7 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_co
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         if (S > 1) {
             if (worker)
-                for (int b = group; b < blocks; b += 3) {
+                for (int b = group; b < blocks; b += FINISHERS) {
                     const int to = b % S;
                     if (to == slice) continue;
                     uint32_t v[32];
@@ -479,7 +492,7 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_co
         }
         if (worker) {
             CT *stage = reinterpret_cast<CT *>(gen_base + b_off) + (group * 4 + quarter) * 1024;
-            for (int b = slice + S * group; b < blocks; b += 3 * S) {
+            for (int b = slice + S * group; b < blocks; b += FINISHERS * S) {
                 uint32_t v[32];
                 tmem_ld32(t_lane + (uint32_t)(b * 32), v);
                 if (S > 1) fold_partials(v, gen_base, b, S, slice, r);

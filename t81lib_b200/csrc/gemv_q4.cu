@@ -1,7 +1,7 @@
 // Products of 4-bit weights (q4.cuh) for few activation rows: y[t][o] = sum_k x[t][k] code[o][k] scale[o][k / group] (+ bias[o]).
 //
 // Bound by reading the weights (half a byte each and two bytes a group).  Every warp streams them through a ring of its own in shared memory:
-// TMA copies of the 128 columns (a unit) of RT row tiles, 1 KB each, and their scales, kStages units ahead, across rows and
+// TMA copies of the 128 or 256 columns (a unit) of RT row tiles, 1 or 2 KB each, and their scales, some units ahead, across rows and
 // experts: some 70 KB under way per SM, which the bandwidth times the latency wants (loads to registers two units ahead in 16 warps an
 // SM were 16 KB, and 65536 x 4096 with 8 tokens took 69 us).  A warp waits for and refills its own stages only.
 // A lane's 16 bytes of a tile are the A fragments of four mma.sync m16n8k16, the codes as exact numbers -8 .. 7, and its eight columns of an
@@ -32,7 +32,7 @@ int gemm_q4_tc_launch(const uint8_t *codes, const void *scales, const float *bia
 
 namespace {
 
-constexpr int kWarps = 8, kThreads = kWarps * 32, kStages = 4, kMostExperts = 1024, kBlocksPerSm = 2;
+constexpr int kWarps = 8, kThreads = kWarps * 32, kMostExperts = 1024, kBlocksPerSm = 2;
 enum { STATUS_CONSUMER = 6 };
 
 __device__ int g_gemv_q4_status = 0;
@@ -44,8 +44,9 @@ struct Q4Params {
     const void *x;
     void *y;
     int64_t ldx, ldy, plane_elems;  // elements
-    int64_t M, kx;                  // kx: columns of x that may be read, a multiple of 8 (zeros past K)
-    int64_t rows;                   // of x
+    int M, kx;                      // kx: columns of x that may be read, a multiple of 8 (zeros past K)
+    int rows;                       // of x
+    int y_dtype;
     int64_t bias_stride;            // from one expert to the next
     const int32_t *offsets;         // n_experts + 1, or null: one matrix for all rows
     int n_experts;
@@ -54,16 +55,23 @@ struct Q4Params {
     int k_warps;                    // warps that share a row tile's units
 };
 
-template <typename T> __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
-template <> __device__ __forceinline__ void mma_16816<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-template <> __device__ __forceinline__ void mma_16816<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+// c = a b, or (ADD) c += a b.
+template <typename T, bool ADD> __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+#define T81_MMA(TYPE)                                                                                                                                  \
+    if constexpr (ADD)                                                                                                                                 \
+        asm("mma.sync.aligned.m16n8k16.row.col.f32." TYPE "." TYPE ".f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"              \
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])                                                                                           \
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));                                                                           \
+    else                                                                                                                                               \
+        asm("mma.sync.aligned.m16n8k16.row.col.f32." TYPE "." TYPE ".f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"          \
+            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])                                                                                           \
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f))
+    if constexpr (std::is_same<T, __half>::value) {
+        T81_MMA("f16");
+    } else {
+        T81_MMA("bf16");
+    }
+#undef T81_MMA
 }
 
 template <typename T>
@@ -76,8 +84,7 @@ __device__ __forceinline__ void fragments(const Q4Decode<T> &decode, uint32_t w,
 
 // Where a warp is: a block's share `item` of the row tiles (of an expert), and a pass over TOK of its rows of x.
 template <int TOK> struct Walk {
-    int item, expert, tile0;
-    int64_t tok, end;
+    int item, expert, tile0, tok, end;
     __device__ __forceinline__ void open(const Q4Params &p, const int16_t *active, int items, int tiles_per_item, int tile_of_item) {
         if (item >= items) return;
         int share = item;
@@ -89,7 +96,7 @@ template <int TOK> struct Walk {
             share = item - at * p.row_items;
             expert = active[at];
             tok = max(p.offsets[expert], 0);
-            end = min((int64_t)p.offsets[expert + 1], p.rows);  // whatever the offsets say, nothing lies outside the rows
+            end = min(p.offsets[expert + 1], p.rows);  // whatever the offsets say, nothing lies outside the rows
         }
         tile0 = share * tiles_per_item + tile_of_item;
     }
@@ -103,20 +110,79 @@ template <int TOK> struct Walk {
     }
 };
 
-template <int RT, int GROUP> constexpr int kStageBytes = RT * 1024 + (RT * (128 / GROUP) * 32 + 127) / 128 * 128;
+// A unit is W x 128 columns; four stages of 128 or two of 256.
+template <int RT, int W, int GROUP> struct Stage {
+    static constexpr int kCodes = RT * W * 1024, kScales = W * (128 / GROUP) * 32, kBytes = kCodes + (RT * kScales + 127) / 128 * 128, kCount = W == 1 ? 4 : 2;
+};
 
-// T: type of the operands; PLANES: 1, or 3 of float32 activations; RT: row tiles a warp; NT: blocks of 8 rows of x at a time.
-template <typename T, int PLANES, int RT, int NT, int GROUP, typename CT>
-__global__ void __launch_bounds__(kThreads, kBlocksPerSm) gemv_q4_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_constant__ CUtensorMap map_scales, const __grid_constant__ Q4Params p) {
-    constexpr int PER = 128 / GROUP, SUMS = PLANES == 1 ? 1 : 2, TOK = 8 * NT, SCALES = PER * 32, CODES = RT * 1024, STAGE = kStageBytes<RT, GROUP>;
+// acc = (FIRST) or += the fragment's product with x, columns 16 j .. of the unit.
+template <typename T, int PLANES, int NT, bool FIRST>
+__device__ __forceinline__ void products(float (&acc)[NT][PLANES == 1 ? 1 : 2][4], const uint32_t (&a)[4], const uint4 (&b)[PLANES][NT][4], int j) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        auto b0 = [&](int pl) { return j & 1 ? b[pl][n][j >> 1].z : b[pl][n][j >> 1].x; };
+        auto b1 = [&](int pl) { return j & 1 ? b[pl][n][j >> 1].w : b[pl][n][j >> 1].y; };
+        mma_16816<T, !FIRST>(acc[n][0], a, b0(0), b1(0));
+        if constexpr (PLANES == 3) {
+            mma_16816<T, !FIRST>(acc[n][1], a, b0(1), b1(1));
+            mma_16816<T, true>(acc[n][1], a, b0(2), b1(2));
+        }
+    }
+}
+
+// 128 columns of RT row tiles: sum += scale * sums over the columns of a group, group after group.
+// (What lies past the last column meets zeros of x, rows past the last are not stored.)
+template <typename T, int PLANES, int RT, int NT, int GROUP>
+__device__ __forceinline__ void multiply(const Q4Decode<T> &decode, const uint32_t (&word)[RT][8], const uint32_t (&scale)[RT][128 / GROUP], const uint4 (&b)[PLANES][NT][4],
+                                         float (&sum)[RT][NT][PLANES == 1 ? 1 : 2][4]) {
+    constexpr int PER = 128 / GROUP, SUMS = PLANES == 1 ? 1 : 2;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        float c[RT][NT][SUMS][4];
+#pragma unroll
+        for (int j = i * (8 / PER); j < (i + 1) * (8 / PER); ++j)
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                uint32_t a[4];
+                fragments<T>(decode, word[r][j], a);
+                if (j == i * (8 / PER)) products<T, PLANES, NT, true>(c[r], a, b, j);
+                else products<T, PLANES, NT, false>(c[r], a, b, j);
+            }
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            const float lo = __uint_as_float(scale[r][i] << 16), hi = __uint_as_float(scale[r][i] & 0xFFFF0000u);
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int u = 0; u < SUMS; ++u)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) sum[r][n][u][k] = fmaf(c[r][n][u][k], k < 2 ? lo : hi, sum[r][n][u][k]);
+        }
+    }
+}
+
+__device__ __forceinline__ void store(void *y, int64_t at, float v, int dtype) {
+    if (dtype == T81B200_F32) static_cast<float *>(y)[at] = v;
+    else if (dtype == T81B200_BF16) static_cast<__nv_bfloat16 *>(y)[at] = __float2bfloat16_rn(v);
+    else static_cast<__half *>(y)[at] = __float2half_rn(v);
+}
+
+// T: type of the operands; PLANES: 1, or 3 of float32 activations; RT: row tiles a warp; NT: blocks of 8 rows of x at a time; W: 128
+// columns of a unit.
+template <typename T, int PLANES, int RT, int NT, int W, int GROUP>
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm)
+gemv_q4_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_constant__ CUtensorMap map_scales, const __grid_constant__ Q4Params p) {
+    using S = Stage<RT, W, GROUP>;
+    constexpr int PER = 128 / GROUP, SUMS = PLANES == 1 ? 1 : 2, TOK = 8 * NT;
     extern __shared__ __align__(128) uint8_t ring[];  // [warps][stages][RT units of codes, RT of scales], then part
-    __shared__ __align__(8) uint64_t full[kWarps][kStages];
+    __shared__ __align__(8) uint64_t full[kWarps][S::kCount];
     __shared__ int16_t active[kMostExperts];
     __shared__ int n_active, failed;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int kw = warp % p.k_warps, row_warps = kWarps / p.k_warps, rw = warp / p.k_warps;
-    float *part = reinterpret_cast<float *>(ring + kWarps * kStages * STAGE);  // [warps][TOK][RT * 16 + 1]
-    if (lane < kStages) mbar_init(smem_u32(&full[warp][lane]), 1);
+    constexpr int WIDTH = RT * 16 + 1, PART = kWarps * TOK * WIDTH;
+    float *part = reinterpret_cast<float *>(ring + kWarps * S::kCount * S::kBytes);  // two of [warps][TOK][WIDTH] in turn, so that one barrier a pass is enough
+    if (lane < S::kCount) mbar_init(smem_u32(&full[warp][lane]), 1);
     if (threadIdx.x == 0) {
         failed = 0;
         prefetch_map(&map_codes);
@@ -130,7 +196,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) gemv_q4_kernel(const _
             int seen = 0;
             for (int e0 = 0; e0 < p.n_experts; e0 += 32) {
                 const int e = e0 + lane;
-                const bool some = e < p.n_experts && min((int64_t)p.offsets[e + 1], p.rows) > max(p.offsets[e], 0);
+                const bool some = e < p.n_experts && min(p.offsets[e + 1], p.rows) > max(p.offsets[e], 0);
                 const uint32_t ballot = __ballot_sync(0xffffffffu, some);
                 if (some) active[seen + __popc(ballot & ((1u << lane) - 1u))] = (int16_t)e;
                 seen += __popc(ballot);
@@ -139,13 +205,13 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) gemv_q4_kernel(const _
         }
         const int64_t kept = max(p.offsets[p.n_experts], 0);  // rows of no expert: a warp each
         for (int64_t row = kept + blockIdx.x * kWarps + warp; row < p.rows; row += (int64_t)gridDim.x * kWarps)
-            for (int64_t i = lane; i < p.M; i += 32) static_cast<CT *>(p.y)[row * p.ldy + i] = from_float<CT>(0.0f);
+            for (int i = lane; i < p.M; i += 32) store(p.y, row * p.ldy + i, 0.0f, p.y_dtype);
     }
     __syncthreads();
     if (p.offsets) items = n_active * p.row_items;
 
-    const uint32_t my_ring = smem_u32(ring) + (uint32_t)warp * kStages * STAGE, my_full = smem_u32(&full[warp][0]);
-    const int per_item = row_warps * RT, last_unit = p.units - 1;
+    const uint32_t my_ring = smem_u32(ring) + (uint32_t)(warp * S::kCount * S::kBytes), my_full = smem_u32(&full[warp][0]);
+    const int per_item = row_warps * RT;
     Walk<TOK> fill, use;
     fill.item = use.item = (int)blockIdx.x;
     fill.open(p, active, items, per_item, rw * RT);
@@ -156,88 +222,81 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) gemv_q4_kernel(const _
     auto issue = [&]() {
         if (fill.item >= items) return;
         if (elect_one()) {
-            const uint32_t bar = my_full + 8u * slot, dst = my_ring + slot * STAGE;
-            mbar_arrive_expect_tx(bar, (uint32_t)(CODES + RT * SCALES));
-            tma_load_2d(dst, &map_codes, fill_unit * 256, fill_row, bar);
-            tma_load_2d(dst + CODES, &map_scales, fill_unit * (PER * 16), fill_row, bar);
+            const uint32_t bar = my_full + 8u * slot, dst = my_ring + slot * S::kBytes;
+            mbar_arrive_expect_tx(bar, (uint32_t)(S::kCodes + RT * S::kScales));
+            tma_load_3d(dst, &map_codes, 0, fill_unit * (2 * W), fill_row, bar);
+            tma_load_2d(dst + S::kCodes, &map_scales, fill_unit * (W * PER * 16), fill_row, bar);
         }
         __syncwarp();
-        slot = slot + 1 == kStages ? 0 : slot + 1;
+        slot = slot + 1 == S::kCount ? 0 : slot + 1;
         fill_unit += p.k_warps;
-        if (fill_unit > last_unit) {
+        if (fill_unit >= p.units) {
             fill_unit = kw;
             if (fill.next(p, active, items, per_item, rw * RT)) fill_row = fill.expert * p.row_tiles + fill.tile0;
         }
     };
     if (p.units > 0)
-        for (int i = 0; i < kStages; ++i) issue();
+        for (int i = 0; i < S::kCount; ++i) issue();
     const Q4Decode<T> decode;
+    const uint32_t nothing = opaque(0u);
     Ring at;
-    bool ok = true;
+    bool ok = true, buffer = false;
     while (use.item < items) {
         const int tile0 = use.tile0;
         float sum[RT][NT][SUMS][4] = {};
         // this lane's eight columns of a row of x for the B fragments; rows past the last are some other row's, and not stored
         const T *src_x[NT];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) src_x[n] = static_cast<const T *>(p.x) + min(use.tok + 8 * n + g, use.end - 1) * p.ldx + kw * 128 + 8 * t;
-        auto multiply = [&](int unit, auto is_last) {
-            constexpr bool LAST = decltype(is_last)::value;
-            uint4 b[PLANES][NT][4];  // [.. 32 columns]
+        for (int n = 0; n < NT; ++n) src_x[n] = static_cast<const T *>(p.x) + (int64_t)min(use.tok + 8 * n + g, use.end - 1) * p.ldx + kw * (W * 128) + 8 * t;
+        for (int unit = kw; unit < p.units; unit += p.k_warps) {
+            const int columns = p.kx - unit * (W * 128);  // from here on
+            uint4 b[W][PLANES][NT][4];                    // [.. 32 columns]
+            auto load_x = [&](int h) {
 #pragma unroll
-            for (int pl = 0; pl < PLANES; ++pl)
+                for (int pl = 0; pl < PLANES; ++pl)
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+                    for (int n = 0; n < NT; ++n) {
+                        const T *src = src_x[n] + pl * p.plane_elems + h * 128;
+                        if (columns >= W * 128) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        b[pl][n][i] = !LAST || (int64_t)unit * 128 + 32 * i + 8 * t < p.kx ? __ldg(reinterpret_cast<const uint4 *>(src_x[n] + pl * p.plane_elems + 32 * i)) : make_uint4(0u, 0u, 0u, 0u);
-            ok = __all_sync(0xffffffffu, mbar_wait(my_full + 8u * at.stage, at.phase));
-            if (!ok) return;
-            const uint8_t *src = ring + (warp * kStages + at.stage) * STAGE;
+                            for (int i = 0; i < 4; ++i) b[h][pl][n][i] = __ldg(reinterpret_cast<const uint4 *>(src + 32 * i));
+                        } else {
 #pragma unroll
-            for (int r = 0; r < RT; ++r) {
-                // (what lies past the last column meets zeros of x, rows past the last are not stored)
-                const uint4 q0 = *reinterpret_cast<const uint4 *>(src + r * 1024 + lane * 16), q1 = *reinterpret_cast<const uint4 *>(src + r * 1024 + 512 + lane * 16);
-                const uint32_t word[8] = {q0.x, q0.y, q0.z, q0.w, q1.x, q1.y, q1.z, q1.w};
-#pragma unroll
-                for (int i = 0; i < PER; ++i) {
-                    float c[NT][SUMS][4] = {};
-#pragma unroll
-                    for (int j = i * (8 / PER); j < (i + 1) * (8 / PER); ++j) {
-                        uint32_t a[4];
-                        fragments<T>(decode, word[j], a);
-#pragma unroll
-                        for (int pl = 0; pl < PLANES; ++pl)
-#pragma unroll
-                            for (int n = 0; n < NT; ++n) {
-                                const uint4 &v = b[pl][n][j >> 1];
-                                mma_16816<T>(c[n][pl > 0 ? SUMS - 1 : 0], a, j & 1 ? v.z : v.x, j & 1 ? v.w : v.y);
-                            }
-                    }
-                    const uint32_t s = !LAST || unit * PER + i < p.groups ? *reinterpret_cast<const uint32_t *>(src + CODES + r * SCALES + i * 32 + 4 * g) : 0u;
-                    const float lo = __uint_as_float(s << 16), hi = __uint_as_float(s & 0xFFFF0000u);
-#pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int u = 0; u < SUMS; ++u) {
-                            sum[r][n][u][0] = fmaf(c[n][u][0], lo, sum[r][n][u][0]);
-                            sum[r][n][u][1] = fmaf(c[n][u][1], lo, sum[r][n][u][1]);
-                            sum[r][n][u][2] = fmaf(c[n][u][2], hi, sum[r][n][u][2]);
-                            sum[r][n][u][3] = fmaf(c[n][u][3], hi, sum[r][n][u][3]);
+                            for (int i = 0; i < 4; ++i) b[h][pl][n][i] = h * 128 + 32 * i + 8 * t < columns ? __ldg(reinterpret_cast<const uint4 *>(src + 32 * i)) : make_uint4(0u, 0u, 0u, 0u);
                         }
-                }
-            }
-            __syncwarp();
-            issue();  // into the stage just read
-            at.advance(kStages);
+                    }
+            };
+            if (PLANES * NT == 1)  // before the wait, where registers hold it
 #pragma unroll
-            for (int n = 0; n < NT; ++n) src_x[n] += p.k_warps * 128;
-        };
-        int unit = kw;
-        for (; unit < last_unit && ok; unit += p.k_warps) multiply(unit, std::false_type{});
-        if (unit == last_unit && ok) multiply(unit, std::true_type{});
+                for (int h = 0; h < W; ++h) load_x(h);
+            ok = __all_sync(0xffffffffu, mbar_wait(my_full + 8u * at.stage, at.phase));
+            if (!ok) break;
+            const uint8_t *src = ring + (warp * S::kCount + at.stage) * S::kBytes;
+#pragma unroll
+            for (int h = 0; h < W; ++h) {
+                if (PLANES * NT > 1) load_x(h);
+                uint32_t word[RT][8], scale[RT][PER];
+#pragma unroll
+                for (int r = 0; r < RT; ++r) {
+                    const uint8_t *at_r = src + (r * W + h) * 1024 + lane * 16;
+                    const uint4 q0 = *reinterpret_cast<const uint4 *>(at_r), q1 = *reinterpret_cast<const uint4 *>(at_r + 512);
+                    word[r][0] = q0.x; word[r][1] = q0.y; word[r][2] = q0.z; word[r][3] = q0.w;
+                    word[r][4] = q1.x; word[r][5] = q1.y; word[r][6] = q1.z; word[r][7] = q1.w;
+#pragma unroll
+                    for (int i = 0; i < PER; ++i) scale[r][i] = *reinterpret_cast<const uint32_t *>(src + S::kCodes + r * S::kScales + (h * PER + i) * 32 + 4 * g);
+                }
+                multiply<T, PLANES, RT, NT, GROUP>(decode, word, scale, b[h], sum);
+            }
+            // Into the stage just read, once what was read has been used: a copy does not wait for loads of shared memory still on their way.
+            uint32_t used = 0;
+#pragma unroll
+            for (int r = 0; r < RT; ++r) used |= __float_as_uint(sum[r][0][0][0]);
+            if (!__any_sync(0xffffffffu, (used & nothing) != 0u)) issue();
+            at.advance(S::kCount);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) src_x[n] += p.k_warps * (W * 128);
+        }
         if (!ok && lane == 0) failed = 1;
-        constexpr int WIDTH = RT * 16 + 1;
 #pragma unroll
         for (int r = 0; r < RT; ++r)
 #pragma unroll
@@ -248,37 +307,41 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) gemv_q4_kernel(const _
                     part[(warp * TOK + 8 * n + 2 * t + (i & 1)) * WIDTH + r * 16 + g + 8 * (i >> 1)] = v;
                 }
         __syncthreads();
-        if (failed) break;  // the same for all: it is set before the barrier only
+        if (failed) break;  // whoever reads it late finds it, too, at the next barrier: it is never taken back
         for (int i = threadIdx.x; i < TOK * row_warps * RT * 16; i += kThreads) {
             const int r = i % (RT * 16), share = i / (RT * 16) % row_warps, tok = i / (RT * 16 * row_warps);
-            const int64_t row = (int64_t)(tile0 - rw * RT + share * RT) * 16 + r;
+            const int row = (tile0 - rw * RT + share * RT) * 16 + r;
             if (use.tok + tok >= use.end || row >= p.M) continue;
             float v = 0.0f;
             for (int w = 0; w < p.k_warps; ++w) v += part[((share * p.k_warps + w) * TOK + tok) * WIDTH + r];
             if (p.bias) v += p.bias[use.expert * p.bias_stride + row];
-            static_cast<CT *>(p.y)[(use.tok + tok) * p.ldy + row] = from_float<CT>(v);
+            store(p.y, (int64_t)(use.tok + tok) * p.ldy + row, v, p.y_dtype);
         }
-        __syncthreads();
+        part = buffer ? part - PART : part + PART;
+        buffer = !buffer;
         use.next(p, active, items, per_item, rw * RT);
     }
     if (failed) give_up(&g_gemv_q4_status, STATUS_CONSUMER);
 }
 
-template <typename T, int PLANES, int RT, int NT, int GROUP, typename CT>
+template <typename T, int PLANES, int RT, int NT, int W, int GROUP>
 int launch(Q4Params &p, cudaStream_t st) {
+    using S = Stage<RT, W, GROUP>;
     const int row_warps = kWarps / p.k_warps;
     p.row_items = (p.row_tiles + RT * row_warps - 1) / (RT * row_warps);
     const int64_t items = (int64_t)p.row_items * (p.offsets ? (p.rows < p.n_experts ? p.rows : p.n_experts) : 1), most = (int64_t)sm_count() * kBlocksPerSm;
-    constexpr size_t smem = (size_t)kWarps * (kStages * kStageBytes<RT, GROUP> + 8 * NT * (RT * 16 + 1) * sizeof(float));
+    constexpr size_t smem = (size_t)kWarps * (S::kCount * S::kBytes + 2 * 8 * NT * (RT * 16 + 1) * sizeof(float));
     CUtensorMap mc, ms;
     memset(&mc, 0, sizeof mc);
     memset(&ms, 0, sizeof ms);
     if (p.units > 0) {
-        const uint64_t tiles = (uint64_t)p.row_tiles * (p.offsets ? p.n_experts : 1), scale_row = (uint64_t)(p.groups + 1) * 16;
-        if (int rc = make_map_2d(&mc, CU_TENSOR_MAP_DATA_TYPE_UINT32, p.codes, (uint64_t)p.col_tiles * 128, tiles, (uint64_t)p.col_tiles * kQ4TileBytes, 256, RT, CU_TENSOR_MAP_SWIZZLE_NONE)) return rc;
-        if (int rc = make_map_2d(&ms, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p.scales, scale_row, tiles, scale_row * 2, 128 / GROUP * 16, RT, CU_TENSOR_MAP_SWIZZLE_NONE)) return rc;
+        const cuuint64_t tiles = (cuuint64_t)p.row_tiles * (p.offsets ? p.n_experts : 1), scale_row = (cuuint64_t)(p.groups + 1) * 16;
+        const cuuint64_t dims[3] = {kQ4TileBytes / 4, (cuuint64_t)p.col_tiles, tiles}, strides[2] = {kQ4TileBytes, (cuuint64_t)p.col_tiles * kQ4TileBytes};
+        const cuuint32_t box[3] = {kQ4TileBytes / 4, 2 * W, RT};
+        if (int rc = make_map(&mc, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, p.codes, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE)) return rc;
+        if (int rc = make_map_2d(&ms, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p.scales, scale_row, tiles, scale_row * 2, W * (128 / GROUP) * 16, RT, CU_TENSOR_MAP_SWIZZLE_NONE)) return rc;
     }
-    auto kernel = gemv_q4_kernel<T, PLANES, RT, NT, GROUP, CT>;
+    auto kernel = gemv_q4_kernel<T, PLANES, RT, NT, W, GROUP>;
     static std::atomic<bool> configured[64];  // the shared-memory limit is an attribute of the function on a device
     int dev = 0;
     T81_CUDA_TRY(cudaGetDevice(&dev));
@@ -290,32 +353,30 @@ int launch(Q4Params &p, cudaStream_t st) {
     return T81B200_OK;
 }
 
-template <typename T, int PLANES, int RT, int NT, int GROUP>
-int launch_ct(Q4Params &p, int c_dtype, cudaStream_t st) {
-    switch (c_dtype) {
-        case T81B200_F32: return launch<T, PLANES, RT, NT, GROUP, float>(p, st);
-        case T81B200_BF16: return launch<T, PLANES, RT, NT, GROUP, __nv_bfloat16>(p, st);
-        case T81B200_F16: return launch<T, PLANES, RT, NT, GROUP, __half>(p, st);
-    }
-    return fail(T81B200_EINVAL, "linear_q4: unknown output dtype %d", c_dtype);
+template <typename T, int PLANES, int RT, int NT, int W>
+int launch_group(Q4Params &p, int group, cudaStream_t st) {
+    p.units = (p.units + W - 1) / W;
+    p.k_warps = p.units >= 8 ? 8 : (p.units >= 4 ? 4 : (p.units >= 2 ? 2 : 1));
+    if (group == 32) return launch<T, PLANES, RT, NT, W, 32>(p, st);
+    if (group == 64) return launch<T, PLANES, RT, NT, W, 64>(p, st);
+    return launch<T, PLANES, RT, NT, W, 128>(p, st);
 }
 
 template <typename T, int PLANES, int RT, int NT>
-int launch_group(Q4Params &p, int group, int c_dtype, cudaStream_t st) {
-    if (group == 32) return launch_ct<T, PLANES, RT, NT, 32>(p, c_dtype, st);
-    if (group == 64) return launch_ct<T, PLANES, RT, NT, 64>(p, c_dtype, st);
-    return launch_ct<T, PLANES, RT, NT, 128>(p, c_dtype, st);
+int launch_width(Q4Params &p, int group, cudaStream_t st) {
+    if constexpr (PLANES == 1)
+        if (p.units >= 16) return launch_group<T, PLANES, RT, NT, 2>(p, group, st);
+    return launch_group<T, PLANES, RT, NT, 1>(p, group, st);
 }
 
+// p.units: of 128 columns.
 template <typename T, int PLANES>
-int launch_shape(Q4Params &p, int group, int c_dtype, cudaStream_t st) {
-    p.k_warps = p.units >= 8 ? 8 : (p.units >= 4 ? 4 : (p.units >= 2 ? 2 : 1));
+int launch_shape(Q4Params &p, int group, cudaStream_t st) {
     // two row tiles a warp read each piece of an activation row once for both, where that leaves every block a share
-    const int64_t shares = (int64_t)p.row_tiles * p.k_warps / kWarps * (p.offsets ? (p.rows < p.n_experts ? p.rows : p.n_experts) : 1);
-    const bool wide = shares >= 2 * (int64_t)sm_count() * kBlocksPerSm;
+    const bool wide = (int64_t)p.row_tiles * (p.offsets ? (p.rows < p.n_experts ? p.rows : p.n_experts) : 1) >= 4 * (int64_t)sm_count();
     if constexpr (PLANES == 1)
-        if (p.rows > 8 && !p.offsets) return wide ? launch_group<T, PLANES, 2, 2>(p, group, c_dtype, st) : launch_group<T, PLANES, 1, 2>(p, group, c_dtype, st);
-    return wide ? launch_group<T, PLANES, 2, 1>(p, group, c_dtype, st) : launch_group<T, PLANES, 1, 1>(p, group, c_dtype, st);  // three planes of 16 rows do not fit the registers
+        if (p.rows > 8 && !p.offsets) return wide ? launch_width<T, PLANES, 2, 2>(p, group, st) : launch_width<T, PLANES, 1, 2>(p, group, st);
+    return wide ? launch_width<T, PLANES, 2, 1>(p, group, st) : launch_width<T, PLANES, 1, 1>(p, group, st);  // three planes of 16 rows do not fit the registers
 }
 
 // Rows that the kernels read where they are: 16-bit, on 16-byte boundaries, whole pieces of eight columns.
@@ -337,9 +398,9 @@ int product_q4(const char *name, const uint8_t *codes, const void *scales, const
     if (reinterpret_cast<uintptr_t>(codes) % 16 != 0 || reinterpret_cast<uintptr_t>(scales) % 16 != 0) return fail(T81B200_EALIGN, "%s: codes and scales must be 16-byte aligned", name);
     Q4Params p = {};
     p.codes = codes; p.scales = static_cast<const __nv_bfloat16 *>(scales); p.bias = bias;
-    p.x = B; p.ldx = ldb; p.kx = K;
-    p.y = C; p.ldy = ldc;
-    p.M = M; p.rows = N;
+    p.x = B; p.ldx = ldb; p.kx = (int)K;
+    p.y = C; p.ldy = ldc; p.y_dtype = c_dtype;
+    p.M = (int)M; p.rows = (int)N;
     p.offsets = offsets; p.n_experts = n_experts;
     p.bias_stride = M;
     p.col_tiles = (int)q4_col_tiles(K); p.groups = (int)q4_groups(K, group); p.units = (int)((K + 127) / 128); p.row_tiles = (int)q4_row_tiles(M);
@@ -350,13 +411,14 @@ int product_q4(const char *name, const uint8_t *codes, const void *scales, const
             return fail(T81B200_EWORKSPACE, "%s: %zu bytes of 16-byte aligned workspace needed, %zu given", name, need, workspace_bytes);
         if (int rc = stage_planes(B, b_dtype, T81B200_LAYOUT_NK, ldb, N, K, 3, workspace, st)) return rc;
         p.x = workspace;
-        p.ldx = p.kx = staged_row(K);
+        p.ldx = staged_row(K);
+        p.kx = (int)p.ldx;
         p.plane_elems = N * p.ldx;
     }
     if (b_dtype != T81B200_F32 && K > 0 && N >= (offsets ? 8 * (int64_t)n_experts : 33))
         return gemm_q4_tc_launch(codes, scales, bias, C, M, p.x, b_dtype == T81B200_F16, p.ldx, c_dtype, ldc, N, K, group, offsets, n_experts, st);
-    if (b_dtype == T81B200_F32) return launch_shape<__nv_bfloat16, 3>(p, group, c_dtype, st);
-    return b_dtype == T81B200_BF16 ? launch_shape<__nv_bfloat16, 1>(p, group, c_dtype, st) : launch_shape<__half, 1>(p, group, c_dtype, st);
+    if (b_dtype == T81B200_F32) return launch_shape<__nv_bfloat16, 3>(p, group, st);
+    return b_dtype == T81B200_BF16 ? launch_shape<__nv_bfloat16, 1>(p, group, st) : launch_shape<__half, 1>(p, group, st);
 }
 
 }  // namespace
