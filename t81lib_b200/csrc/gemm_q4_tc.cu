@@ -39,8 +39,8 @@ namespace {
 
 constexpr int BM = 128, BK = 64, CHUNK = 128;
 constexpr int A_ATOM_BYTES = BM * BK * 2, A_CHUNK_BYTES = 2 * A_ATOM_BYTES;  // 16 and 32 KB
-constexpr int RAW_CODES = 8 * 1024, RAW_BYTES = RAW_CODES + 1024;            // a chunk's codes and scales
-constexpr int A_STAGES = 3, RAW_STAGES = 4, B_MAX = 12, MAX_SPLITS = 4;
+constexpr int RAW_CODES = 8 * 1024;                                          // a chunk's codes; its scales lie behind them
+constexpr int A_STAGES = 3, RAW_MAX = 8, B_MAX = 12, MAX_SPLITS = 4;
 constexpr int NUM_THREADS = 23 * 32, EPILOGUE_WARP0 = 2, CONVERTER_WARP0 = 6, CONVERTERS = 8, RAW_WARP = 22;
 constexpr int FINISHERS = (RAW_WARP - EPILOGUE_WARP0) / 4;  // groups of four warps that finish a tile alone in its launch
 constexpr int BARRIER_BYTES = 512, MOST_EXPERTS = 1024;
@@ -62,7 +62,7 @@ struct Q4TcParams {
     int m_tiles, n_tiles;       // 256-row pair tiles; tiles of bn rows of x (one matrix)
     int bn, box_rows;           // most rows of x a tile, a multiple of 32; rows of a TMA box
     int n_atoms, n_chunks;
-    int splits, b_stages, one_tile, out_bytes;
+    int splits, raw_stages, b_stages, one_tile, out_bytes, list_bytes;
     int vec;                    // 16-byte stores are possible
 };
 
@@ -176,30 +176,29 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_co
                   const __grid_constant__ Q4TcParams p) {
     constexpr bool F16 = std::is_same<T, __half>::value;
     constexpr int PER = CHUNK / GROUP;
-    constexpr uint32_t RAW_TX = RAW_CODES + 8 * PER * 32;
+    constexpr uint32_t RAW_BYTES = RAW_CODES + 8 * PER * 32;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ int32_t list[EXPERTS ? 2 * (MOST_EXPERTS + 1) : 1];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t *gen_base = smem_raw + (base - smem_u32(smem_raw));
     const uint32_t b_stage_bytes = (uint32_t)p.bn * (BK * 2 / 2);  // this CTA's half of the rows
-    const uint32_t b_off = A_STAGES * A_CHUNK_BYTES, raw_off = b_off + (uint32_t)p.b_stages * b_stage_bytes, out_off = raw_off + RAW_STAGES * RAW_BYTES;
+    const uint32_t b_off = A_STAGES * A_CHUNK_BYTES, raw_off = b_off + (uint32_t)p.b_stages * b_stage_bytes, out_off = raw_off + (uint32_t)p.raw_stages * RAW_BYTES;
     const uint32_t bars = base + out_off + (uint32_t)p.out_bytes;
     auto a_full = [&](int s) { return bars + 8u * s; };
     auto a_empty = [&](int s) { return bars + 8u * (A_STAGES + s); };
     auto raw_full = [&](int s) { return bars + 8u * (2 * A_STAGES + s); };
-    auto raw_empty = [&](int s) { return bars + 8u * (2 * A_STAGES + RAW_STAGES + s); };
-    auto acc_full = [&](int s) { return bars + 8u * (2 * A_STAGES + 2 * RAW_STAGES + s); };
-    auto acc_empty = [&](int s) { return bars + 8u * (2 * A_STAGES + 2 * RAW_STAGES + 2 + s); };
-    auto b_full = [&](int s) { return bars + 8u * (2 * A_STAGES + 2 * RAW_STAGES + 4 + s); };
-    auto b_empty = [&](int s) { return bars + 8u * (2 * A_STAGES + 2 * RAW_STAGES + 4 + B_MAX + s); };
-    const uint32_t tmem_slot = bars + 8u * (2 * A_STAGES + 2 * RAW_STAGES + 4 + 2 * B_MAX);
+    auto raw_empty = [&](int s) { return bars + 8u * (2 * A_STAGES + RAW_MAX + s); };
+    auto acc_full = [&](int s) { return bars + 8u * (2 * A_STAGES + 2 * RAW_MAX + s); };
+    auto acc_empty = [&](int s) { return bars + 8u * (2 * A_STAGES + 2 * RAW_MAX + 2 + s); };
+    auto b_full = [&](int s) { return bars + 8u * (2 * A_STAGES + 2 * RAW_MAX + 4 + s); };
+    auto b_empty = [&](int s) { return bars + 8u * (2 * A_STAGES + 2 * RAW_MAX + 4 + B_MAX + s); };
+    const uint32_t tmem_slot = bars + 8u * (2 * A_STAGES + 2 * RAW_MAX + 4 + 2 * B_MAX);
 
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
     const int half = (int)(rank & 1u), slice = (int)(rank >> 1);
     if (threadIdx.x == 0) {
         for (int s = 0; s < A_STAGES; ++s) { mbar_init(a_full(s), 2 * CONVERTERS); mbar_init(a_empty(s), 1); }
-        for (int s = 0; s < RAW_STAGES; ++s) { mbar_init(raw_full(s), 1); mbar_init(raw_empty(s), CONVERTERS); }
+        for (int s = 0; s < RAW_MAX; ++s) { mbar_init(raw_full(s), 1); mbar_init(raw_empty(s), CONVERTERS); }
         for (int s = 0; s < 2; ++s) { mbar_init(acc_full(s), 1); mbar_init(acc_empty(s), 8); }
         for (int s = 0; s < B_MAX; ++s) { mbar_init(b_full(s), 1); mbar_init(b_empty(s), 1); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -220,8 +219,8 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_co
 
     TileList<EXPERTS> tiles;
     if constexpr (EXPERTS) {
-        tiles.first = list;
-        tiles.before = list + MOST_EXPERTS + 1;
+        tiles.first = reinterpret_cast<int32_t *>(gen_base + (bars - base) + BARRIER_BYTES);
+        tiles.before = tiles.first + p.n_experts + 1;
     }
     const int total_tiles = tiles.build(p);
     const int n_clusters = (int)gridDim.x / (2 * p.splits), cluster_id = (int)blockIdx.x / (2 * p.splits);
@@ -288,13 +287,13 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_co
                 ok = mbar_wait(raw_empty(raw.stage), raw.phase ^ 1);
                 if (!ok) break;
                 if (elect_one()) {
-                    mbar_arrive_expect_tx(raw_full(raw.stage), RAW_TX);
+                    mbar_arrive_expect_tx(raw_full(raw.stage), RAW_BYTES);
                     const uint32_t dst = base + raw_off + (uint32_t)raw.stage * RAW_BYTES;
                     tma_load_2d(dst, &map_codes, c * 256, y, raw_full(raw.stage));
                     tma_load_2d(dst + RAW_CODES, &map_scales, c * PER * 16, y, raw_full(raw.stage));
                 }
                 __syncwarp();
-                raw.advance(RAW_STAGES);
+                raw.advance(p.raw_stages);
             }
         }
         if (!ok) give_up(&g_q4_status, STATUS_PRODUCER);
@@ -373,11 +372,11 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_co
 #pragma unroll
         for (int s = 0; s < 2; ++s) off[s] = (uint32_t)(cw * 16 + g) * 128u + (uint32_t)((4 * (s ^ (int)swap) + t4) ^ g) * 16u;
         const Q4Decode<T> decode;
-        // Slots of the raw ring (four) stay with a group.  Those of the operand ring (three) change hands: a group waits for the MMAs of the slot's
+        // Slots of the raw ring (an even number) stay with a group.  Those of the operand ring (three) change hands: a group waits for the MMAs of the slot's
         // last chunk, k - 3.  It has seen those of k - 5 end when it took its own last chunk, and MMAs end in order, so those of k - 6, the
         // slot's use before, have ended too, and the wait cannot be a whole use behind.
         Ring a, raw;
-        if (group == 1) { a.advance(A_STAGES); raw.advance(RAW_STAGES); }
+        if (group == 1) { a.advance(A_STAGES); raw.advance(p.raw_stages); }
         bool ok = true;
         const int span = c1 - c0;
         int c = group;  // of the tile's span
@@ -456,8 +455,8 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_co
                     mbar_arrive_leader(a_full(a.stage));
                     mbar_arrive(raw_empty(raw.stage));
                 }
-                raw.advance(RAW_STAGES);
-                raw.advance(RAW_STAGES);
+                raw.advance(p.raw_stages);
+                raw.advance(p.raw_stages);
                 a.advance(A_STAGES);
                 a.advance(A_STAGES);
             }
@@ -519,7 +518,7 @@ double step_cost(int n) {
 template <typename T, int GROUP, typename CT, bool EXPERTS>
 int launch(const CUtensorMap &mc, const CUtensorMap &ms, const CUtensorMap &mx, const Q4TcParams &p, int clusters, size_t smem, cudaStream_t st) {
     auto kern = gemm_q4_tc_kernel<T, GROUP, CT, EXPERTS>;
-    constexpr int most = SMEM_LIMIT - (EXPERTS ? 2 * (MOST_EXPERTS + 1) * 4 + 256 : 64);
+    constexpr int most = SMEM_LIMIT;
     static std::atomic<bool> configured[64];
     int dev = 0;
     T81_CUDA_TRY(cudaGetDevice(&dev));
@@ -596,11 +595,16 @@ int gemm_q4_tc_launch(const uint8_t *codes, const void *scales, const float *bia
         clusters = p.one_tile ? tiles : resident;
     }
     p.out_bytes = p.one_tile ? 0 : 4 * 1024 * (int)dtype_size(c_dtype);
-    const int limit = SMEM_LIMIT - (offsets ? 2 * (MOST_EXPERTS + 1) * 4 + 256 : 64);
-    const int fixed = A_STAGES * A_CHUNK_BYTES + RAW_STAGES * RAW_BYTES + p.out_bytes + BARRIER_BYTES + 1024, stage = p.bn * BK;
-    const int fit = (limit - fixed) / stage;
-    p.b_stages = fit > B_MAX ? B_MAX : fit;
-    const size_t smem = (size_t)fixed + (size_t)p.b_stages * stage;
+    p.list_bytes = offsets ? 2 * (experts + 1) * 4 : 0;
+    // What is left after four stages of activations goes to the codes, two stages for either group of converters at least, the rest to the
+    // activations again.
+    const int raw = RAW_CODES + CHUNK / group * 256, stage = p.bn * BK;
+    const int room = SMEM_LIMIT - A_STAGES * A_CHUNK_BYTES - p.out_bytes - BARRIER_BYTES - p.list_bytes - 1024;
+    p.raw_stages = (room - 4 * stage) / raw / 2 * 2;
+    p.raw_stages = p.raw_stages > RAW_MAX ? RAW_MAX : (p.raw_stages < 4 ? 4 : p.raw_stages);
+    p.b_stages = (room - p.raw_stages * raw) / stage;
+    p.b_stages = p.b_stages > B_MAX ? B_MAX : p.b_stages;
+    const size_t smem = (size_t)(SMEM_LIMIT - room) + (size_t)p.raw_stages * raw + (size_t)p.b_stages * stage;
     CUtensorMap mc, ms, mx;
     const int64_t tiles16 = (int64_t)experts * p.row_tiles, ktiles = q4_col_tiles(K);
     if (int rc = make_map_2d(&mc, CU_TENSOR_MAP_DATA_TYPE_UINT32, codes, (uint64_t)ktiles * 128, (uint64_t)tiles16, (uint64_t)ktiles * kQ4TileBytes, 256, 8, CU_TENSOR_MAP_SWIZZLE_NONE)) return rc;

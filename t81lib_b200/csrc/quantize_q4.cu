@@ -4,14 +4,13 @@
 // the whole number nearest to w / s, ties to even, held in -8 .. 7.  Eight steps reach from 0 to the largest value and seven the
 // other way.  Five bits for the scale make code * s a bf16 number, and cost little: N(0, 1) weights in groups of 128 come back with
 // a mean square error 0.3 % above that of an unrounded scale.
-// The code is exact: w times 1 / s finds it or a neighbour, and the rest w - code * s, which has no rounding error (both are
-// multiples of w's last place, and the difference is below s), decides.
-//
 // Bound by memory: a weight is read once, half a byte is written.  A warp holds 16 rows x 128 columns in registers, a lane eight columns
 // of two rows at a time as the format has them: 64 (16-bit) or 128 bytes of a row side by side per load.
 #include "common.cuh"
 #include "launch_order.cuh"
 #include "q4.cuh"
+
+#include <type_traits>
 
 namespace t81b200 {
 
@@ -21,38 +20,71 @@ constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr float kMost = 8.507059173023462e37f;   // 2^126: larger magnitudes count as this, so that 8 s is finite
 constexpr float kLeast = 7.888609052210118e-31f; // 2^-100: a group of smaller ones is zero (s would leave the normal numbers)
 
-// Eight neighbouring elements of a row as fp32; columns at and past `left` are 0.
+// Eight neighbouring elements of a row as they lie in memory.
+template <typename T> struct Eight { uint4 w[sizeof(T) / 2]; };
+
+// Columns at and past `left` are 0.  VEC: the row lies on 16-byte boundaries.
 template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T *src, int64_t left, float (&v)[8]) {
+__device__ __forceinline__ Eight<T> load8(const T *src, int64_t left) {
+    Eight<T> e;
     if (VEC && left >= 8) {
-        if constexpr (sizeof(T) == 4) {
-            const float4 a = __ldcs(reinterpret_cast<const float4 *>(src)), b = __ldcs(reinterpret_cast<const float4 *>(src) + 1);
-            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-        } else {
-            const uint4 a = __ldcs(reinterpret_cast<const uint4 *>(src));
-            const T *e = reinterpret_cast<const T *>(&a);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = to_float<T>(e[i]);
-        }
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) e.w[i] = __ldcs(reinterpret_cast<const uint4 *>(src) + i);
     } else {
+        T v[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = i < left ? to_float<T>(src[i]) : 0.0f;
+        for (int i = 0; i < 8; ++i) v[i] = i < left ? src[i] : from_float<T>(0.0f);
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) e.w[i] = reinterpret_cast<const uint4 *>(v)[i];
     }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = v[i] != v[i] ? 0.0f : fminf(fmaxf(v[i], -kMost), kMost);  // no number: 0
+    return e;
 }
 
-// The group's value of largest magnitude over the four lanes of a row, the first of equals: a lane's columns lie before the next one's.
-__device__ __forceinline__ float largest_of_lanes(float m, int t) {
+// Largest and smallest of the elements, and whether one is no number or infinite (`probe` stays 0 otherwise): two elements at a time in
+// 16-bit types.
+template <typename T> struct Extremes {
+    float high = 0.0f, low = 0.0f, probe = 0.0f;
+    __device__ __forceinline__ void take(const Eight<T> &e) {
 #pragma unroll
-    for (int d = 1; d < 4; d <<= 1) {
-        const float o = __shfl_xor_sync(0xffffffffu, m, d);
-        const bool other_first = (t & d) != 0;
-        if (fabsf(o) > fabsf(m) || (other_first && fabsf(o) == fabsf(m))) m = o;
+        for (int i = 0; i < 8; ++i) {
+            const float x = reinterpret_cast<const float *>(&e)[i];
+            high = fmaxf(high, x);
+            low = fminf(low, x);
+            probe = fmaf(x, 0.0f, probe);
+        }
     }
-    return m;
+    __device__ __forceinline__ void done() {}
+};
+template <typename T, typename T2> struct Extremes16 {
+    T2 high2 = T2(from_float<T>(0.0f), from_float<T>(0.0f)), low2 = high2, probe2 = high2;
+    float high, low, probe;
+    __device__ __forceinline__ void take(const Eight<T> &e) {
+        const T2 zero(from_float<T>(0.0f), from_float<T>(0.0f));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const T2 x = reinterpret_cast<const T2 *>(&e)[i];
+            high2 = __hmax2(high2, x);
+            low2 = __hmin2(low2, x);
+            probe2 = __hfma2(x, zero, probe2);
+        }
+    }
+    __device__ __forceinline__ void done() {
+        high = fmaxf(to_float<T>(high2.x), to_float<T>(high2.y));
+        low = fminf(to_float<T>(low2.x), to_float<T>(low2.y));
+        probe = to_float<T>(probe2.x) + to_float<T>(probe2.y);
+    }
+};
+template <> struct Extremes<__nv_bfloat16> : Extremes16<__nv_bfloat16, __nv_bfloat162> {};
+template <> struct Extremes<__half> : Extremes16<__half, __half2> {};
+
+template <typename T> __device__ __forceinline__ float element(const Eight<T> &e, int i) {
+    const uint32_t *w = reinterpret_cast<const uint32_t *>(&e);
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+    else if constexpr (std::is_same<T, __nv_bfloat16>::value) return __uint_as_float(i & 1 ? w[i >> 1] & 0xFFFF0000u : w[i >> 1] << 16);
+    else return __half2float(__ushort_as_half((unsigned short)(w[i >> 1] >> (16 * (i & 1)))));
 }
-__device__ __forceinline__ float larger(float first, float then) { return fabsf(then) > fabsf(first) ? then : first; }
+// What the rule makes of it: no number counts as 0, magnitudes above kMost as that.
+__device__ __forceinline__ float tamed(float v) { return v != v ? 0.0f : fminf(fmaxf(v, -kMost), kMost); }
 
 // m / -8 rounded to five significant bits, ties to even.
 __device__ __forceinline__ float scale_of(float m) {
@@ -62,88 +94,123 @@ __device__ __forceinline__ float scale_of(float m) {
     return __uint_as_float(b & 0xFFF80000u);
 }
 
-// code + 8 of w.
-__device__ __forceinline__ uint32_t code_of(float w, float s, float inverse) {
-    float q = rintf(w * inverse);
-    const float half = 0.5f * fabsf(s), rest = copysignf(1.0f, s) * fmaf(-q, s, w);
-    const bool odd = (__float2int_rn(q) & 1) != 0;
-    if (rest > half || (odd && rest == half)) q += 1.0f;
-    else if (rest < -half || (odd && rest == -half)) q -= 1.0f;
-    return (uint32_t)(__float2int_rn(fminf(fmaxf(q, -8.0f), 7.0f)) + 8);
+// 1.5 * 2^23 + 8 plus the code of w in its last bits.  The quotient is the correctly rounded one (one correction by the exact rest, from the
+// correctly rounded reciprocal), which meets a border between two codes only where w / s does: w / s is at least 2^-23 / (s's
+// mantissa) of its binade from one otherwise, more than half a last place.  Adding 1.5 * 2^23 rounds it, ties to even.
+__device__ __forceinline__ uint32_t code_bits(float w, float s, float inverse) {
+    float q = w * inverse;
+    q = fmaf(fmaf(-q, s, w), inverse, q);
+    return __float_as_uint(fminf(q, 7.0f) + 12582920.0f);  // (the largest of its sign comes to -8.26 at most, which is -8)
 }
+constexpr uint32_t kCodeBits = 0x4B400000u;  // what code_bits has beside the code
 
 // A block takes 16 rows, its warps units of 128 columns in turn.
 template <typename T, int GROUP, bool VEC>
 __global__ void __launch_bounds__(kThreads) quantize_q4_kernel(const T *__restrict__ w, int64_t rows, int64_t cols, int64_t ld, int64_t matrix_stride,
                                                                uint4 *__restrict__ codes, __nv_bfloat16 *__restrict__ scales) {
+    // A step is a group of 128 columns, or 64 columns of smaller groups; a lane has eight columns of two rows of each half of 64.
+    constexpr int TILES = GROUP == 128 ? 2 : 1, PER_TILE = GROUP == 32 ? 2 : 1;
     __shared__ float most[kWarps][16];
-    const int64_t row_tiles = q4_row_tiles(rows), col_tiles = q4_col_tiles(cols), groups = q4_groups(cols, GROUP), units = (cols + 127) / 128;
+    const int64_t row_tiles = q4_row_tiles(rows), col_tiles = q4_col_tiles(cols), groups = q4_groups(cols, GROUP), steps = (col_tiles + TILES - 1) / TILES;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int64_t matrix = blockIdx.y, T16 = blockIdx.x, out_tile = matrix * row_tiles + T16;
     float largest[2] = {0.0f, 0.0f};  // of the lane's rows
-    for (int64_t unit = warp; unit < units; unit += kWarps) {
-        float v[2][2][2][8];  // [tile][half of its columns][row of the lane]
+    const T *const matrix_at = w + matrix * matrix_stride;
+    auto load = [&](int64_t step, Eight<T>(&v)[TILES][2][2]) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int half = 0; half < 2; ++half)
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    const int64_t row = 16 * T16 + g + 8 * r, col = unit * 128 + 64 * c + 32 * half + 8 * t;
-                    load8<T, VEC>(w + matrix * matrix_stride + row * ld + col, row < rows ? cols - col : 0, v[c][half][r]);
-                }
-        float m[2][2][2];
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
+        for (int c = 0; c < TILES; ++c)
 #pragma unroll
             for (int half = 0; half < 2; ++half)
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    float x = v[c][half][r][0];
-#pragma unroll
-                    for (int i = 1; i < 8; ++i) x = larger(x, v[c][half][r][i]);
-                    m[c][half][r] = largest_of_lanes(x, t);
+                    const int64_t row = 16 * T16 + g + 8 * r, col = step * (64 * TILES) + 64 * c + 32 * half + 8 * t;
+                    v[c][half][r] = load8<T, VEC>(matrix_at + (row < rows ? row : 0) * ld + col, row < rows ? cols - col : 0);
                 }
-        float s[2][2][2];
+    };
+    for (int64_t step = warp; step < steps; step += kWarps) {
+        Eight<T> v[TILES][2][2];  // [tile][half of its columns][row of the lane]
+        load(step, v);
+        float s[PER_TILE][2];  // [group][row]
+        bool wild = false;
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            if (GROUP >= 64)
+        for (int u = 0; u < PER_TILE; ++u)
 #pragma unroll
-                for (int c = 0; c < 2; ++c) m[c][0][r] = m[c][1][r] = larger(m[c][0][r], m[c][1][r]);
-            if (GROUP == 128) m[0][0][r] = m[0][1][r] = m[1][0][r] = m[1][1][r] = larger(m[0][0][r], m[1][0][r]);
+            for (int r = 0; r < 2; ++r) {
+                Extremes<T> all;
 #pragma unroll
-            for (int c = 0; c < 2; ++c)
+                for (int c = 0; c < TILES; ++c)
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    s[c][half][r] = scale_of(m[c][half][r]);
-                    largest[r] = fmaxf(largest[r], fabsf(s[c][half][r]));
+                    for (int half = (GROUP == 32 ? u : 0); half < (GROUP == 32 ? u + 1 : 2); ++half) all.take(v[c][half][r]);
+                all.done();
+                float high = all.high, low = all.low;
+#pragma unroll
+                for (int d = 1; d < 4; d <<= 1) {
+                    high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, d));
+                    low = fminf(low, __shfl_xor_sync(0xffffffffu, low, d));
                 }
-        }
-        constexpr int PER = 128 / GROUP;  // groups of the 128 columns; lane t == 0 of a row writes them
-        if (t == 0) {
+                float m = high > -low ? high : low;
+                const bool here = all.probe != 0.0f || high > kMost || low < -kMost;
+                wild = wild || here;
+                if (__any_sync(0xffffffffu, here || (high == -low && high > 0.0f))) {
+                    // equal magnitudes of both signs, the first of which gives the sign, or what the rule tames: element by element
+                    m = 0.0f;
 #pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                const int64_t u = unit * PER + i;
-                if (u >= groups) break;
-                const int c = i * GROUP / 64, half = i * GROUP % 64 / 32;
-                const __nv_bfloat162 pair(__float2bfloat16_rn(s[c][half][0]), __float2bfloat16_rn(s[c][half][1]));
-                *reinterpret_cast<uint32_t *>(scales + (out_tile * (groups + 1) + u) * 16 + 2 * g) = bf162_bits(pair);
+                    for (int c = 0; c < TILES; ++c)
+#pragma unroll
+                        for (int half = (GROUP == 32 ? u : 0); half < (GROUP == 32 ? u + 1 : 2); ++half) {
+                            float mine = 0.0f;
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                const float x = tamed(element(v[c][half][r], i));
+                                if (fabsf(x) > fabsf(mine)) mine = x;
+                            }
+#pragma unroll
+                            for (int d = 1; d < 4; d <<= 1) {  // a lane's columns lie before the next one's
+                                const float o = __shfl_xor_sync(0xffffffffu, mine, d);
+                                if (fabsf(o) > fabsf(mine) || ((t & d) != 0 && fabsf(o) == fabsf(mine))) mine = o;
+                            }
+                            if (fabsf(mine) > fabsf(m)) m = mine;
+                        }
+                }
+                s[u][r] = scale_of(m);
+            }
+        const bool wild_warp = __any_sync(0xffffffffu, wild);
+#pragma unroll
+        for (int u = 0; u < PER_TILE; ++u) {
+#pragma unroll
+            for (int r = 0; r < 2; ++r) largest[r] = fmaxf(largest[r], fabsf(s[u][r]));
+            const int64_t group = step * PER_TILE + u;
+            if (t == 0 && group < groups) {
+                const __nv_bfloat162 pair(__float2bfloat16_rn(s[u][0]), __float2bfloat16_rn(s[u][1]));
+                *reinterpret_cast<uint32_t *>(scales + (out_tile * (groups + 1) + group) * 16 + 2 * g) = bf162_bits(pair);
             }
         }
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            if (unit * 2 + c >= col_tiles) break;
+        for (int c = 0; c < TILES; ++c) {
+            if (TILES == 2 && step * 2 + c >= col_tiles) break;
             uint32_t word[4] = {0u, 0u, 0u, 0u};
+            auto encode = [&](auto tame) {
 #pragma unroll
-            for (int half = 0; half < 2; ++half)
+                for (int half = 0; half < 2; ++half)
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    const float scale = s[c][half][r], inverse = scale != 0.0f ? 1.0f / scale : 0.0f;
+                    for (int r = 0; r < 2; ++r) {
+                        // (a group of zeros: scale and reciprocal 0 make every code 0, that is 8)
+                        const float scale = s[GROUP == 32 ? half : 0][r], inverse = scale != 0.0f ? 1.0f / scale : 0.0f;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)  // column 4 (j % 2) + 2 (register / 2) + h of the lane's eight
-                        word[2 * half + (i >> 2)] |= (scale != 0.0f ? code_of(v[c][half][r][i], scale, inverse) : 8u) << (4 * (r + 2 * ((i >> 1) & 1)) + 16 * (i & 1));
-                }
-            codes[(out_tile * col_tiles + unit * 2 + c) * 32 + lane] = make_uint4(word[0], word[1], word[2], word[3]);
+                        for (int i = 0; i < 8; ++i) {  // column 4 (j % 2) + 2 (register / 2) + h of the lane's eight
+                            const float x = element(v[c][half][r], i);
+                            const int shift = 4 * (r + 2 * ((i >> 1) & 1)) + 16 * (i & 1);
+                            word[2 * half + (i >> 2)] += code_bits(decltype(tame)::value ? tamed(x) : x, scale, inverse) << shift;
+                        }
+                    }
+            };
+            if (wild_warp) encode(std::true_type{});
+            else encode(std::false_type{});
+            // what the codes' numbers have beside them, the same in every word
+            constexpr uint32_t beside = kCodeBits * 0x11111111u;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) word[j] -= beside;
+            codes[(out_tile * col_tiles + step * TILES + c) * 32 + lane] = make_uint4(word[0], word[1], word[2], word[3]);
         }
     }
     if (t == 0) {
@@ -159,39 +226,78 @@ __global__ void __launch_bounds__(kThreads) quantize_q4_kernel(const T *__restri
     }
 }
 
-// One warp per tile; every value is exact in fp32 and in bf16.
+// Every value is exact in fp32 and in bf16.  A warp takes a tile; fp32 halves of eight columns change places between two lanes, so that a
+// store fills whole sectors.  Rows off 16-byte boundaries go through shared memory, four tiles in turn, so that a warp's stores lie side by
+// side.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads) dequantize_q4_kernel(const uint4 *__restrict__ codes, const __nv_bfloat16 *__restrict__ scales, int64_t matrices, int64_t rows,
                                                                  int64_t cols, int group, T *__restrict__ out) {
+    constexpr int TILES = VEC ? 1 : 4;
+    __shared__ T through[VEC ? 1 : kWarps][VEC ? 1 : 16][VEC ? 1 : 65];
     wait_for_kernel_ahead();
-    const int64_t row_tiles = q4_row_tiles(rows), col_tiles = q4_col_tiles(cols), groups = q4_groups(cols, group);
-    const int64_t tile = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
-    if (tile >= matrices * row_tiles * col_tiles) return;
-    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int64_t c = tile % col_tiles, all_T = tile / col_tiles, matrix = all_T / row_tiles, T16 = all_T % row_tiles;
-    const uint4 q = codes[tile * 32 + lane];
-    const uint32_t word[4] = {q.x, q.y, q.z, q.w};
+    const int64_t row_tiles = q4_row_tiles(rows), col_tiles = q4_col_tiles(cols), groups = q4_groups(cols, group), across = (col_tiles + TILES - 1) / TILES;
+    const int64_t at = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+    if (at >= matrices * row_tiles * across) return;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int64_t c0 = at % across * TILES, all_T = at / across, matrix = all_T / row_tiles, T16 = all_T % row_tiles;
+    T *const matrix_at = out + matrix * rows * cols;
+    uint4 q[TILES];
+    uint32_t pair[TILES][2];
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        const int64_t col = 64 * c + 32 * half + 8 * t;
-        if (col >= cols) continue;
-        const uint32_t pair = *reinterpret_cast<const uint32_t *>(scales + (all_T * (groups + 1) + col / group) * 16 + 2 * g);
+    for (int c = 0; c < TILES; ++c) {
+        const bool there = c0 + c < col_tiles;
+        q[c] = there ? __ldcs(codes + (all_T * col_tiles + c0 + c) * 32 + lane) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const int64_t row = 16 * T16 + g + 8 * r;
-            if (row >= rows) continue;
-            const float s = __uint_as_float(r ? pair & 0xFFFF0000u : pair << 16);
-            T v[8];
+        for (int half = 0; half < 2; ++half) {
+            const int64_t col = 64 * (c0 + c) + 32 * half;
+            pair[c][half] = col < cols ? *reinterpret_cast<const uint32_t *>(scales + (all_T * (groups + 1) + col / group) * 16 + 2 * g) : 0u;
+        }
+    }
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                v[i] = from_float<T>((float)((int)((word[2 * half + (i >> 2)] >> (4 * (r + 2 * ((i >> 1) & 1)) + 16 * (i & 1))) & 15u) - 8) * s);
-            T *dst = out + (matrix * rows + row) * cols + col;
-            if (VEC && col + 8 <= cols) {
+    for (int c = 0; c < TILES; ++c) {
+        if (c0 + c >= col_tiles) break;
+        const uint32_t word[4] = {q[c].x, q[c].y, q[c].z, q[c].w};
+        if (!VEC) __syncwarp();
 #pragma unroll
-                for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4 *>(dst)[i] = reinterpret_cast<const uint4 *>(v)[i];
-            } else {
+        for (int half = 0; half < 2; ++half)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) if (col + i < cols) dst[i] = v[i];
+            for (int r = 0; r < 2; ++r) {
+                const float s = __uint_as_float(r ? pair[c][half] & 0xFFFF0000u : pair[c][half] << 16);
+                __align__(16) T v[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    v[i] = from_float<T>((float)((int)((word[2 * half + (i >> 2)] >> (4 * (r + 2 * ((i >> 1) & 1)) + 16 * (i & 1))) & 15u) - 8) * s);
+                if constexpr (VEC && sizeof(T) == 4) {  // (rows of whole 16 bytes end with one)
+                    const bool odd = (t & 1) != 0;
+                    float mine[4], other[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        other[i] = __shfl_xor_sync(0xffffffffu, odd ? v[i] : v[4 + i], 1);
+                        mine[i] = odd ? v[4 + i] : v[i];
+                    }
+                    // the pair's sixteen columns: the even lane has columns 0 .. 3 and 8 .. 11, the odd one 4 .. 7 and 12 .. 15
+                    const int64_t row = 16 * T16 + g + 8 * r, col = 64 * (c0 + c) + 32 * half + 16 * (t >> 1) + 4 * (t & 1);
+                    float *at_row = reinterpret_cast<float *>(matrix_at) + row * cols + col;
+                    if (row < rows && col < cols) *reinterpret_cast<float4 *>(at_row) = odd ? make_float4(other[0], other[1], other[2], other[3]) : make_float4(mine[0], mine[1], mine[2], mine[3]);
+                    if (row < rows && col + 8 < cols) *reinterpret_cast<float4 *>(at_row + 8) = odd ? make_float4(mine[0], mine[1], mine[2], mine[3]) : make_float4(other[0], other[1], other[2], other[3]);
+                } else if constexpr (VEC) {
+                    const int64_t row = 16 * T16 + g + 8 * r, col = 64 * (c0 + c) + 32 * half + 8 * t;
+                    if (row < rows && col < cols) *reinterpret_cast<uint4 *>(matrix_at + row * cols + col) = *reinterpret_cast<const uint4 *>(v);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) through[warp][g + 8 * r][32 * half + 8 * t + i] = v[i];
+                }
+            }
+        if constexpr (!VEC) {
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int64_t row = 16 * T16 + i;
+#pragma unroll
+                for (int k = 0; k < 64; k += 32) {
+                    const int64_t col = 64 * (c0 + c) + k + lane;
+                    if (row < rows && col < cols) matrix_at[row * cols + col] = through[warp][i][k + lane];
+                }
             }
         }
     }
@@ -215,9 +321,9 @@ int launch_quantize(const void *w, int64_t matrices, int64_t rows, int64_t cols,
 
 template <typename T>
 int launch_dequantize(const uint8_t *codes, const void *scales, int64_t matrices, int64_t rows, int64_t cols, int group, void *out, cudaStream_t st) {
-    const int64_t blocks = (matrices * q4_row_tiles(rows) * q4_col_tiles(cols) + kWarps - 1) / kWarps;
-    if (blocks > 0x7FFFFFFF) return fail(T81B200_ELIMIT, "dequantize_q4: matrix too large");
     const bool vec = reinterpret_cast<uintptr_t>(out) % 16 == 0 && cols * sizeof(T) % 16 == 0;
+    const int64_t blocks = (matrices * q4_row_tiles(rows) * (vec ? q4_col_tiles(cols) : (q4_col_tiles(cols) + 3) / 4) + kWarps - 1) / kWarps;
+    if (blocks > 0x7FFFFFFF) return fail(T81B200_ELIMIT, "dequantize_q4: matrix too large");
     T81_CUDA_TRY(launch_behind(vec ? dequantize_q4_kernel<T, true> : dequantize_q4_kernel<T, false>, dim3((unsigned)blocks), kThreads, 0, st,
                                reinterpret_cast<const uint4 *>(codes), static_cast<const __nv_bfloat16 *>(scales), matrices, rows, cols, group, static_cast<T *>(out)));
     return T81B200_OK;
