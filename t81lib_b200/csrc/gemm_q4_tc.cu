@@ -43,7 +43,7 @@ constexpr int RAW_CODES = 8 * 1024;                                          // 
 constexpr int A_STAGES = 3, RAW_MAX = 8, B_MAX = 12, MAX_SPLITS = 4;
 constexpr int NUM_THREADS = 23 * 32, EPILOGUE_WARP0 = 2, CONVERTER_WARP0 = 6, CONVERTERS = 8, RAW_WARP = 22;
 constexpr int FINISHERS = (RAW_WARP - EPILOGUE_WARP0) / 4;  // groups of four warps that finish a tile alone in its launch
-constexpr int BARRIER_BYTES = 512, MOST_EXPERTS = 1024;
+constexpr int BARRIER_BYTES = 512;
 constexpr int SMEM_LIMIT = 227 * 1024;
 
 enum { STATUS_PRODUCER = 1, STATUS_MMA = 2, STATUS_EPILOGUE = 3, STATUS_CONVERTER = 4 };
@@ -73,58 +73,21 @@ struct Tile {
 
 template <bool EXPERTS> struct TileList;
 template <> struct TileList<false> {
-    __device__ __forceinline__ int build(const Q4TcParams &p) { return p.m_tiles * p.n_tiles; }
+    __device__ __forceinline__ int build(const Q4TcParams &p, int32_t *) { return p.m_tiles * p.n_tiles; }
     __device__ __forceinline__ Tile tile(const Q4TcParams &p, int i, int half) const {
         const int tok = i / p.m_tiles * p.bn;
         return {0, (i % p.m_tiles * 2 + half) * BM, tok, min(tok + p.bn, p.N), p.bn};
     }
 };
 template <> struct TileList<true> {
-    int32_t *first, *before;  // [experts + 1] in shared memory: an expert's first row, tiles of experts ahead (in n)
-    // Whole CTA; the offsets are held to rising numbers within the rows whatever they say.
-    __device__ __forceinline__ int build(const Q4TcParams &p) {
-        if (threadIdx.x < 32) {
-            int sum = 0, last = 0;
-            for (int e0 = 0; e0 <= p.n_experts; e0 += 32) {
-                const int e = e0 + (int)threadIdx.x;
-                int at = e <= p.n_experts ? min(max(p.offsets[e], 0), p.N) : 0;
-#pragma unroll
-                for (int d = 1; d < 32; d <<= 1) {
-                    const int o = __shfl_up_sync(0xffffffffu, at, d);
-                    if ((int)threadIdx.x >= d) at = max(at, o);
-                }
-                at = max(at, last);
-                last = __shfl_sync(0xffffffffu, at, 31);
-                if (e <= p.n_experts) first[e] = at;
-            }
-            __syncwarp();
-            for (int e0 = 0; e0 <= p.n_experts; e0 += 32) {
-                const int e = e0 + (int)threadIdx.x, tiles = e < p.n_experts ? (first[e + 1] - first[e] + p.bn - 1) / p.bn : 0;
-                int scan = tiles;
-#pragma unroll
-                for (int d = 1; d < 32; d <<= 1) {
-                    const int o = __shfl_up_sync(0xffffffffu, scan, d);
-                    if ((int)threadIdx.x >= d) scan += o;
-                }
-                if (e <= p.n_experts) before[e] = sum + scan - tiles;
-                sum += __shfl_sync(0xffffffffu, scan, 31);
-            }
-        }
-        __syncthreads();
-        return before[p.n_experts] * p.m_tiles;
-    }
+    ExpertList list;
+    __device__ __forceinline__ int build(const Q4TcParams &p, int32_t *memory) { return list.build(memory, p.offsets, p.n_experts, p.N, p.bn) * p.m_tiles; }
     __device__ __forceinline__ Tile tile(const Q4TcParams &p, int i, int half) const {
-        const int at = i / p.m_tiles;
-        int lo = 0, hi = p.n_experts;  // the last expert with before[e] <= at that has a tile
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (before[mid] <= at) lo = mid;
-            else hi = mid;
-        }
-        const int tiles = before[lo + 1] - before[lo], rows = first[lo + 1] - first[lo];
+        const int at = i / p.m_tiles, e = list.expert_of(at, p.n_experts);
+        const int tiles = list.before[e + 1] - list.before[e], first = list.first[e], rows = list.first[e + 1] - first;
         const int width = ((rows + tiles - 1) / tiles + 31) / 32 * 32;
-        const int tok = first[lo] + (at - before[lo]) * width, end = min(tok + width, first[lo + 1]);
-        return {lo, (i % p.m_tiles * 2 + half) * BM, tok, end, max((end - tok + 31) / 32 * 32, 32)};
+        const int tok = first + (at - list.before[e]) * width, end = min(tok + width, first + rows);
+        return {e, (i % p.m_tiles * 2 + half) * BM, tok, end, max((end - tok + 31) / 32 * 32, 32)};
     }
 };
 
@@ -218,17 +181,13 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_co
     const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t *>(gen_base + (tmem_slot - base));
 
     TileList<EXPERTS> tiles;
-    if constexpr (EXPERTS) {
-        tiles.first = reinterpret_cast<int32_t *>(gen_base + (bars - base) + BARRIER_BYTES);
-        tiles.before = tiles.first + p.n_experts + 1;
-    }
-    const int total_tiles = tiles.build(p);
+    const int total_tiles = tiles.build(p, reinterpret_cast<int32_t *>(gen_base + (bars - base) + BARRIER_BYTES));
     const int n_clusters = (int)gridDim.x / (2 * p.splits), cluster_id = (int)blockIdx.x / (2 * p.splits);
     const int c0 = p.n_chunks * slice / p.splits, c1 = p.n_chunks * (slice + 1) / p.splits;
     const uint16_t pair_mask = (uint16_t)(3u << (rank & ~1u));
 
     if constexpr (EXPERTS) {  // rows of no expert: a warp each
-        const int kept = tiles.first[p.n_experts];
+        const int kept = tiles.list.first[p.n_experts];
         for (int64_t row = (int64_t)kept + blockIdx.x * (NUM_THREADS / 32) + warp; row < p.N; row += (int64_t)gridDim.x * (NUM_THREADS / 32)) {
             CT *dst = static_cast<CT *>(p.C) + row * p.ldc;
             if (p.vec && p.M % 8 == 0)
@@ -595,7 +554,7 @@ int gemm_q4_tc_launch(const uint8_t *codes, const void *scales, const float *bia
         clusters = p.one_tile ? tiles : resident;
     }
     p.out_bytes = p.one_tile ? 0 : 4 * 1024 * (int)dtype_size(c_dtype);
-    p.list_bytes = offsets ? 2 * (experts + 1) * 4 : 0;
+    p.list_bytes = offsets ? ExpertList::bytes(experts) : 0;
     // What is left after four stages of activations goes to the codes, two stages for either group of converters at least, the rest to the
     // activations again.
     const int raw = RAW_CODES + CHUNK / group * 256, stage = p.bn * BK;

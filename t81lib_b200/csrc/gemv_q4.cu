@@ -32,7 +32,7 @@ int gemm_q4_tc_launch(const uint8_t *codes, const void *scales, const float *bia
 
 namespace {
 
-constexpr int kWarps = 8, kThreads = kWarps * 32, kMostExperts = 1024, kBlocksPerSm = 2;
+constexpr int kWarps = 8, kThreads = kWarps * 32, kMostExperts = 1024, kOwners = 1024, kBlocksPerSm = 2;
 enum { STATUS_CONSUMER = 6 };
 
 __device__ int g_gemv_q4_status = 0;
@@ -82,31 +82,27 @@ __device__ __forceinline__ void fragments(const Q4Decode<T> &decode, uint32_t w,
     a[3] = decode.code(decode.template biased<3>(w));
 }
 
-// Where a warp is: a block's share `item` of the row tiles (of an expert), and a pass over TOK of its rows of x.
+// Where a warp is: a block's share of the row tiles (of an expert), and a piece of at most TOK rows of x.  Items go through the shares of one
+// piece before those of the next, and a block takes every gridDim.x-th.
 template <int TOK> struct Walk {
-    int item, expert, tile0, tok, end;
-    __device__ __forceinline__ void open(const Q4Params &p, const int16_t *active, int items, int tiles_per_item, int tile_of_item) {
-        if (item >= items) return;
-        int share = item;
-        expert = 0;
-        tok = 0;
-        end = p.rows;
-        if (p.offsets) {
-            const int at = item / p.row_items;
-            share = item - at * p.row_items;
-            expert = active[at];
-            tok = max(p.offsets[expert], 0);
-            end = min(p.offsets[expert + 1], p.rows);  // whatever the offsets say, nothing lies outside the rows
+    int share, piece, expert, tile0, tok, end;
+    // `owner`: the experts of the first kOwners pieces; items of one unit or two leave no time to look for them.
+    __device__ __forceinline__ void open(const Q4Params &p, const ExpertList &list, const int16_t *owner, int tiles_per_item, int tile_of_item, int steps) {
+        share += steps;
+        if (steps == 0 || share >= p.row_items) {
+            const int more = share / p.row_items;
+            piece += more;
+            share -= more * p.row_items;
+            tok = piece * TOK;
+            end = p.rows;
+            if (p.offsets) {
+                expert = piece < kOwners ? owner[piece] : list.expert_of(piece, p.n_experts);
+                tok = list.first[expert] + (piece - list.before[expert]) * TOK;
+                end = list.first[expert + 1];
+            }
+            end = min(end, tok + TOK);
         }
         tile0 = share * tiles_per_item + tile_of_item;
-    }
-    // True where the next pass starts other rows of the weights.
-    __device__ __forceinline__ bool next(const Q4Params &p, const int16_t *active, int items, int tiles_per_item, int tile_of_item) {
-        tok += TOK;
-        if (tok < end) return false;
-        item += (int)gridDim.x;
-        open(p, active, items, tiles_per_item, tile_of_item);
-        return true;
     }
 };
 
@@ -115,48 +111,15 @@ template <int RT, int W, int GROUP> struct Stage {
     static constexpr int kCodes = RT * W * 1024, kScales = W * (128 / GROUP) * 32, kBytes = kCodes + (RT * kScales + 127) / 128 * 128, kCount = W == 1 ? 4 : 2;
 };
 
-// acc = (FIRST) or += the fragment's product with x, columns 16 j .. of the unit.
+// acc = (FIRST) or += the fragment's product with 16 of the 32 columns of x at hand, the second ones with `second`.
 template <typename T, int PLANES, int NT, bool FIRST>
-__device__ __forceinline__ void products(float (&acc)[NT][PLANES == 1 ? 1 : 2][4], const uint32_t (&a)[4], const uint4 (&b)[PLANES][NT][4], int j) {
+__device__ __forceinline__ void products(float (&acc)[NT][PLANES == 1 ? 1 : 2][4], const uint32_t (&a)[4], const uint4 (&x)[PLANES][NT], int second) {
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-        auto b0 = [&](int pl) { return j & 1 ? b[pl][n][j >> 1].z : b[pl][n][j >> 1].x; };
-        auto b1 = [&](int pl) { return j & 1 ? b[pl][n][j >> 1].w : b[pl][n][j >> 1].y; };
-        mma_16816<T, !FIRST>(acc[n][0], a, b0(0), b1(0));
+        mma_16816<T, !FIRST>(acc[n][0], a, second ? x[0][n].z : x[0][n].x, second ? x[0][n].w : x[0][n].y);
         if constexpr (PLANES == 3) {
-            mma_16816<T, !FIRST>(acc[n][1], a, b0(1), b1(1));
-            mma_16816<T, true>(acc[n][1], a, b0(2), b1(2));
-        }
-    }
-}
-
-// 128 columns of RT row tiles: sum += scale * sums over the columns of a group, group after group.
-// (What lies past the last column meets zeros of x, rows past the last are not stored.)
-template <typename T, int PLANES, int RT, int NT, int GROUP>
-__device__ __forceinline__ void multiply(const Q4Decode<T> &decode, const uint32_t (&word)[RT][8], const uint32_t (&scale)[RT][128 / GROUP], const uint4 (&b)[PLANES][NT][4],
-                                         float (&sum)[RT][NT][PLANES == 1 ? 1 : 2][4]) {
-    constexpr int PER = 128 / GROUP, SUMS = PLANES == 1 ? 1 : 2;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        float c[RT][NT][SUMS][4];
-#pragma unroll
-        for (int j = i * (8 / PER); j < (i + 1) * (8 / PER); ++j)
-#pragma unroll
-            for (int r = 0; r < RT; ++r) {
-                uint32_t a[4];
-                fragments<T>(decode, word[r][j], a);
-                if (j == i * (8 / PER)) products<T, PLANES, NT, true>(c[r], a, b, j);
-                else products<T, PLANES, NT, false>(c[r], a, b, j);
-            }
-#pragma unroll
-        for (int r = 0; r < RT; ++r) {
-            const float lo = __uint_as_float(scale[r][i] << 16), hi = __uint_as_float(scale[r][i] & 0xFFFF0000u);
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int u = 0; u < SUMS; ++u)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) sum[r][n][u][k] = fmaf(c[r][n][u][k], k < 2 ? lo : hi, sum[r][n][u][k]);
+            mma_16816<T, !FIRST>(acc[n][1], a, second ? x[1][n].z : x[1][n].x, second ? x[1][n].w : x[1][n].y);
+            mma_16816<T, true>(acc[n][1], a, second ? x[2][n].z : x[2][n].x, second ? x[2][n].w : x[2][n].y);
         }
     }
 }
@@ -174,10 +137,11 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
 gemv_q4_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_constant__ CUtensorMap map_scales, const __grid_constant__ Q4Params p) {
     using S = Stage<RT, W, GROUP>;
     constexpr int PER = 128 / GROUP, SUMS = PLANES == 1 ? 1 : 2, TOK = 8 * NT;
+    // Rows of x are fetched a unit at a time before the wait for its codes, or 128 columns at a time, as registers hold them.
+    constexpr bool EARLY = PLANES * NT == 1;
     extern __shared__ __align__(128) uint8_t ring[];  // [warps][stages][RT units of codes, RT of scales], then part
     __shared__ __align__(8) uint64_t full[kWarps][S::kCount];
-    __shared__ int16_t active[kMostExperts];
-    __shared__ int n_active, failed;
+    __shared__ int failed;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int kw = warp % p.k_warps, row_warps = kWarps / p.k_warps, rw = warp / p.k_warps;
     constexpr int WIDTH = RT * 16 + 1, PART = kWarps * TOK * WIDTH;
@@ -190,37 +154,33 @@ gemv_q4_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_const
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     wait_for_kernel_ahead();
-    int items = p.row_items;
+    ExpertList list;
+    int16_t *const owner = reinterpret_cast<int16_t *>(reinterpret_cast<uint8_t *>(part + 2 * PART) + ExpertList::bytes(p.n_experts));
+    int items = (p.rows + TOK - 1) / TOK * p.row_items;
     if (p.offsets) {
-        if (warp == 0) {
-            int seen = 0;
-            for (int e0 = 0; e0 < p.n_experts; e0 += 32) {
-                const int e = e0 + lane;
-                const bool some = e < p.n_experts && min(p.offsets[e + 1], p.rows) > max(p.offsets[e], 0);
-                const uint32_t ballot = __ballot_sync(0xffffffffu, some);
-                if (some) active[seen + __popc(ballot & ((1u << lane) - 1u))] = (int16_t)e;
-                seen += __popc(ballot);
-            }
-            if (lane == 0) n_active = seen;
-        }
-        const int64_t kept = max(p.offsets[p.n_experts], 0);  // rows of no expert: a warp each
-        for (int64_t row = kept + blockIdx.x * kWarps + warp; row < p.rows; row += (int64_t)gridDim.x * kWarps)
-            for (int i = lane; i < p.M; i += 32) store(p.y, row * p.ldy + i, 0.0f, p.y_dtype);
+        items = list.build(reinterpret_cast<int32_t *>(part + 2 * PART), p.offsets, p.n_experts, p.rows, TOK) * p.row_items;
+        for (int e = threadIdx.x; e < p.n_experts; e += kThreads)
+            for (int q = list.before[e]; q < min(list.before[e + 1], kOwners); ++q) owner[q] = (int16_t)e;
+        for (int row = list.first[p.n_experts] + (int)blockIdx.x * kWarps + warp; row < p.rows; row += (int)gridDim.x * kWarps)  // rows of no expert: a warp each
+            for (int i = lane; i < p.M; i += 32) store(p.y, (int64_t)row * p.ldy + i, 0.0f, p.y_dtype);
     }
     __syncthreads();
-    if (p.offsets) items = n_active * p.row_items;
 
     const uint32_t my_ring = smem_u32(ring) + (uint32_t)(warp * S::kCount * S::kBytes), my_full = smem_u32(&full[warp][0]);
     const int per_item = row_warps * RT;
     Walk<TOK> fill, use;
-    fill.item = use.item = (int)blockIdx.x;
-    fill.open(p, active, items, per_item, rw * RT);
-    use.open(p, active, items, per_item, rw * RT);
+    fill.share = use.share = (int)blockIdx.x;
+    fill.piece = use.piece = fill.expert = use.expert = 0;
+    int fill_item = (int)blockIdx.x, item = fill_item;
+    if (item < items) {
+        fill.open(p, list, owner, per_item, rw * RT, 0);
+        use.open(p, list, owner, per_item, rw * RT, 0);
+    }
     // ---- copies (what lies past the matrix arrives as zeros, or is the next expert's rows) ----
     int fill_unit = kw, fill_row = fill.expert * p.row_tiles + fill.tile0;
     uint32_t slot = 0;
     auto issue = [&]() {
-        if (fill.item >= items) return;
+        if (fill_item >= items) return;
         if (elect_one()) {
             const uint32_t bar = my_full + 8u * slot, dst = my_ring + slot * S::kBytes;
             mbar_arrive_expect_tx(bar, (uint32_t)(S::kCodes + RT * S::kScales));
@@ -232,7 +192,9 @@ gemv_q4_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_const
         fill_unit += p.k_warps;
         if (fill_unit >= p.units) {
             fill_unit = kw;
-            if (fill.next(p, active, items, per_item, rw * RT)) fill_row = fill.expert * p.row_tiles + fill.tile0;
+            fill_item += (int)gridDim.x;
+            if (fill_item < items) fill.open(p, list, owner, per_item, rw * RT, (int)gridDim.x);
+            fill_row = fill.expert * p.row_tiles + fill.tile0;
         }
     };
     if (p.units > 0)
@@ -241,7 +203,7 @@ gemv_q4_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_const
     const uint32_t nothing = opaque(0u);
     Ring at;
     bool ok = true, buffer = false;
-    while (use.item < items) {
+    for (; item < items; item += (int)gridDim.x) {
         const int tile0 = use.tile0;
         float sum[RT][NT][SUMS][4] = {};
         // this lane's eight columns of a row of x for the B fragments; rows past the last are some other row's, and not stored
@@ -250,31 +212,29 @@ gemv_q4_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_const
         for (int n = 0; n < NT; ++n) src_x[n] = static_cast<const T *>(p.x) + (int64_t)min(use.tok + 8 * n + g, use.end - 1) * p.ldx + kw * (W * 128) + 8 * t;
         for (int unit = kw; unit < p.units; unit += p.k_warps) {
             const int columns = p.kx - unit * (W * 128);  // from here on
-            uint4 b[W][PLANES][NT][4];                    // [.. 32 columns]
-            auto load_x = [&](int h) {
+            const bool whole = columns >= W * 128;
+            uint4 b[EARLY ? 4 * W : 4][PLANES][NT];       // 32 columns each
+            auto load_x = [&](int i, int into) {
 #pragma unroll
                 for (int pl = 0; pl < PLANES; ++pl)
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        const T *src = src_x[n] + pl * p.plane_elems + h * 128;
-                        if (columns >= W * 128) {
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) b[h][pl][n][i] = __ldg(reinterpret_cast<const uint4 *>(src + 32 * i));
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) b[h][pl][n][i] = h * 128 + 32 * i + 8 * t < columns ? __ldg(reinterpret_cast<const uint4 *>(src + 32 * i)) : make_uint4(0u, 0u, 0u, 0u);
-                        }
+                        const T *src = src_x[n] + pl * p.plane_elems + 32 * i;
+                        if (whole) b[into][pl][n] = __ldg(reinterpret_cast<const uint4 *>(src));
+                        else b[into][pl][n] = 32 * i + 8 * t < columns ? __ldg(reinterpret_cast<const uint4 *>(src)) : make_uint4(0u, 0u, 0u, 0u);
                     }
             };
-            if (PLANES * NT == 1)  // before the wait, where registers hold it
+            if constexpr (EARLY)
 #pragma unroll
-                for (int h = 0; h < W; ++h) load_x(h);
+                for (int i = 0; i < 4 * W; ++i) load_x(i, i);
             ok = __all_sync(0xffffffffu, mbar_wait(my_full + 8u * at.stage, at.phase));
             if (!ok) break;
             const uint8_t *src = ring + (warp * S::kCount + at.stage) * S::kBytes;
 #pragma unroll
             for (int h = 0; h < W; ++h) {
-                if (PLANES * NT > 1) load_x(h);
+                if constexpr (!EARLY)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) load_x(4 * h + i, i);
                 uint32_t word[RT][8], scale[RT][PER];
 #pragma unroll
                 for (int r = 0; r < RT; ++r) {
@@ -285,7 +245,34 @@ gemv_q4_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_const
 #pragma unroll
                     for (int i = 0; i < PER; ++i) scale[r][i] = *reinterpret_cast<const uint32_t *>(src + S::kCodes + r * S::kScales + (h * PER + i) * 32 + 4 * g);
                 }
-                multiply<T, PLANES, RT, NT, GROUP>(decode, word, scale, b[h], sum);
+                // 128 columns: sum += scale * sums over the columns of a group, group after group.
+                // (What lies past the last column meets zeros of x, rows past the last are not stored.)
+                float c[RT][NT][SUMS][4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {  // 32 columns
+                    const auto &x = b[EARLY ? 4 * h + i : i];
+#pragma unroll
+                    for (int j = 2 * i; j < 2 * i + 2; ++j)
+#pragma unroll
+                        for (int r = 0; r < RT; ++r) {
+                            uint32_t a[4];
+                            fragments<T>(decode, word[r][j], a);
+                            if (j % (GROUP / 16) == 0) products<T, PLANES, NT, true>(c[r], a, x, j & 1);
+                            else products<T, PLANES, NT, false>(c[r], a, x, j & 1);
+                        }
+                    if ((i + 1) % (GROUP / 32) != 0) continue;
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) {
+                        const uint32_t s = scale[r][i / (GROUP / 32)];
+                        const float lo = __uint_as_float(s << 16), hi = __uint_as_float(s & 0xFFFF0000u);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int u = 0; u < SUMS; ++u)
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) sum[r][n][u][k] = fmaf(c[r][n][u][k], k < 2 ? lo : hi, sum[r][n][u][k]);
+                    }
+                }
             }
             // Into the stage just read, once what was read has been used: a copy does not wait for loads of shared memory still on their way.
             uint32_t used = 0;
@@ -308,10 +295,10 @@ gemv_q4_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_const
                 }
         __syncthreads();
         if (failed) break;  // whoever reads it late finds it, too, at the next barrier: it is never taken back
-        for (int i = threadIdx.x; i < TOK * row_warps * RT * 16; i += kThreads) {
+        for (int i = threadIdx.x; i < (use.end - use.tok) * row_warps * RT * 16; i += kThreads) {
             const int r = i % (RT * 16), share = i / (RT * 16) % row_warps, tok = i / (RT * 16 * row_warps);
             const int row = (tile0 - rw * RT + share * RT) * 16 + r;
-            if (use.tok + tok >= use.end || row >= p.M) continue;
+            if (row >= p.M) continue;
             float v = 0.0f;
             for (int w = 0; w < p.k_warps; ++w) v += part[((share * p.k_warps + w) * TOK + tok) * WIDTH + r];
             if (p.bias) v += p.bias[use.expert * p.bias_stride + row];
@@ -319,7 +306,7 @@ gemv_q4_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_const
         }
         part = buffer ? part - PART : part + PART;
         buffer = !buffer;
-        use.next(p, active, items, per_item, rw * RT);
+        if (item + (int)gridDim.x < items) use.open(p, list, owner, per_item, rw * RT, (int)gridDim.x);
     }
     if (failed) give_up(&g_gemv_q4_status, STATUS_CONSUMER);
 }
@@ -329,8 +316,11 @@ int launch(Q4Params &p, cudaStream_t st) {
     using S = Stage<RT, W, GROUP>;
     const int row_warps = kWarps / p.k_warps;
     p.row_items = (p.row_tiles + RT * row_warps - 1) / (RT * row_warps);
-    const int64_t items = (int64_t)p.row_items * (p.offsets ? (p.rows < p.n_experts ? p.rows : p.n_experts) : 1), most = (int64_t)sm_count() * kBlocksPerSm;
-    constexpr size_t smem = (size_t)kWarps * (S::kCount * S::kBytes + 2 * 8 * NT * (RT * 16 + 1) * sizeof(float));
+    const int64_t pieces = p.offsets ? (p.rows + 8 * NT - 1) / (8 * NT) + (p.rows < p.n_experts ? p.rows : p.n_experts) : (p.rows + 8 * NT - 1) / (8 * NT);
+    const int64_t items = (int64_t)p.row_items * pieces, most = (int64_t)sm_count() * kBlocksPerSm;
+    if (items >= 1ll << 31) return fail(T81B200_ELIMIT, "linear_q4: too many rows for a matrix of this size");
+    constexpr size_t fixed = (size_t)kWarps * (S::kCount * S::kBytes + 2 * 8 * NT * (RT * 16 + 1) * sizeof(float)), limit = fixed + ExpertList::bytes(kMostExperts) + kOwners * 2;
+    const size_t smem = fixed + (p.offsets ? ExpertList::bytes(p.n_experts) + kOwners * 2 : 0);
     CUtensorMap mc, ms;
     memset(&mc, 0, sizeof mc);
     memset(&ms, 0, sizeof ms);
@@ -346,7 +336,7 @@ int launch(Q4Params &p, cudaStream_t st) {
     int dev = 0;
     T81_CUDA_TRY(cudaGetDevice(&dev));
     if (dev < 0 || dev >= 64 || !configured[dev].load(std::memory_order_acquire)) {
-        T81_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        T81_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)limit));
         if (dev >= 0 && dev < 64) configured[dev].store(true, std::memory_order_release);
     }
     T81_CUDA_TRY(launch_behind(kernel, dim3((unsigned)(items < most ? items : most)), dim3(kThreads), smem, st, mc, ms, p));
@@ -372,11 +362,16 @@ int launch_width(Q4Params &p, int group, cudaStream_t st) {
 // p.units: of 128 columns.
 template <typename T, int PLANES>
 int launch_shape(Q4Params &p, int group, cudaStream_t st) {
-    // two row tiles a warp read each piece of an activation row once for both, where that leaves every block a share
-    const bool wide = (int64_t)p.row_tiles * (p.offsets ? (p.rows < p.n_experts ? p.rows : p.n_experts) : 1) >= 4 * (int64_t)sm_count();
+    // Sixteen rows of x at a time beyond eight: 16 tokens of 4096 x 14336, bf16, 16.3 us, in two passes of eight 21.4.  Not for experts, most of
+    // which have a few rows (64 of 2816 x 2048, 8 tokens in 6 each: 28 and 36 us), and not in three planes, which the registers do not hold.
+    const bool two = PLANES == 1 && p.rows > 8 && !p.offsets;
+    const int64_t pieces = p.offsets ? (p.rows < p.n_experts ? p.rows : p.n_experts) : (two ? (p.rows + 15) / 16 : (p.rows + 7) / 8);
+    // Two row tiles a warp read each piece of an activation row once for both, where that leaves every block its shares (us, one and two: 65536 x
+    // 4096, 8 tokens 47.7 and 39.7, 4096 x 14336 11.4 and 12.0, 1024 x 4096 3.3 and 4.1).
+    const bool wide = p.row_tiles * pieces >= 4 * (int64_t)sm_count();
     if constexpr (PLANES == 1)
-        if (p.rows > 8 && !p.offsets) return wide ? launch_width<T, PLANES, 2, 2>(p, group, st) : launch_width<T, PLANES, 1, 2>(p, group, st);
-    return wide ? launch_width<T, PLANES, 2, 1>(p, group, st) : launch_width<T, PLANES, 1, 1>(p, group, st);  // three planes of 16 rows do not fit the registers
+        if (two) return wide ? launch_width<T, PLANES, 2, 2>(p, group, st) : launch_width<T, PLANES, 1, 2>(p, group, st);
+    return wide ? launch_width<T, PLANES, 2, 1>(p, group, st) : launch_width<T, PLANES, 1, 1>(p, group, st);
 }
 
 // Rows that the kernels read where they are: 16-bit, on 16-byte boundaries, whole pieces of eight columns.

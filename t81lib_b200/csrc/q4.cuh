@@ -70,4 +70,50 @@ template <> struct Q4Decode<__half> {
     }
 };
 
+// Rows sorted by expert as a list of pieces of at most `width` rows: in shared memory, made by every block from the experts' first rows.
+struct ExpertList {
+    int32_t *first, *before;  // [experts + 1] each: an expert's first row, the pieces of experts ahead of it
+
+    static __host__ __device__ constexpr int bytes(int n_experts) { return 2 * (n_experts + 1) * 4; }
+
+    // Whole block; returns the number of pieces.  Whatever the offsets say, no row outside 0 .. rows - 1 is named.
+    __device__ __forceinline__ int build(int32_t *memory, const int32_t *offsets, int n_experts, int rows, int width) {
+        first = memory;
+        before = memory + n_experts + 1;
+        const int lane = (int)threadIdx.x;
+        if (lane < 32) {
+            int sum = 0;
+            for (int e0 = 0; e0 <= n_experts; e0 += 32) {
+                const int e = e0 + lane;
+                const int at = e <= n_experts ? min(max(offsets[e], 0), rows) : 0, end = e < n_experts ? min(max(offsets[e + 1], 0), rows) : 0;
+                const int pieces = e < n_experts && end > at ? (end - at + width - 1) / width : 0;
+                int scan = pieces;
+#pragma unroll
+                for (int d = 1; d < 32; d <<= 1) {
+                    const int o = __shfl_up_sync(0xffffffffu, scan, d);
+                    if (lane >= d) scan += o;
+                }
+                if (e <= n_experts) {
+                    first[e] = at;
+                    before[e] = sum + scan - pieces;
+                }
+                sum += __shfl_sync(0xffffffffu, scan, 31);
+            }
+        }
+        __syncthreads();
+        return before[n_experts];
+    }
+
+    // The expert that piece `at` belongs to.
+    __device__ __forceinline__ int expert_of(int at, int n_experts) const {
+        int lo = 0, hi = n_experts;  // the last one with before[e] <= at has a piece
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (before[mid] <= at) lo = mid;
+            else hi = mid;
+        }
+        return lo;
+    }
+};
+
 }  // namespace t81b200

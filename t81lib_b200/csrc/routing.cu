@@ -18,13 +18,26 @@
 
 #include <cooperative_groups.h>
 
+#include <atomic>
+
 namespace t81b200 {
 
 namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32, kMostExperts = 1024, kSortCluster = 8;
+constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32, kMostExperts = 1024, kSortCluster = 16, kSortKept = 4;
+
+// The lanes with this lane's value, of `bits` bits: a vote per bit (match_any takes its turn on one unit of the SM: 131072 ids 42 us).
+__device__ __forceinline__ uint32_t equal_lanes(int v, int bits) {
+    uint32_t equal = 0xffffffffu;
+    for (int b = 0; b < bits; ++b) {
+        const bool one = ((v >> b) & 1) != 0;
+        const uint32_t ones = __ballot_sync(0xffffffffu, one);
+        equal &= one ? ones : ~ones;
+    }
+    return equal;
+}
 
 template <typename ID>
 __global__ void __launch_bounds__(kSortThreads, 1) sort_by_expert_kernel(const ID *__restrict__ ids, int n, int n_experts, int run, int32_t *__restrict__ order,
@@ -35,8 +48,10 @@ __global__ void __launch_bounds__(kSortThreads, 1) sort_by_expert_kernel(const I
     wait_for_kernel_ahead();
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks(), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    int32_t *mine = counts + warp * n_experts, *cta_total = counts + kSortWarps * n_experts;
-    for (int i = threadIdx.x; i < kSortWarps * n_experts; i += kSortThreads) counts[i] = 0;
+    const int bits = 32 - __clz(n_experts);  // ids and n_experts itself
+    const int pitch = n_experts | 1;  // odd: the warps' counts of an expert lie in different banks
+    int32_t *mine = counts + warp * pitch, *cta_total = counts + kSortWarps * pitch;
+    for (int i = threadIdx.x; i < kSortWarps * pitch; i += kSortThreads) counts[i] = 0;
     __syncthreads();
     const int64_t lo64 = (int64_t)(rank * kSortWarps + warp) * run;
     const int lo = lo64 < n ? (int)lo64 : n, hi = n - lo < run ? n : lo + run;
@@ -45,31 +60,47 @@ __global__ void __launch_bounds__(kSortThreads, 1) sort_by_expert_kernel(const I
         const ID id = ids[i];
         return id >= 0 && id < (ID)n_experts ? (int)id : n_experts;
     };
-    for (int i0 = lo; i0 < hi; i0 += 32) {
-        const int e = expert_of(i0 + lane);
-        const uint32_t equal = __match_any_sync(0xffffffffu, e);
+    // the ids of a warp's first steps stay in registers for the second pass
+    int kept_ids[kSortKept];
+#pragma unroll
+    for (int k = 0; k < kSortKept; ++k) kept_ids[k] = expert_of(lo + 32 * k + lane);
+    auto steps = [&](auto &&body) {
+#pragma unroll
+        for (int k = 0; k < kSortKept; ++k)
+            if (lo + 32 * k < hi) body(lo + 32 * k, kept_ids[k]);
+        for (int i0 = lo + 32 * kSortKept; i0 < hi; i0 += 32) body(i0, expert_of(i0 + lane));
+    };
+    steps([&](int, int e) {
+        const uint32_t equal = equal_lanes(e, bits);
         if (e < n_experts && lane == __ffs(equal) - 1) mine[e] += __popc(equal);
         __syncwarp();
-    }
+    });
     __syncthreads();
-    const int e = threadIdx.x;
-    int32_t total = 0;
-    if (e < n_experts) {
-        for (int w = 0; w < kSortWarps; ++w) {
-            const int32_t c = counts[w * n_experts + e];
-            counts[w * n_experts + e] = total;
-            total += c;
+    // counts to the number in warps ahead: a warp per expert, a lane per warp
+    for (int x = warp; x < n_experts; x += kSortWarps) {
+        const int32_t c = counts[lane * pitch + x];
+        int32_t sum = c;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int32_t o = __shfl_up_sync(0xffffffffu, sum, d);
+            if (lane >= d) sum += o;
         }
-        cta_total[e] = total;
+        counts[lane * pitch + x] = sum - c;
+        if (lane == 31) cta_total[x] = sum;
     }
     cluster.sync();
+    const int e = threadIdx.x;
     int32_t before = 0, all = 0;  // of this expert: in CTAs ahead, in all
-    if (e < n_experts)
-        for (int r = 0; r < ctas; ++r) {
-            const int32_t c = cluster.map_shared_rank(cta_total, r)[e];
-            before += r < rank ? c : 0;
-            all += c;
+    if (e < n_experts) {
+        int32_t of[kSortCluster];
+#pragma unroll
+        for (int r = 0; r < kSortCluster; ++r) of[r] = r < ctas ? cluster.map_shared_rank(cta_total, r)[e] : 0;
+#pragma unroll
+        for (int r = 0; r < kSortCluster; ++r) {
+            before += r < rank ? of[r] : 0;
+            all += of[r];
         }
+    }
     cluster.sync();  // nobody reads another CTA's counts from here on
     int32_t scan = all;
 #pragma unroll
@@ -91,9 +122,9 @@ __global__ void __launch_bounds__(kSortThreads, 1) sort_by_expert_kernel(const I
         if (rank == 0) offsets[n_experts] = kept;
     }
     __syncthreads();
-    for (int i0 = lo; i0 < hi; i0 += 32) {
-        const int i = i0 + lane, id = expert_of(i);
-        const uint32_t equal = __match_any_sync(0xffffffffu, id);
+    steps([&](int i0, int id) {
+        const int i = i0 + lane;
+        const uint32_t equal = equal_lanes(id, bits);
         if (id < n_experts) {
             const int32_t at = cta_total[id] + mine[id] + __popc(equal & ((1u << lane) - 1u));
             order[at] = i;
@@ -102,7 +133,7 @@ __global__ void __launch_bounds__(kSortThreads, 1) sort_by_expert_kernel(const I
         __syncwarp();
         if (id < n_experts && lane == __ffs(equal) - 1) mine[id] += __popc(equal);
         __syncwarp();
-    }
+    });
     for (int64_t p = (int64_t)kept + rank * kSortThreads + threadIdx.x; p < n; p += ctas * kSortThreads) order[p] = -1;
 }
 
@@ -138,13 +169,22 @@ __global__ void __launch_bounds__(kThreads) combine_rows_kernel(const T *__restr
     if (chunk >= pieces) return;
     for (int64_t t = blockIdx.x; t < tokens; t += gridDim.x) {
         float sum[N] = {};
-        for (int j = 0; j < top; ++j) {
-            const int64_t p = position[t * top + j];
-            if (p < 0 || p >= n) continue;
-            const float w = weights ? to_float<W>(weights[t * top + j]) : 1.0f;
-            const Piece<T, N> v = reinterpret_cast<const Piece<T, N> *>(rows + p * ld)[chunk];
+        for (int j0 = 0; j0 < top; j0 += 4) {  // four rows on their way at a time
+            Piece<T, N> v[4];
+            float w[4];
+            bool there[4];
 #pragma unroll
-            for (int i = 0; i < N; ++i) sum[i] = fmaf(w, to_float<T>(v.v[i]), sum[i]);
+            for (int k = 0; k < 4; ++k) {
+                const int64_t p = j0 + k < top ? position[t * top + j0 + k] : -1;
+                there[k] = p >= 0 && p < n;
+                v[k] = reinterpret_cast<const Piece<T, N> *>(rows + (there[k] ? p : 0) * ld)[chunk];  // (a slot without a row reads one all the same: no branch between loads)
+                w[k] = weights && there[k] ? to_float<W>(weights[t * top + j0 + k]) : 1.0f;
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (there[k])
+#pragma unroll
+                    for (int i = 0; i < N; ++i) sum[i] = fmaf(w[k], to_float<T>(v[k].v[i]), sum[i]);
         }
         Piece<T, N> out;
 #pragma unroll
@@ -201,24 +241,46 @@ __global__ void __launch_bounds__(kThreads) combine_rows_grad_kernel(const T *__
 
 template <typename ID>
 int launch_sort(const void *ids, int64_t n, int n_experts, int32_t *order, int32_t *position, int32_t *offsets, cudaStream_t st) {
-    const int ctas = n > kSortThreads ? kSortCluster : 1;
-    const int64_t run = ((n + (int64_t)ctas * kSortWarps - 1) / ((int64_t)ctas * kSortWarps) + 31) / 32 * 32;
-    const size_t smem = (size_t)(kSortWarps + 1) * n_experts * sizeof(int32_t);
+    const size_t smem = ((size_t)kSortWarps * (n_experts | 1) + n_experts) * sizeof(int32_t);
     auto kernel = sort_by_expert_kernel<ID>;
-    if (smem > 40 * 1024) T81_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    T81_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)((kSortWarps + 1) * (kMostExperts + 1) * sizeof(int32_t))));
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)ctas);
     cfg.blockDim = dim3(kSortThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = (unsigned)ctas;
-    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
+    auto shape = [&](int ctas) {
+        cfg.gridDim = dim3((unsigned)ctas);
+        attr[0].val.clusterDim.x = (unsigned)ctas;
+    };
+    // Sixteen CTAs where the device runs that many as a cluster (131072 ids 19 us, 30 with eight), eight for up to 8192 ids, one for up to 1024.
+    int ctas = n > 8192 ? kSortCluster : (n > kSortThreads ? 8 : 1);
+    if (ctas == kSortCluster) {
+        static std::atomic<int> fits[64];  // 1: a cluster of sixteen fits, 2: it does not
+        int dev = 0, known = 0;
+        T81_CUDA_TRY(cudaGetDevice(&dev));
+        if (dev >= 0 && dev < 64) known = fits[dev].load(std::memory_order_relaxed);
+        if (known == 0) {
+            int clusters = 0;
+            shape(ctas);
+            cfg.numAttrs = 1;
+            cfg.dynamicSmemBytes = (kSortWarps + 1) * (kMostExperts + 1) * sizeof(int32_t);
+            known = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
+                            cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) == cudaSuccess && clusters > 0 ? 1 : 2;
+            (void)cudaGetLastError();
+            cfg.dynamicSmemBytes = smem;
+            if (dev >= 0 && dev < 64) fits[dev].store(known, std::memory_order_relaxed);
+        }
+        if (known == 2) ctas = 8;
+    }
+    shape(ctas);
     cfg.numAttrs = 2;
+    const int64_t run = ((n + (int64_t)ctas * kSortWarps - 1) / ((int64_t)ctas * kSortWarps) + 31) / 32 * 32;
     T81_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, static_cast<const ID *>(ids), (int)n, n_experts, (int)run, order, position, offsets));
     return T81B200_OK;
 }
