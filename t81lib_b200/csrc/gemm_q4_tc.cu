@@ -30,6 +30,7 @@
 #include "umma.cuh"
 
 #include <atomic>
+#include <cmath>
 #include <cstring>
 #include <type_traits>
 
@@ -60,10 +61,16 @@ struct Q4TcParams {
     int n_experts, row_tiles;   // 16-row tiles of an expert
     int groups;
     int m_tiles, n_tiles;       // 256-row pair tiles; tiles of bn rows of x (one matrix)
-    int bn, box_rows;           // most rows of x a tile, a multiple of 32; rows of a TMA box
+    int bn;                     // most rows of x a tile, a multiple of 32
     int n_atoms, n_chunks;
     int splits, raw_stages, b_stages, one_tile, out_bytes, list_bytes;
     int vec;                    // 16-byte stores are possible
+};
+
+// Tensor maps of x.  One matrix: [0] with boxes of half a tile.  Experts, whose tiles differ: boxes of 128, 64, 32 and 16 rows, the binary digits of
+// half a tile (in boxes of 16 alone 37 experts of 2048 x 4096 with 256 rows each took 119 us, 109 so).
+struct XMaps {
+    CUtensorMap m[4];
 };
 
 // What a tile is: its expert, first output feature, rows [tok, end) and their number rounded up to 32.
@@ -84,9 +91,9 @@ template <> struct TileList<true> {
     __device__ __forceinline__ int build(const Q4TcParams &p, int32_t *memory) { return list.build(memory, p.offsets, p.n_experts, p.N, p.bn) * p.m_tiles; }
     __device__ __forceinline__ Tile tile(const Q4TcParams &p, int i, int half) const {
         const int at = i / p.m_tiles, e = list.expert_of(at, p.n_experts);
-        const int tiles = list.before[e + 1] - list.before[e], first = list.first[e], rows = list.first[e + 1] - first;
-        const int width = ((rows + tiles - 1) / tiles + 31) / 32 * 32;
-        const int tok = first + (at - list.before[e]) * width, end = min(tok + width, first + rows);
+        const int2 here = list.at[e], then = list.at[e + 1];  // first row, tiles ahead
+        const int tiles = then.y - here.y, width = ((then.x - here.x + tiles - 1) / tiles + 31) / 32 * 32;
+        const int tok = here.x + (at - here.y) * width, end = min(tok + width, then.x);
         return {e, (i % p.m_tiles * 2 + half) * BM, tok, end, max((end - tok + 31) / 32 * 32, 32)};
     }
 };
@@ -135,7 +142,7 @@ __device__ __forceinline__ uint32_t row_exponent(const __nv_bfloat16 *scales, in
 
 template <typename T, int GROUP, typename CT, bool EXPERTS>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
-gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_constant__ CUtensorMap map_scales, const __grid_constant__ CUtensorMap map_x,
+gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_constant__ CUtensorMap map_scales, const __grid_constant__ XMaps map_x,
                   const __grid_constant__ Q4TcParams p) {
     constexpr bool F16 = std::is_same<T, __half>::value;
     constexpr int PER = CHUNK / GROUP;
@@ -167,7 +174,7 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_co
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         prefetch_map(&map_codes);
         prefetch_map(&map_scales);
-        prefetch_map(&map_x);
+        prefetch_map(&map_x.m[0]);
     }
     __syncthreads();
     if (warp == 1) tmem_alloc_pair(tmem_slot);
@@ -187,7 +194,7 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_co
     const uint16_t pair_mask = (uint16_t)(3u << (rank & ~1u));
 
     if constexpr (EXPERTS) {  // rows of no expert: a warp each
-        const int kept = tiles.list.first[p.n_experts];
+        const int kept = tiles.list.first(p.n_experts);
         for (int64_t row = (int64_t)kept + blockIdx.x * (NUM_THREADS / 32) + warp; row < p.N; row += (int64_t)gridDim.x * (NUM_THREADS / 32)) {
             CT *dst = static_cast<CT *>(p.C) + row * p.ldc;
             if (p.vec && p.M % 8 == 0)
@@ -211,17 +218,24 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_co
         int chunks = 0;
         for (int i = cluster_id; i < total_tiles && ok; i += n_clusters) {
             const Tile t = tiles.tile(p, i, half);
-            const int boxes = (t.n / 2 + p.box_rows - 1) / p.box_rows, row = t.tok + half * (t.n / 2);
-            const uint32_t box_bytes = (uint32_t)p.box_rows * (BK * 2);
+            const int rows = t.n / 2, row = t.tok + half * rows;
             for (int c = c0; c < c1 && ok; ++c, ++chunks) {
                 const int a1 = min(2 * c + 2, p.n_atoms);
                 for (int a = 2 * c; a < a1; ++a) {
                     ok = mbar_wait(b_empty(b.stage), b.phase ^ 1);
                     if (!ok) break;
                     if (elect_one()) {
-                        if (half == 0) mbar_arrive_expect_tx(b_full(b.stage), 2u * (uint32_t)boxes * box_bytes);
+                        if (half == 0) mbar_arrive_expect_tx(b_full(b.stage), 2u * (uint32_t)rows * (BK * 2));
                         const uint32_t dst = base + b_off + (uint32_t)b.stage * b_stage_bytes;
-                        for (int k = 0; k < boxes; ++k) tma_load_2d_pair(dst + (uint32_t)k * box_bytes, &map_x, a * BK, row + k * p.box_rows, b_full(b.stage));
+                        if constexpr (EXPERTS) {
+                            int done = 0;
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                if (rows & (128 >> k)) {
+                                    tma_load_2d_pair(dst + (uint32_t)done * (BK * 2), &map_x.m[k], a * BK, row + done, b_full(b.stage));
+                                    done += 128 >> k;
+                                }
+                        } else tma_load_2d_pair(dst, &map_x.m[0], a * BK, row, b_full(b.stage));
                     }
                     __syncwarp();
                     b.advance(p.b_stages);
@@ -337,88 +351,93 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_co
         Ring a, raw;
         if (group == 1) { a.advance(A_STAGES); raw.advance(p.raw_stages); }
         bool ok = true;
+        float shrink[2] = {1.0f, 1.0f};
+        // the chunks of this CTA's tiles; `c`: of the tile's, where its rows' powers of two matter
         const int span = c1 - c0;
-        int c = group;  // of the tile's span
-        for (int i = cluster_id; i < total_tiles && ok; i += n_clusters, c -= span) {
-            float shrink[2] = {1.0f, 1.0f};
+        int c = group, i = cluster_id;
+        bool fresh = true;
+        for (int left = (cluster_id < total_tiles ? (total_tiles - 1 - cluster_id) / n_clusters + 1 : 0) * span - group; left > 0; left -= 2) {
             if constexpr (F16) {
-                const Tile t = tiles.tile(p, i, half);
-                const int64_t tile = (int64_t)t.expert * p.row_tiles + (t.row0 >> 4) + cw;
+                for (; c >= span; c -= span, i += n_clusters) fresh = true;
+                if (fresh) {
+                    const Tile t = tiles.tile(p, i, half);
+                    const int64_t tile = (int64_t)t.expert * p.row_tiles + (t.row0 >> 4) + cw;
 #pragma unroll
-                for (int r = 0; r < 2; ++r)
-                    if (t.row0 + cw * 16 < p.M) shrink[r] = __uint_as_float(0x7F000000u - row_exponent(p.scales, tile, p.groups, g + 8 * r));  // 2^-e
+                    for (int r = 0; r < 2; ++r)
+                        shrink[r] = t.row0 + cw * 16 < p.M ? __uint_as_float(0x7F000000u - row_exponent(p.scales, tile, p.groups, g + 8 * r)) : 1.0f;  // 2^-e
+                    fresh = false;
+                }
+                c += 2;
             }
-            for (; c < span; c += 2) {
-                ok = __all_sync(0xffffffffu, mbar_wait(raw_full(raw.stage), raw.phase));
-                if (!ok) break;
-                const uint8_t *src = gen_base + raw_off + raw.stage * RAW_BYTES;
-                uint4 q[2];
-                uint32_t s[PER];
+            ok = __all_sync(0xffffffffu, mbar_wait(raw_full(raw.stage), raw.phase));
+            if (!ok) break;
+            const uint8_t *src = gen_base + raw_off + raw.stage * RAW_BYTES;
+            uint4 q[2];
+            uint32_t s[PER];
 #pragma unroll
-                for (int k = 0; k < 2; ++k) q[k] = *reinterpret_cast<const uint4 *>(src + cw * 1024 + k * 512 + lane * 16);
+            for (int k = 0; k < 2; ++k) q[k] = *reinterpret_cast<const uint4 *>(src + cw * 1024 + k * 512 + lane * 16);
 #pragma unroll
-                for (int u = 0; u < PER; ++u) s[u] = *reinterpret_cast<const uint32_t *>(src + RAW_CODES + (cw * PER + u) * 32 + g * 4);
-                // a row's scale twice in a word, and -24 times it
-                uint32_t s2[2][PER], n2[2][PER];
+            for (int u = 0; u < PER; ++u) s[u] = *reinterpret_cast<const uint32_t *>(src + RAW_CODES + (cw * PER + u) * 32 + g * 4);
+            // a row's scale twice in a word, and -24 times it
+            uint32_t s2[2][PER], n2[2][PER];
 #pragma unroll
-                for (int u = 0; u < PER; ++u)
+            for (int u = 0; u < PER; ++u)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    if constexpr (F16) {
+                        const __half h = __float2half_rn(__uint_as_float(r ? s[u] & 0xFFFF0000u : s[u] << 16) * shrink[r]);
+                        const __half2 hh(h, h), nn = __hmul2(hh, __half2(__float2half_rn(-24.0f), __float2half_rn(-24.0f)));
+                        s2[r][u] = *reinterpret_cast<const uint32_t *>(&hh);
+                        n2[r][u] = *reinterpret_cast<const uint32_t *>(&nn);
+                    } else {
+                        s2[r][u] = __byte_perm(s[u], s[u], r ? 0x3232 : 0x1010);
+                        n2[r][u] = fma_bf16x2(s2[r][u], 0xC1C0C1C0u, 0x80008000u);
+                    }
+                }
+            ok = __all_sync(0xffffffffu, mbar_wait(a_empty(a.stage), a.phase ^ 1));
+            if (!ok) break;
+            uint8_t *dst = gen_base + a.stage * A_CHUNK_BYTES;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const uint32_t w[4] = {swap ? q[k].z : q[k].x, swap ? q[k].w : q[k].y, swap ? q[k].x : q[k].z, swap ? q[k].y : q[k].w};
+#pragma unroll
+                for (int h = 0; h < 2; ++h)  // the lane's first and second half to be stored
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
-                        if constexpr (F16) {
-                            const __half h = __float2half_rn(__uint_as_float(r ? s[u] & 0xFFFF0000u : s[u] << 16) * shrink[r]);
-                            const __half2 hh(h, h), nn = __hmul2(hh, __half2(__float2half_rn(-24.0f), __float2half_rn(-24.0f)));
-                            s2[r][u] = *reinterpret_cast<const uint32_t *>(&hh);
-                            n2[r][u] = *reinterpret_cast<const uint32_t *>(&nn);
+                        uint32_t sc, nc;
+                        if constexpr (GROUP == 32) {
+                            sc = swap ? s2[r][2 * k + 1 - h] : s2[r][2 * k + h];
+                            nc = swap ? n2[r][2 * k + 1 - h] : n2[r][2 * k + h];
                         } else {
-                            s2[r][u] = __byte_perm(s[u], s[u], r ? 0x3232 : 0x1010);
-                            n2[r][u] = fma_bf16x2(s2[r][u], 0xC1C0C1C0u, 0x80008000u);
+                            sc = s2[r][GROUP == 64 ? k : 0];
+                            nc = n2[r][GROUP == 64 ? k : 0];
                         }
-                    }
-                ok = __all_sync(0xffffffffu, mbar_wait(a_empty(a.stage), a.phase ^ 1));
-                if (!ok) break;
-                uint8_t *dst = gen_base + a.stage * A_CHUNK_BYTES;
+                        uint32_t o[4];
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const uint32_t w[4] = {swap ? q[k].z : q[k].x, swap ? q[k].w : q[k].y, swap ? q[k].x : q[k].z, swap ? q[k].y : q[k].w};
+                        for (int j = 0; j < 2; ++j)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)  // the lane's first and second half to be stored
-#pragma unroll
-                        for (int r = 0; r < 2; ++r) {
-                            uint32_t sc, nc;
-                            if constexpr (GROUP == 32) {
-                                sc = swap ? s2[r][2 * k + 1 - h] : s2[r][2 * k + h];
-                                nc = swap ? n2[r][2 * k + 1 - h] : n2[r][2 * k + h];
-                            } else {
-                                sc = s2[r][GROUP == 64 ? k : 0];
-                                nc = n2[r][GROUP == 64 ? k : 0];
+                            for (int pr = 0; pr < 2; ++pr) {
+                                const uint32_t x = w[2 * h + j];
+                                const uint32_t v = r == 0 ? (pr == 0 ? decode.template biased<0>(x) : decode.template biased<2>(x))
+                                                          : (pr == 0 ? decode.template biased<1>(x) : decode.template biased<3>(x));
+                                o[2 * j + pr] = Q4Decode<T>::scaled(v, sc, nc);
                             }
-                            uint32_t o[4];
-#pragma unroll
-                            for (int j = 0; j < 2; ++j)
-#pragma unroll
-                                for (int pr = 0; pr < 2; ++pr) {
-                                    const uint32_t x = w[2 * h + j];
-                                    const uint32_t v = r == 0 ? (pr == 0 ? decode.template biased<0>(x) : decode.template biased<2>(x))
-                                                              : (pr == 0 ? decode.template biased<1>(x) : decode.template biased<3>(x));
-                                    o[2 * j + pr] = Q4Decode<T>::scaled(v, sc, nc);
-                                }
-                            *reinterpret_cast<uint4 *>(dst + k * A_ATOM_BYTES + off[h] + r * 1024) = make_uint4(o[0], o[1], o[2], o[3]);
-                        }
-                }
-                // generic-proxy writes must be visible to the tensor core's async proxy
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                // The codes are handed back only now that they have been used: an arrival overtakes loads of shared memory that are still on their way
-                // (16 warps' stores ahead of them), and the next copy overwrote what they were to read.
-                if (lane == 0) {
-                    mbar_arrive_leader(a_full(a.stage));
-                    mbar_arrive(raw_empty(raw.stage));
-                }
-                raw.advance(p.raw_stages);
-                raw.advance(p.raw_stages);
-                a.advance(A_STAGES);
-                a.advance(A_STAGES);
+                        *reinterpret_cast<uint4 *>(dst + k * A_ATOM_BYTES + off[h] + r * 1024) = make_uint4(o[0], o[1], o[2], o[3]);
+                    }
             }
+            // generic-proxy writes must be visible to the tensor core's async proxy
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            // The codes are handed back only now that they have been used: an arrival overtakes loads of shared memory that are still on their way
+            // (16 warps' stores ahead of them), and the next copy overwrote what they were to read.
+            if (lane == 0) {
+                mbar_arrive_leader(a_full(a.stage));
+                mbar_arrive(raw_empty(raw.stage));
+            }
+            raw.advance(p.raw_stages);
+            raw.advance(p.raw_stages);
+            a.advance(A_STAGES);
+            a.advance(A_STAGES);
         }
         if (!ok) give_up(&g_q4_status, STATUS_CONVERTER);
     }
@@ -468,14 +487,36 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_co
     }
 }
 
-// Time of a 64-deep step at n columns, in units of 1.7 ns (gemm_trit_tc.cu's figures).
+// Time of a 64-deep step at n columns, in ns: 18944 rows of 8192 columns, one tile a pair, 34 to 256 rows of x, without 5.5 us.
 double step_cost(int n) {
-    constexpr double cost[8] = {115, 119, 122, 125, 130, 153, 169, 187};  // 32, 64, .. 256 columns
-    return cost[n / 32 - 1];
+    constexpr double cost[9] = {235, 235, 236, 252, 259, 279, 297, 349, 375};  // 0, 32, .. 256 columns
+    const int at = n / 32;
+    return n % 32 == 0 ? cost[at] : cost[at] + (cost[at + 1] - cost[at]) * (n % 32) / 32;
+}
+
+// Tile width and split of one matrix: the smallest estimate, in ns without the launch.
+struct Shape {
+    int bn = 0, n_tiles = 0, splits = 1;
+    double ns = 1e30;
+};
+Shape pick_shape(int64_t M, int64_t N, int64_t K) {
+    const int64_t m_tiles = (M + 255) / 256, chunks = (K + CHUNK - 1) / CHUNK, least = (N + 255) / 256;
+    Shape best;
+    for (int64_t want = least; want <= least + 8 && want <= (N + 31) / 32; ++want) {
+        const int bn = (int)(((N + want - 1) / want + 31) / 32 * 32);
+        const int64_t n_tiles = (N + bn - 1) / bn, tiles = m_tiles * n_tiles;
+        for (int s = 1; s <= MAX_SPLITS; ++s) {
+            const int fit = resident_pair_clusters(s);
+            if (s > chunks || (s > 1 && tiles > fit)) continue;
+            const double ns = (double)((tiles + fit - 1) / fit) * (2.0 * (double)((chunks + s - 1) / s) * step_cost(bn) + 700.0) + 5.0 * bn + (s > 1 ? 2200.0 + 5.0 * bn : 0.0);
+            if (ns < best.ns) best = {bn, (int)n_tiles, s, ns};
+        }
+    }
+    return best;
 }
 
 template <typename T, int GROUP, typename CT, bool EXPERTS>
-int launch(const CUtensorMap &mc, const CUtensorMap &ms, const CUtensorMap &mx, const Q4TcParams &p, int clusters, size_t smem, cudaStream_t st) {
+int launch(const CUtensorMap &mc, const CUtensorMap &ms, const XMaps &mx, const Q4TcParams &p, int clusters, size_t smem, cudaStream_t st) {
     auto kern = gemm_q4_tc_kernel<T, GROUP, CT, EXPERTS>;
     constexpr int most = SMEM_LIMIT;
     static std::atomic<bool> configured[64];
@@ -514,6 +555,15 @@ int gemm_q4_tc_status(int reset) {
     return v;
 }
 
+// Time of a launch, for the choice between this and the streaming kernel.  Experts: of the number that N rows reach of a router without
+// preferences, each with its share of the rows.
+double gemm_q4_tc_estimate_us(int64_t M, int64_t N, int64_t K, int n_experts, double reached) {
+    if (n_experts == 0) return 4.5 + 1e-3 * pick_shape(M, N, K).ns;
+    const double rows = (double)N / reached, tiles = reached * (double)((M + 255) / 256) * ceil(rows / 256.0), fit = resident_pair_clusters(1);
+    const int n = rows >= 256.0 ? 256 : ((int)rows + 31) / 32 * 32;
+    return 5.0 + 1e-3 * ceil(tiles / fit) * (2.0 * (double)((K + CHUNK - 1) / CHUNK) * step_cost(n) + 700.0);
+}
+
 // x: 16-bit rows on 16-byte boundaries, kx >= K columns of them readable (zeros past K), N rows.  Arguments are checked by the caller.
 int gemm_q4_tc_launch(const uint8_t *codes, const void *scales, const float *bias, void *C, int64_t M, const void *x, bool f16, int64_t ldx, int c_dtype, int64_t ldc, int64_t N,
                       int64_t K, int group, const int32_t *offsets, int n_experts, cudaStream_t st) {
@@ -532,47 +582,38 @@ int gemm_q4_tc_launch(const uint8_t *codes, const void *scales, const float *bia
     if (offsets) {
         // rows of an expert go evenly into tiles of at most 256
         p.bn = 256;
-        p.box_rows = 16;
         const int64_t most = (N / p.bn + (N < experts ? N : experts)) * p.m_tiles;
         clusters = (int)(most < resident ? (most < 1 ? 1 : most) : resident);
     } else {
-        const int64_t least = (N + 255) / 256, most = least + 8;
-        double best_t = 1e30;
-        for (int64_t want = least; want <= most && want <= (N + 31) / 32; ++want) {
-            const int bn = (int)(((N + want - 1) / want + 31) / 32 * 32);
-            const int64_t n_tiles = (N + bn - 1) / bn, tiles = p.m_tiles * n_tiles;
-            for (int s = 1; s <= MAX_SPLITS; ++s) {
-                const int fit = resident_pair_clusters(s);
-                if (s > p.n_chunks || (s > 1 && tiles > fit)) continue;
-                const double t = (double)((tiles + fit - 1) / fit) * (2.0 * (double)((p.n_chunks + s - 1) / s) * step_cost(bn) + 400.0) + 3.0 * bn + (s > 1 ? 1300.0 + 3.0 * bn : 0.0);
-                if (t < best_t) { best_t = t; p.bn = bn; p.n_tiles = (int)n_tiles; p.splits = s; }
-            }
-        }
-        p.box_rows = p.bn / 2;
+        const Shape shape = pick_shape(M, N, K);
+        p.bn = shape.bn; p.n_tiles = shape.n_tiles; p.splits = shape.splits;
         const int tiles = p.m_tiles * p.n_tiles;
         p.one_tile = p.splits > 1 || tiles <= resident ? 1 : 0;
         clusters = p.one_tile ? tiles : resident;
     }
     p.out_bytes = p.one_tile ? 0 : 4 * 1024 * (int)dtype_size(c_dtype);
     p.list_bytes = offsets ? ExpertList::bytes(experts) : 0;
-    // What is left after four stages of activations goes to the codes, two stages for either group of converters at least, the rest to the
-    // activations again.
+    // Two stages of codes for either group of converters, the rest for the activations (us with four, six and eight of codes: 14336 x 4096, 2048
+    // tokens 153.9, 155.9, 162.9, 37 experts of 2048 x 4096 with 256 rows each 118.5, 118.8, 129.5); four where activations are narrow (18944 x
+    // 8192, 64 tokens 38.1 and 35.7, 4096 x 14336 28.5 and 26.3).
     const int raw = RAW_CODES + CHUNK / group * 256, stage = p.bn * BK;
     const int room = SMEM_LIMIT - A_STAGES * A_CHUNK_BYTES - p.out_bytes - BARRIER_BYTES - p.list_bytes - 1024;
-    p.raw_stages = (room - 4 * stage) / raw / 2 * 2;
-    p.raw_stages = p.raw_stages > RAW_MAX ? RAW_MAX : (p.raw_stages < 4 ? 4 : p.raw_stages);
+    p.raw_stages = p.bn <= 128 ? RAW_MAX : 4;
     p.b_stages = (room - p.raw_stages * raw) / stage;
     p.b_stages = p.b_stages > B_MAX ? B_MAX : p.b_stages;
     const size_t smem = (size_t)(SMEM_LIMIT - room) + (size_t)p.raw_stages * raw + (size_t)p.b_stages * stage;
-    CUtensorMap mc, ms, mx;
+    CUtensorMap mc, ms;
+    XMaps mx;
+    memset(&mx, 0, sizeof mx);
     const int64_t tiles16 = (int64_t)experts * p.row_tiles, ktiles = q4_col_tiles(K);
     if (int rc = make_map_2d(&mc, CU_TENSOR_MAP_DATA_TYPE_UINT32, codes, (uint64_t)ktiles * 128, (uint64_t)tiles16, (uint64_t)ktiles * kQ4TileBytes, 256, 8, CU_TENSOR_MAP_SWIZZLE_NONE)) return rc;
     if (int rc = make_map_2d(&ms, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, scales, (uint64_t)(p.groups + 1) * 16, (uint64_t)tiles16, (uint64_t)(p.groups + 1) * 32, (uint32_t)(CHUNK / group) * 16, 8,
                              CU_TENSOR_MAP_SWIZZLE_NONE))
         return rc;
-    if (int rc = make_map_2d(&mx, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, x, (uint64_t)K, (uint64_t)N, (uint64_t)ldx * 2, BK, (uint32_t)p.box_rows,
-                             CU_TENSOR_MAP_SWIZZLE_128B))
-        return rc;
+    for (int k = 0; k < (offsets ? 4 : 1); ++k)
+        if (int rc = make_map_2d(&mx.m[k], f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, x, (uint64_t)K, (uint64_t)N, (uint64_t)ldx * 2, BK,
+                                 (uint32_t)(offsets ? 128 >> k : p.bn / 2), CU_TENSOR_MAP_SWIZZLE_128B))
+            return rc;
     auto go = [&](auto t, auto g, auto ct, auto e) { return launch<decltype(t), decltype(g)::value, decltype(ct), decltype(e)::value>(mc, ms, mx, p, clusters, smem, st); };
     auto by_experts = [&](auto t, auto g, auto ct) { return offsets ? go(t, g, ct, std::true_type{}) : go(t, g, ct, std::false_type{}); };
     auto by_out = [&](auto t, auto g) {

@@ -21,6 +21,7 @@
 #include "umma.cuh"
 
 #include <atomic>
+#include <cmath>
 #include <cstring>
 #include <type_traits>
 
@@ -29,6 +30,7 @@ namespace t81b200 {
 // gemm_q4_tc.cu
 int gemm_q4_tc_launch(const uint8_t *codes, const void *scales, const float *bias, void *C, int64_t M, const void *x, bool f16, int64_t ldx, int c_dtype, int64_t ldc, int64_t N,
                       int64_t K, int group, const int32_t *offsets, int n_experts, cudaStream_t st);
+double gemm_q4_tc_estimate_us(int64_t M, int64_t N, int64_t K, int n_experts, double reached);
 
 namespace {
 
@@ -97,8 +99,8 @@ template <int TOK> struct Walk {
             end = p.rows;
             if (p.offsets) {
                 expert = piece < kOwners ? owner[piece] : list.expert_of(piece, p.n_experts);
-                tok = list.first[expert] + (piece - list.before[expert]) * TOK;
-                end = list.first[expert + 1];
+                tok = list.first(expert) + (piece - list.before(expert)) * TOK;
+                end = list.first(expert + 1);
             }
             end = min(end, tok + TOK);
         }
@@ -160,8 +162,8 @@ gemv_q4_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_const
     if (p.offsets) {
         items = list.build(reinterpret_cast<int32_t *>(part + 2 * PART), p.offsets, p.n_experts, p.rows, TOK) * p.row_items;
         for (int e = threadIdx.x; e < p.n_experts; e += kThreads)
-            for (int q = list.before[e]; q < min(list.before[e + 1], kOwners); ++q) owner[q] = (int16_t)e;
-        for (int row = list.first[p.n_experts] + (int)blockIdx.x * kWarps + warp; row < p.rows; row += (int)gridDim.x * kWarps)  // rows of no expert: a warp each
+            for (int q = list.before(e); q < min(list.before(e + 1), kOwners); ++q) owner[q] = (int16_t)e;
+        for (int row = list.first(p.n_experts) + (int)blockIdx.x * kWarps + warp; row < p.rows; row += (int)gridDim.x * kWarps)  // rows of no expert: a warp each
             for (int i = lane; i < p.M; i += 32) store(p.y, (int64_t)row * p.ldy + i, 0.0f, p.y_dtype);
     }
     __syncthreads();
@@ -380,6 +382,19 @@ bool in_place(const void *B, int b_dtype, int64_t ldb, int64_t K) {
 }
 int64_t staged_row(int64_t K) { return (K + 7) & ~(int64_t)7; }
 
+// Whether the tensor-core kernel's tiles take less time than this kernel's pieces of 16 rows of x (8 of experts' rows), by both estimates.  Ours:
+// fitted to 9 to 128 rows of 512 x 512 to 32768 x 4096 and 32 to 1024 rows of 8 to 64 experts (us, tiles and pieces: 32 rows of 1024 x 4096 10.9
+// and 5.6, of 4096 x 4096 12.6 and 12.2, of 14336 x 4096 20.4 and 29.8, 64 of 2048 x 2048 9.8 and 7.9; 256 rows in 64 experts of 2816 x
+// 2048 58 and 52, 512 67 and 84).
+bool tiles_are_faster(int64_t M, int64_t N, int64_t K, int n_experts) {
+    if (N <= 16 && n_experts == 0) return false;
+    const double tiles = (double)q4_row_tiles(M) * (double)q4_col_tiles(K);
+    const double reached = n_experts == 0 ? 1.0 : n_experts * (1.0 - pow(1.0 - 1.0 / n_experts, (double)N));
+    const double pieces = n_experts == 0 ? (double)((N + 15) / 16) : reached + (double)N / 8.0;
+    const double ours = 3.5 + pieces * (n_experts == 0 ? 1.95e-4 * tiles : 0.05 + 1.15e-4 * tiles);
+    return gemm_q4_tc_estimate_us(M, N, K, n_experts, reached) < ours;
+}
+
 int product_q4(const char *name, const uint8_t *codes, const void *scales, const float *bias, void *C, int64_t M, const void *B, int b_dtype, int64_t ldb, int c_dtype, int64_t ldc,
                int64_t N, int64_t K, int group, const int32_t *offsets, int n_experts, void *workspace, size_t workspace_bytes, cudaStream_t st) {
     if (M < 0 || N < 0 || K < 0 || ldb < K || ldc < M || n_experts < 0) return fail(T81B200_EINVAL, "%s: bad dimensions", name);
@@ -410,7 +425,7 @@ int product_q4(const char *name, const uint8_t *codes, const void *scales, const
         p.kx = (int)p.ldx;
         p.plane_elems = N * p.ldx;
     }
-    if (b_dtype != T81B200_F32 && K > 0 && N >= (offsets ? 8 * (int64_t)n_experts : 33))
+    if (b_dtype != T81B200_F32 && K > 0 && tiles_are_faster(M, N, K, offsets ? n_experts : 0))
         return gemm_q4_tc_launch(codes, scales, bias, C, M, p.x, b_dtype == T81B200_F16, p.ldx, c_dtype, ldc, N, K, group, offsets, n_experts, st);
     if (b_dtype == T81B200_F32) return launch_shape<__nv_bfloat16, 3>(p, group, st);
     return b_dtype == T81B200_BF16 ? launch_shape<__nv_bfloat16, 1>(p, group, st) : launch_shape<__half, 1>(p, group, st);

@@ -28,24 +28,25 @@ inline bool q4_group_ok(int group) { return group == 32 || group == 64 || group 
 
 // Register r of a word as a pair of exact numbers -8 .. 7.  The four bits go to where the units 1 to 8 lie in the mantissa of 16 (bf16: bit
 // 3, fp16: bit 6), which gives 16 + code + 8; one packed add takes the 24 away, or one packed FMA with a scale s and -24 s.
-// The constants are made opaque: known ones are made again for every use where registers are short, which doubled the instructions of
-// the streaming kernel.
+// What an instruction cannot hold of the constants is made opaque: known ones are made again for every use where registers are short, which
+// doubled the instructions of the streaming kernel.
 __device__ __forceinline__ uint32_t opaque(uint32_t v) {
     uint32_t r;
     asm volatile("mov.b32 %0, %1;" : "=r"(r) : "r"(v));
     return r;
 }
-__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
+template <uint32_t B> __device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t c) {
     uint32_t d;
-    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(a), "n"(B), "r"(c));
     return d;
 }
 
 template <typename T> struct Q4Decode;
 template <> struct Q4Decode<__nv_bfloat16> {
-    uint32_t mask, sixteen, minus24;
-    __device__ __forceinline__ Q4Decode() : mask(opaque(0x00780078u)), sixteen(opaque(0x41804180u)), minus24(opaque(0xC1C0C1C0u)) {}
-    template <int R> __device__ __forceinline__ uint32_t biased(uint32_t w) const { return and_or(R == 0 ? w << 3 : w >> (4 * R - 3), mask, sixteen); }
+    static constexpr uint32_t mask = 0x00780078u;
+    uint32_t sixteen, minus24;
+    __device__ __forceinline__ Q4Decode() : sixteen(opaque(0x41804180u)), minus24(opaque(0xC1C0C1C0u)) {}
+    template <int R> __device__ __forceinline__ uint32_t biased(uint32_t w) const { return and_or<mask>(R == 0 ? w << 3 : w >> (4 * R - 3), sixteen); }
     __device__ __forceinline__ uint32_t code(uint32_t v) const {
         uint32_t d;
         asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(v), "r"(minus24));
@@ -55,9 +56,10 @@ template <> struct Q4Decode<__nv_bfloat16> {
     static __device__ __forceinline__ uint32_t scaled(uint32_t v, uint32_t s, uint32_t n) { return fma_bf16x2(v, s, n); }
 };
 template <> struct Q4Decode<__half> {
-    uint32_t mask, sixteen, minus24;
-    __device__ __forceinline__ Q4Decode() : mask(opaque(0x03C003C0u)), sixteen(opaque(0x4C004C00u)), minus24(opaque(0xCE00CE00u)) {}
-    template <int R> __device__ __forceinline__ uint32_t biased(uint32_t w) const { return and_or(R < 2 ? w << (6 - 4 * R) : w >> (4 * R - 6), mask, sixteen); }
+    static constexpr uint32_t mask = 0x03C003C0u;
+    uint32_t sixteen, minus24;
+    __device__ __forceinline__ Q4Decode() : sixteen(opaque(0x4C004C00u)), minus24(opaque(0xCE00CE00u)) {}
+    template <int R> __device__ __forceinline__ uint32_t biased(uint32_t w) const { return and_or<mask>(R < 2 ? w << (6 - 4 * R) : w >> (4 * R - 6), sixteen); }
     __device__ __forceinline__ uint32_t code(uint32_t v) const {
         uint32_t d;
         asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(v), "r"(minus24));
@@ -72,44 +74,43 @@ template <> struct Q4Decode<__half> {
 
 // Rows sorted by expert as a list of pieces of at most `width` rows: in shared memory, made by every block from the experts' first rows.
 struct ExpertList {
-    int32_t *first, *before;  // [experts + 1] each: an expert's first row, the pieces of experts ahead of it
+    int2 *at;  // [experts + 1]: an expert's first row, the pieces of experts ahead of it
 
     static __host__ __device__ constexpr int bytes(int n_experts) { return 2 * (n_experts + 1) * 4; }
 
     // Whole block; returns the number of pieces.  Whatever the offsets say, no row outside 0 .. rows - 1 is named.
     __device__ __forceinline__ int build(int32_t *memory, const int32_t *offsets, int n_experts, int rows, int width) {
-        first = memory;
-        before = memory + n_experts + 1;
+        at = reinterpret_cast<int2 *>(memory);
         const int lane = (int)threadIdx.x;
         if (lane < 32) {
             int sum = 0;
             for (int e0 = 0; e0 <= n_experts; e0 += 32) {
                 const int e = e0 + lane;
-                const int at = e <= n_experts ? min(max(offsets[e], 0), rows) : 0, end = e < n_experts ? min(max(offsets[e + 1], 0), rows) : 0;
-                const int pieces = e < n_experts && end > at ? (end - at + width - 1) / width : 0;
+                const int row = e <= n_experts ? min(max(offsets[e], 0), rows) : 0, end = e < n_experts ? min(max(offsets[e + 1], 0), rows) : 0;
+                const int pieces = e < n_experts && end > row ? (end - row + width - 1) / width : 0;
                 int scan = pieces;
 #pragma unroll
                 for (int d = 1; d < 32; d <<= 1) {
                     const int o = __shfl_up_sync(0xffffffffu, scan, d);
                     if (lane >= d) scan += o;
                 }
-                if (e <= n_experts) {
-                    first[e] = at;
-                    before[e] = sum + scan - pieces;
-                }
+                if (e <= n_experts) at[e] = make_int2(row, sum + scan - pieces);
                 sum += __shfl_sync(0xffffffffu, scan, 31);
             }
         }
         __syncthreads();
-        return before[n_experts];
+        return at[n_experts].y;
     }
 
-    // The expert that piece `at` belongs to.
-    __device__ __forceinline__ int expert_of(int at, int n_experts) const {
-        int lo = 0, hi = n_experts;  // the last one with before[e] <= at has a piece
+    __device__ __forceinline__ int first(int e) const { return at[e].x; }
+    __device__ __forceinline__ int before(int e) const { return at[e].y; }
+
+    // The expert that a piece belongs to.
+    __device__ __forceinline__ int expert_of(int piece, int n_experts) const {
+        int lo = 0, hi = n_experts;  // the last one with no more pieces ahead of it has a piece
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
-            if (before[mid] <= at) lo = mid;
+            if (before(mid) <= piece) lo = mid;
             else hi = mid;
         }
         return lo;
