@@ -427,7 +427,7 @@ T81B200_API size_t t81b200_gemm_trit_workspace_bytes(int b_dtype, int layout, in
  *   q4_bytes / q4_scales: bytes of the codes and number of scales of one matrix, -1 on bad arguments.
  *   quantize_q4:   `matrices` matrices `matrix_stride` elements apart, row stride ld; their codes and scales lie one behind the other
  *                  (16-byte aligned).
- *   dequantize_q4: (matrices, rows, cols) contiguous, exact in fp32 and bf16.
+ *   dequantize_q4: (matrices, rows, cols) contiguous, exact in fp32 and bf16.  q4_group_scales: (matrices, rows, groups) bf16, contiguous.
  *   linear_q4:     C (N, M) = B (N, K) W^T + bias, W (M, K); B as it is where its type is 16-bit, its rows lie on 16-byte boundaries and
  *                  K % 8 == 0, else through the workspace (linear_q4_workspace_bytes for this very B, 16-byte aligned).  Products are
  *                  exact and sums fp32; fp32 activations keep all 24 bits.
@@ -439,6 +439,7 @@ T81B200_API int64_t t81b200_q4_scales(int64_t rows, int64_t cols, int group);
 T81B200_API int t81b200_quantize_q4(const void *w, int w_dtype, int64_t matrices, int64_t rows, int64_t cols, int64_t ld, int64_t matrix_stride, int group, uint8_t *codes,
                                     void *scales, void *stream);
 T81B200_API int t81b200_dequantize_q4(const uint8_t *codes, const void *scales, int64_t matrices, int64_t rows, int64_t cols, int group, void *out, int out_dtype, void *stream);
+T81B200_API int t81b200_q4_group_scales(const void *scales, int64_t matrices, int64_t rows, int64_t cols, int group, void *out, void *stream);
 T81B200_API size_t t81b200_linear_q4_workspace_bytes(const void *B, int b_dtype, int64_t ldb, int64_t N, int64_t K);
 T81B200_API int t81b200_linear_q4(const uint8_t *codes, const void *scales, const float *bias, void *C, int64_t M, const void *B, int b_dtype, int64_t ldb, int c_dtype, int64_t ldc,
                                   int64_t N, int64_t K, int group, void *workspace, size_t workspace_bytes, void *stream);

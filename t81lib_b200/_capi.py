@@ -30,7 +30,7 @@ EXPORTS = (
     "t81b200_release_staging", "t81b200_exchange_signal", "t81b200_gemm_trit_grouped", "t81b200_t2_bytes", "t81b200_pack_t2", "t81b200_prefers_streaming", "t81b200_gemm_trit_t2", "t81b200_gemm_trit_t2_peers", "t81b200_linear_t2_workspace_bytes", "t81b200_linear_t2", "t81b200_tq_bytes", "t81b200_packed_to_tq", "t81b200_tq_to_packed",
     "t81b200_qat_update_scale", "t81b200_qat_quantize_pack", "t81b200_qat_quantize_t2", "t81b200_qat_weight_grad_workspace_bytes", "t81b200_qat_weight_grad", "t81b200_column_sums",
     "t81b200_stage_rows_ld", "t81b200_stage_rows_bytes", "t81b200_stage_rows",
-    "t81b200_q4_bytes", "t81b200_q4_scales", "t81b200_quantize_q4", "t81b200_dequantize_q4", "t81b200_linear_q4_workspace_bytes", "t81b200_linear_q4", "t81b200_experts_q4",
+    "t81b200_q4_bytes", "t81b200_q4_scales", "t81b200_quantize_q4", "t81b200_dequantize_q4", "t81b200_q4_group_scales", "t81b200_linear_q4_workspace_bytes", "t81b200_linear_q4", "t81b200_experts_q4",
     "t81b200_sort_by_expert", "t81b200_gather_rows", "t81b200_combine_rows", "t81b200_combine_rows_grad",
 )
 TQ1_0, TQ2_0 = 0, 1
@@ -119,6 +119,7 @@ def _load() -> ctypes.CDLL:
     lib.t81b200_q4_scales.restype = i64
     lib.t81b200_quantize_q4.argtypes = [vp, ci, i64, i64, i64, i64, i64, ci, vp, vp, vp]
     lib.t81b200_dequantize_q4.argtypes = [vp, vp, i64, i64, i64, ci, vp, ci, vp]
+    lib.t81b200_q4_group_scales.argtypes = [vp, i64, i64, i64, ci, vp, vp]
     lib.t81b200_linear_q4_workspace_bytes.argtypes = [vp, ci, i64, i64, i64]
     lib.t81b200_linear_q4_workspace_bytes.restype = ctypes.c_size_t
     lib.t81b200_linear_q4.argtypes = [vp, vp, vp, vp, i64, vp, ci, i64, ci, i64, i64, i64, ci, vp, ctypes.c_size_t, vp]

@@ -14,6 +14,11 @@
 // two in the row's largest, which the result is multiplied by: fp16 holds all of a row's weights then but those 2^-20 below its
 // largest, which lose places that the sums do not have.
 //
+// float32 activations come as three bf16 planes (all 24 bits, stage_planes), each a product of its own with the same expanded weights.  The tensor
+// core cuts an accumulator off at every 16 columns: 2.4e-7 of the result after 1024 columns, 5.6e-7 after 2048, 1.4e-6 after 4096, 7e-6
+// after 14336 (bf16 values, whose products are exact).  So the first plane has an accumulator per 2048 columns, the other two share one, and
+// the epilogue adds them.
+//
 // Rows sorted by expert: every CTA turns the experts' row counts into a list of tiles of its own (a sum over experts in shared memory) and the
 // persistent clusters take tiles of it in turn.  An expert's rows are split evenly into tiles of whole 32 rows; rows of a tile past
 // the expert's last are multiplied and not stored.
@@ -65,6 +70,8 @@ struct Q4TcParams {
     int n_atoms, n_chunks;
     int splits, raw_stages, b_stages, one_tile, out_bytes, list_bytes;
     int vec;                    // 16-byte stores are possible
+    int bufs, acc_cols;         // tiles whose sums TMEM holds at a time, and the columns of each
+    int seg_chunks;             // three planes: chunks of the first plane that an accumulator takes
 };
 
 // Tensor maps of x.  One matrix: [0] with boxes of half a tile.  Experts, whose tiles differ: boxes of 128, 64, 32 and 16 rows, the binary digits of
@@ -134,13 +141,31 @@ __device__ __forceinline__ void emit(const Q4TcParams &p, const uint32_t (&v)[32
     }
 }
 
+// 32 columns of a tile's sums: with three planes the accumulators of the first plane's segments, bn columns apart, and the others' behind them.
+template <int PLANES>
+__device__ __forceinline__ void load_sums(const Q4TcParams &p, uint32_t taddr, int segments, uint32_t (&v)[32]) {
+    tmem_ld32(taddr, v);
+    if constexpr (PLANES == 3)
+#pragma unroll 1
+        for (int s = 1; s <= segments; ++s) {
+            taddr += (uint32_t)p.bn;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                uint32_t more[8];
+                tmem_ld8(taddr + (uint32_t)(8 * q), more);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[8 * q + i] = __float_as_uint(__uint_as_float(v[8 * q + i]) + __uint_as_float(more[i]));
+            }
+        }
+}
+
 // The power of two in a row's largest scale (1 for a row of zeros), as the exponent bits of a float.
 __device__ __forceinline__ uint32_t row_exponent(const __nv_bfloat16 *scales, int64_t tile, int groups, int r) {
     const uint32_t bits = (uint32_t)__ldg(reinterpret_cast<const unsigned short *>(scales) + (tile * (groups + 1) + groups) * 16 + 2 * (r & 7) + (r >> 3)) & 0x7F80u;
     return bits ? bits << 16 : 0x3F800000u;
 }
 
-template <typename T, int GROUP, typename CT, bool EXPERTS>
+template <typename T, int PLANES, int GROUP, typename CT, bool EXPERTS>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
 gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_constant__ CUtensorMap map_scales, const __grid_constant__ XMaps map_x,
                   const __grid_constant__ Q4TcParams p) {
@@ -150,7 +175,7 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_co
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t *gen_base = smem_raw + (base - smem_u32(smem_raw));
-    const uint32_t b_stage_bytes = (uint32_t)p.bn * (BK * 2 / 2);  // this CTA's half of the rows
+    const uint32_t b_stage_bytes = (uint32_t)(PLANES * p.bn) * (BK * 2 / 2);  // this CTA's half of the rows
     const uint32_t b_off = A_STAGES * A_CHUNK_BYTES, raw_off = b_off + (uint32_t)p.b_stages * b_stage_bytes, out_off = raw_off + (uint32_t)p.raw_stages * RAW_BYTES;
     const uint32_t bars = base + out_off + (uint32_t)p.out_bytes;
     auto a_full = [&](int s) { return bars + 8u * s; };
@@ -192,6 +217,7 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_co
     const int n_clusters = (int)gridDim.x / (2 * p.splits), cluster_id = (int)blockIdx.x / (2 * p.splits);
     const int c0 = p.n_chunks * slice / p.splits, c1 = p.n_chunks * (slice + 1) / p.splits;
     const uint16_t pair_mask = (uint16_t)(3u << (rank & ~1u));
+    const int segments = PLANES == 3 ? (c1 - c0 + p.seg_chunks - 1) / p.seg_chunks : 0;
 
     if constexpr (EXPERTS) {  // rows of no expert: a warp each
         const int kept = tiles.list.first(p.n_experts);
@@ -225,17 +251,20 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_co
                     ok = mbar_wait(b_empty(b.stage), b.phase ^ 1);
                     if (!ok) break;
                     if (elect_one()) {
-                        if (half == 0) mbar_arrive_expect_tx(b_full(b.stage), 2u * (uint32_t)rows * (BK * 2));
-                        const uint32_t dst = base + b_off + (uint32_t)b.stage * b_stage_bytes;
-                        if constexpr (EXPERTS) {
-                            int done = 0;
+                        if (half == 0) mbar_arrive_expect_tx(b_full(b.stage), 2u * (uint32_t)(PLANES * rows) * (BK * 2));
+                        uint32_t dst = base + b_off + (uint32_t)b.stage * b_stage_bytes;
 #pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                if (rows & (128 >> k)) {
-                                    tma_load_2d_pair(dst + (uint32_t)done * (BK * 2), &map_x.m[k], a * BK, row + done, b_full(b.stage));
-                                    done += 128 >> k;
-                                }
-                        } else tma_load_2d_pair(dst, &map_x.m[0], a * BK, row, b_full(b.stage));
+                        for (int pl = 0; pl < PLANES; ++pl, dst += (uint32_t)rows * (BK * 2)) {
+                            if constexpr (EXPERTS) {
+                                int done = 0;
+#pragma unroll
+                                for (int k = 0; k < 4; ++k)
+                                    if (rows & (128 >> k)) {
+                                        tma_load_2d_pair(dst + (uint32_t)done * (BK * 2), &map_x.m[k], a * BK, pl * p.N + row + done, b_full(b.stage));
+                                        done += 128 >> k;
+                                    }
+                            } else tma_load_2d_pair(dst, &map_x.m[0], a * BK, pl * p.N + row, b_full(b.stage));
+                        }
                     }
                     __syncwarp();
                     b.advance(p.b_stages);
@@ -278,12 +307,14 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_co
             int it = 0;
             for (int i = cluster_id; i < total_tiles && ok; i += n_clusters, ++it) {
                 const Tile t = tiles.tile(p, i, half);
-                const int buf = it & 1;
+                const int buf = it & (p.bufs - 1);
                 const uint32_t idesc = umma_instr_desc(t.n, F16);
-                ok = mbar_wait(acc_empty(buf), ((uint32_t)(it >> 1) & 1u) ^ 1u);
+                ok = mbar_wait(acc_empty(buf), ((uint32_t)(it >> (p.bufs - 1)) & 1u) ^ 1u);
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t d_tmem = tmem_base + (uint32_t)buf * 256u;
+                uint32_t d_tmem = tmem_base + (uint32_t)(buf * p.acc_cols);
+                const uint32_t d_rest = d_tmem + (uint32_t)(segments * p.bn);
+                int of_segment = 0;
                 for (int c = c0; c < c1 && ok; ++c) {
                     ok = mbar_wait(a_full(a.stage), a.phase);
                     if (!ok) break;
@@ -297,7 +328,15 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_co
                             const uint64_t ad = umma_desc_k(base + (uint32_t)a.stage * A_CHUNK_BYTES + (uint32_t)j * A_ATOM_BYTES);
 #pragma unroll
                             for (int k = 0; k < BK / 16; ++k)
-                                umma_pair(d_tmem, ad + (uint64_t)(2 * k), bd + (uint64_t)(2 * k), idesc, c > c0 || j > 0 || k > 0 ? 1u : 0u);
+                                umma_pair(d_tmem, ad + (uint64_t)(2 * k), bd + (uint64_t)(2 * k), idesc, (PLANES == 3 ? of_segment > 0 : c > c0) || j > 0 || k > 0 ? 1u : 0u);
+                            if constexpr (PLANES == 3)
+#pragma unroll
+                                for (int pl = 1; pl < 3; ++pl) {
+                                    const uint64_t bp = bd + (uint64_t)((uint32_t)(pl * (t.n / 2)) * (BK * 2) >> 4);
+#pragma unroll
+                                    for (int k = 0; k < BK / 16; ++k)
+                                        umma_pair(d_rest, ad + (uint64_t)(2 * k), bp + (uint64_t)(2 * k), idesc, c > c0 || j > 0 || pl > 1 || k > 0 ? 1u : 0u);
+                                }
                             umma_commit_pair(b_empty(b.stage), pair_mask);
                         }
                         __syncwarp();
@@ -307,6 +346,10 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_co
                     if (elect_one()) umma_commit_pair(a_empty(a.stage), pair_mask);
                     __syncwarp();
                     a.advance(A_STAGES);
+                    if (PLANES == 3 && ++of_segment == p.seg_chunks) {
+                        of_segment = 0;
+                        d_tmem += (uint32_t)p.bn;
+                    }
                 }
                 if (ok && elect_one()) umma_commit_pair(acc_full(buf), pair_mask);
                 __syncwarp();
@@ -321,15 +364,15 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_co
         int it = 0;
         for (int i = cluster_id; i < total_tiles && ok; i += n_clusters, ++it) {
             const Tile t = tiles.tile(p, i, half);
-            const int buf = it & 1, r = quarter * 32 + lane;
+            const int buf = it & (p.bufs - 1), r = quarter * 32 + lane;
             const float factor = p.one_tile ? 1.0f : factor_of(t, r), bias = p.one_tile ? 0.0f : bias_of(t, r);
-            ok = epilogue_all(mbar_wait(acc_full(buf), (uint32_t)(it >> 1) & 1u));
+            ok = epilogue_all(mbar_wait(acc_full(buf), (uint32_t)(it >> (p.bufs - 1)) & 1u));
             if (!ok || p.one_tile) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
             for (int b = 0; b < t.n / 32; ++b) {
                 uint32_t v[32];
-                tmem_ld32(tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * 256 + b * 32), v);
+                load_sums<PLANES>(p, tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * p.acc_cols + b * 32), segments, v);
                 emit<CT>(p, v, t.row0 + quarter * 32, lane, factor, bias, t.tok + b * 32, t.end, stage);
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -461,7 +504,7 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_co
                     const int to = b % S;
                     if (to == slice) continue;
                     uint32_t v[32];
-                    tmem_ld32(t_lane + (uint32_t)(b * 32), v);
+                    load_sums<PLANES>(p, t_lane + (uint32_t)(b * 32), segments, v);
                     push_partial(v, base + partial_slot(b, S, slice, to) * 16384u + r * 4u, (uint32_t)(2 * to + half));
                 }
             __syncthreads();
@@ -471,7 +514,7 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_co
             CT *stage = reinterpret_cast<CT *>(gen_base + b_off) + (group * 4 + quarter) * 1024;
             for (int b = slice + S * group; b < blocks; b += FINISHERS * S) {
                 uint32_t v[32];
-                tmem_ld32(t_lane + (uint32_t)(b * 32), v);
+                load_sums<PLANES>(p, t_lane + (uint32_t)(b * 32), segments, v);
                 if (S > 1) fold_partials(v, gen_base, b, S, slice, r);
                 emit<CT>(p, v, t.row0 + quarter * 32, lane, factor, bias, t.tok + b * 32, t.end, stage);
             }
@@ -487,11 +530,23 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_co
     }
 }
 
-// Time of a 64-deep step at n columns, in ns: 18944 rows of 8192 columns, one tile a pair, 34 to 256 rows of x, without 5.5 us.
-double step_cost(int n) {
-    constexpr double cost[9] = {235, 235, 236, 252, 259, 279, 297, 349, 375};  // 0, 32, .. 256 columns
-    const int at = n / 32;
-    return n % 32 == 0 ? cost[at] : cost[at] + (cost[at + 1] - cost[at]) * (n % 32) / 32;
+// Time of a 64-deep step at n columns, in ns: 18944 rows of 8192 columns (4096 for wide tiles of three planes), one tile a pair, 34 to 256 rows of
+// x, without 5.5 us.
+double step_cost(int n, int planes) {
+    constexpr double one[9] = {235, 235, 236, 252, 259, 279, 297, 349, 375}, three[5] = {300, 300, 331, 417, 533};  // 0, 32, .. columns
+    return planes == 3 ? three[n / 32] : one[n / 32];
+}
+
+// Three planes: chunks that an accumulator takes (2048 columns), and the widest tile whose accumulators TMEM holds: one per 2048 columns and one
+// for the other planes.  (Beyond 30720 columns an accumulator takes more of them.)
+constexpr int SEGMENT = 2048 / CHUNK;
+int segments_of(int64_t K) {
+    const int64_t n = (K + SEGMENT * CHUNK - 1) / (SEGMENT * CHUNK);
+    return n < 1 ? 1 : (n > 15 ? 15 : (int)n);
+}
+int widest_of_planes(int64_t K) {
+    const int s = segments_of(K);
+    return s <= 3 ? 128 : (s <= 7 ? 64 : 32);
 }
 
 // Tile width and split of one matrix: the smallest estimate, in ns without the launch.
@@ -499,8 +554,8 @@ struct Shape {
     int bn = 0, n_tiles = 0, splits = 1;
     double ns = 1e30;
 };
-Shape pick_shape(int64_t M, int64_t N, int64_t K) {
-    const int64_t m_tiles = (M + 255) / 256, chunks = (K + CHUNK - 1) / CHUNK, least = (N + 255) / 256;
+Shape pick_shape(int64_t M, int64_t N, int64_t K, int planes) {
+    const int64_t m_tiles = (M + 255) / 256, chunks = (K + CHUNK - 1) / CHUNK, most = planes == 3 ? widest_of_planes(K) : 256, least = (N + most - 1) / most;
     Shape best;
     for (int64_t want = least; want <= least + 8 && want <= (N + 31) / 32; ++want) {
         const int bn = (int)(((N + want - 1) / want + 31) / 32 * 32);
@@ -508,16 +563,16 @@ Shape pick_shape(int64_t M, int64_t N, int64_t K) {
         for (int s = 1; s <= MAX_SPLITS; ++s) {
             const int fit = resident_pair_clusters(s);
             if (s > chunks || (s > 1 && tiles > fit)) continue;
-            const double ns = (double)((tiles + fit - 1) / fit) * (2.0 * (double)((chunks + s - 1) / s) * step_cost(bn) + 700.0) + 5.0 * bn + (s > 1 ? 2200.0 + 5.0 * bn : 0.0);
+            const double ns = (double)((tiles + fit - 1) / fit) * (2.0 * (double)((chunks + s - 1) / s) * step_cost(bn, planes) + 700.0) + 5.0 * bn + (s > 1 ? 2200.0 + 5.0 * bn : 0.0);
             if (ns < best.ns) best = {bn, (int)n_tiles, s, ns};
         }
     }
     return best;
 }
 
-template <typename T, int GROUP, typename CT, bool EXPERTS>
+template <typename T, int PLANES, int GROUP, typename CT, bool EXPERTS>
 int launch(const CUtensorMap &mc, const CUtensorMap &ms, const XMaps &mx, const Q4TcParams &p, int clusters, size_t smem, cudaStream_t st) {
-    auto kern = gemm_q4_tc_kernel<T, GROUP, CT, EXPERTS>;
+    auto kern = gemm_q4_tc_kernel<T, PLANES, GROUP, CT, EXPERTS>;
     constexpr int most = SMEM_LIMIT;
     static std::atomic<bool> configured[64];
     int dev = 0;
@@ -557,15 +612,17 @@ int gemm_q4_tc_status(int reset) {
 
 // Time of a launch, for the choice between this and the streaming kernel.  Experts: of the number that N rows reach of a router without
 // preferences, each with its share of the rows.
-double gemm_q4_tc_estimate_us(int64_t M, int64_t N, int64_t K, int n_experts, double reached) {
-    if (n_experts == 0) return 4.5 + 1e-3 * pick_shape(M, N, K).ns;
-    const double rows = (double)N / reached, tiles = reached * (double)((M + 255) / 256) * ceil(rows / 256.0), fit = resident_pair_clusters(1);
-    const int n = rows >= 256.0 ? 256 : ((int)rows + 31) / 32 * 32;
-    return 5.0 + 1e-3 * ceil(tiles / fit) * (2.0 * (double)((K + CHUNK - 1) / CHUNK) * step_cost(n) + 700.0);
+double gemm_q4_tc_estimate_us(int64_t M, int64_t N, int64_t K, int planes, int n_experts, double reached) {
+    if (n_experts == 0) return 4.5 + 1e-3 * pick_shape(M, N, K, planes).ns;
+    const double most = planes == 3 ? widest_of_planes(K) : 256;
+    const double rows = (double)N / reached, tiles = reached * (double)((M + 255) / 256) * ceil(rows / most), fit = resident_pair_clusters(1);
+    const int n = rows >= most ? (int)most : ((int)rows + 31) / 32 * 32;
+    return 5.0 + 1e-3 * ceil(tiles / fit) * (2.0 * (double)((K + CHUNK - 1) / CHUNK) * step_cost(n, planes) + 700.0);
 }
 
-// x: 16-bit rows on 16-byte boundaries, kx >= K columns of them readable (zeros past K), N rows.  Arguments are checked by the caller.
-int gemm_q4_tc_launch(const uint8_t *codes, const void *scales, const float *bias, void *C, int64_t M, const void *x, bool f16, int64_t ldx, int c_dtype, int64_t ldc, int64_t N,
+// x: 16-bit rows on 16-byte boundaries, K columns of them, N rows; with three planes three times N, and C is float32.  Arguments are checked by
+// the caller.
+int gemm_q4_tc_launch(const uint8_t *codes, const void *scales, const float *bias, void *C, int64_t M, const void *x, bool f16, int planes, int64_t ldx, int c_dtype, int64_t ldc, int64_t N,
                       int64_t K, int group, const int32_t *offsets, int n_experts, cudaStream_t st) {
     Q4TcParams p;
     memset(&p, 0, sizeof p);
@@ -581,11 +638,11 @@ int gemm_q4_tc_launch(const uint8_t *codes, const void *scales, const float *bia
     int clusters;
     if (offsets) {
         // rows of an expert go evenly into tiles of at most 256
-        p.bn = 256;
+        p.bn = planes == 3 ? widest_of_planes(K) : 256;
         const int64_t most = (N / p.bn + (N < experts ? N : experts)) * p.m_tiles;
         clusters = (int)(most < resident ? (most < 1 ? 1 : most) : resident);
     } else {
-        const Shape shape = pick_shape(M, N, K);
+        const Shape shape = pick_shape(M, N, K, planes);
         p.bn = shape.bn; p.n_tiles = shape.n_tiles; p.splits = shape.splits;
         const int tiles = p.m_tiles * p.n_tiles;
         p.one_tile = p.splits > 1 || tiles <= resident ? 1 : 0;
@@ -596,9 +653,9 @@ int gemm_q4_tc_launch(const uint8_t *codes, const void *scales, const float *bia
     // Two stages of codes for either group of converters, the rest for the activations (us with four, six and eight of codes: 14336 x 4096, 2048
     // tokens 153.9, 155.9, 162.9, 37 experts of 2048 x 4096 with 256 rows each 118.5, 118.8, 129.5); four where activations are narrow (18944 x
     // 8192, 64 tokens 38.1 and 35.7, 4096 x 14336 28.5 and 26.3).
-    const int raw = RAW_CODES + CHUNK / group * 256, stage = p.bn * BK;
+    const int raw = RAW_CODES + CHUNK / group * 256, stage = planes * p.bn * BK;
     const int room = SMEM_LIMIT - A_STAGES * A_CHUNK_BYTES - p.out_bytes - BARRIER_BYTES - p.list_bytes - 1024;
-    p.raw_stages = p.bn <= 128 ? RAW_MAX : 4;
+    p.raw_stages = planes * p.bn <= 128 ? RAW_MAX : 4;
     p.b_stages = (room - p.raw_stages * raw) / stage;
     p.b_stages = p.b_stages > B_MAX ? B_MAX : p.b_stages;
     const size_t smem = (size_t)(SMEM_LIMIT - room) + (size_t)p.raw_stages * raw + (size_t)p.b_stages * stage;
@@ -611,16 +668,29 @@ int gemm_q4_tc_launch(const uint8_t *codes, const void *scales, const float *bia
                              CU_TENSOR_MAP_SWIZZLE_NONE))
         return rc;
     for (int k = 0; k < (offsets ? 4 : 1); ++k)
-        if (int rc = make_map_2d(&mx.m[k], f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, x, (uint64_t)K, (uint64_t)N, (uint64_t)ldx * 2, BK,
+        if (int rc = make_map_2d(&mx.m[k], f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, x, (uint64_t)K, (uint64_t)(planes * N), (uint64_t)ldx * 2, BK,
                                  (uint32_t)(offsets ? 128 >> k : p.bn / 2), CU_TENSOR_MAP_SWIZZLE_128B))
             return rc;
-    auto go = [&](auto t, auto g, auto ct, auto e) { return launch<decltype(t), decltype(g)::value, decltype(ct), decltype(e)::value>(mc, ms, mx, p, clusters, smem, st); };
-    auto by_experts = [&](auto t, auto g, auto ct) { return offsets ? go(t, g, ct, std::true_type{}) : go(t, g, ct, std::false_type{}); };
+    p.bufs = 2;
+    p.acc_cols = 256;
+    if (planes == 3) {
+        const int share = (p.n_chunks + p.splits - 1) / p.splits, segments = segments_of((int64_t)share * CHUNK);
+        p.seg_chunks = (share + segments - 1) / segments;
+        p.acc_cols = (segments + 1) * p.bn;
+        p.bufs = 2 * p.acc_cols <= (int)kTmemCols ? 2 : 1;
+    }
+    auto go = [&](auto t, auto pl, auto g, auto ct, auto e) {
+        return launch<decltype(t), decltype(pl)::value, decltype(g)::value, decltype(ct), decltype(e)::value>(mc, ms, mx, p, clusters, smem, st);
+    };
+    using One = std::integral_constant<int, 1>;
+    auto by_experts = [&](auto t, auto pl, auto g, auto ct) { return offsets ? go(t, pl, g, ct, std::true_type{}) : go(t, pl, g, ct, std::false_type{}); };
     auto by_out = [&](auto t, auto g) {
+        if constexpr (std::is_same<decltype(t), __nv_bfloat16>::value)
+            if (planes == 3) return by_experts(t, std::integral_constant<int, 3>{}, g, float{});
         switch (c_dtype) {
-            case T81B200_F32: return by_experts(t, g, float{});
-            case T81B200_BF16: return by_experts(t, g, __nv_bfloat16{});
-            default: return by_experts(t, g, __half{});
+            case T81B200_F32: return by_experts(t, One{}, g, float{});
+            case T81B200_BF16: return by_experts(t, One{}, g, __nv_bfloat16{});
+            default: return by_experts(t, One{}, g, __half{});
         }
     };
     auto by_group = [&](auto t) {

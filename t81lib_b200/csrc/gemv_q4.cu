@@ -28,9 +28,9 @@
 namespace t81b200 {
 
 // gemm_q4_tc.cu
-int gemm_q4_tc_launch(const uint8_t *codes, const void *scales, const float *bias, void *C, int64_t M, const void *x, bool f16, int64_t ldx, int c_dtype, int64_t ldc, int64_t N,
+int gemm_q4_tc_launch(const uint8_t *codes, const void *scales, const float *bias, void *C, int64_t M, const void *x, bool f16, int planes, int64_t ldx, int c_dtype, int64_t ldc, int64_t N,
                       int64_t K, int group, const int32_t *offsets, int n_experts, cudaStream_t st);
-double gemm_q4_tc_estimate_us(int64_t M, int64_t N, int64_t K, int n_experts, double reached);
+double gemm_q4_tc_estimate_us(int64_t M, int64_t N, int64_t K, int planes, int n_experts, double reached);
 
 namespace {
 
@@ -385,14 +385,14 @@ int64_t staged_row(int64_t K) { return (K + 7) & ~(int64_t)7; }
 // Whether the tensor-core kernel's tiles take less time than this kernel's pieces of 16 rows of x (8 of experts' rows), by both estimates.  Ours:
 // fitted to 9 to 128 rows of 512 x 512 to 32768 x 4096 and 32 to 1024 rows of 8 to 64 experts (us, tiles and pieces: 32 rows of 1024 x 4096 10.9
 // and 5.6, of 4096 x 4096 12.6 and 12.2, of 14336 x 4096 20.4 and 29.8, 64 of 2048 x 2048 9.8 and 7.9; 256 rows in 64 experts of 2816 x
-// 2048 58 and 52, 512 67 and 84).
-bool tiles_are_faster(int64_t M, int64_t N, int64_t K, int n_experts) {
-    if (N <= 16 && n_experts == 0) return false;
+// 2048 58 and 52, 512 67 and 84).  float32, pieces of 8: 77 rows of 1999 x 3001 15.3 and 24.0, 256 of 14336 x 4096 69 and 406.
+bool tiles_are_faster(int64_t M, int64_t N, int64_t K, int planes, int n_experts) {
+    if (N <= (planes == 3 ? 8 : 16) && n_experts == 0) return false;
     const double tiles = (double)q4_row_tiles(M) * (double)q4_col_tiles(K);
     const double reached = n_experts == 0 ? 1.0 : n_experts * (1.0 - pow(1.0 - 1.0 / n_experts, (double)N));
-    const double pieces = n_experts == 0 ? (double)((N + 15) / 16) : reached + (double)N / 8.0;
-    const double ours = 3.5 + pieces * (n_experts == 0 ? 1.95e-4 * tiles : 0.05 + 1.15e-4 * tiles);
-    return gemm_q4_tc_estimate_us(M, N, K, n_experts, reached) < ours;
+    const double pieces = n_experts != 0 ? reached + (double)N / 8.0 : (double)(planes == 3 ? (N + 7) / 8 : (N + 15) / 16);
+    const double ours = 3.5 + pieces * (planes == 3 ? 0.05 + 3.2e-4 * tiles : (n_experts == 0 ? 1.95e-4 * tiles : 0.05 + 1.15e-4 * tiles));
+    return gemm_q4_tc_estimate_us(M, N, K, planes, n_experts, reached) < ours;
 }
 
 int product_q4(const char *name, const uint8_t *codes, const void *scales, const float *bias, void *C, int64_t M, const void *B, int b_dtype, int64_t ldb, int c_dtype, int64_t ldc,
@@ -425,8 +425,9 @@ int product_q4(const char *name, const uint8_t *codes, const void *scales, const
         p.kx = (int)p.ldx;
         p.plane_elems = N * p.ldx;
     }
-    if (b_dtype != T81B200_F32 && K > 0 && tiles_are_faster(M, N, K, offsets ? n_experts : 0))
-        return gemm_q4_tc_launch(codes, scales, bias, C, M, p.x, b_dtype == T81B200_F16, p.ldx, c_dtype, ldc, N, K, group, offsets, n_experts, st);
+    const int planes = b_dtype == T81B200_F32 ? 3 : 1;
+    if (K > 0 && (planes == 1 || (c_dtype == T81B200_F32 && 3 * N < (1ll << 31))) && tiles_are_faster(M, N, K, planes, offsets ? n_experts : 0))
+        return gemm_q4_tc_launch(codes, scales, bias, C, M, p.x, b_dtype == T81B200_F16, planes, p.ldx, c_dtype, ldc, N, K, group, offsets, n_experts, st);
     if (b_dtype == T81B200_F32) return launch_shape<__nv_bfloat16, 3>(p, group, st);
     return b_dtype == T81B200_BF16 ? launch_shape<__nv_bfloat16, 1>(p, group, st) : launch_shape<__half, 1>(p, group, st);
 }

@@ -303,6 +303,16 @@ __global__ void __launch_bounds__(kThreads) dequantize_q4_kernel(const uint4 *__
     }
 }
 
+// Scales in the matrix's order: a thread each, stores side by side.
+__global__ void __launch_bounds__(kThreads) group_scales_kernel(const uint16_t *__restrict__ scales, int64_t rows, int64_t groups, int64_t total, uint16_t *__restrict__ out) {
+    wait_for_kernel_ahead();
+    const int64_t tiles = q4_row_tiles(rows);
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < total; i += (int64_t)gridDim.x * kThreads) {
+        const int64_t u = i % groups, row_of_all = i / groups, matrix = row_of_all / rows, row = row_of_all % rows;
+        out[i] = scales[((matrix * tiles + (row >> 4)) * (groups + 1) + u) * 16 + 2 * (row & 7) + ((row >> 3) & 1)];
+    }
+}
+
 template <typename T>
 int launch_quantize(const void *w, int64_t matrices, int64_t rows, int64_t cols, int64_t ld, int64_t matrix_stride, int group, uint8_t *codes, void *scales, cudaStream_t st) {
     const int64_t blocks = q4_row_tiles(rows);
@@ -375,4 +385,16 @@ extern "C" int t81b200_dequantize_q4(const uint8_t *codes, const void *scales, i
         case T81B200_F16: return launch_dequantize<__half>(codes, scales, matrices, rows, cols, group, out, st);
     }
     return fail(T81B200_EINVAL, "dequantize_q4: unknown dtype %d", out_dtype);
+}
+
+extern "C" int t81b200_q4_group_scales(const void *scales, int64_t matrices, int64_t rows, int64_t cols, int group, void *out, void *stream) {
+    if (matrices < 0 || rows < 0 || cols < 0) return fail(T81B200_EINVAL, "q4_group_scales: bad dimensions");
+    if (!q4_group_ok(group)) return fail(T81B200_EINVAL, "q4_group_scales: groups of 32, 64 or 128 columns, not %d", group);
+    if (int rc = check_device()) return rc;
+    if (matrices == 0 || rows == 0 || cols == 0) return T81B200_OK;
+    if (!scales || !out) return fail(T81B200_EINVAL, "q4_group_scales: null pointer");
+    const int64_t groups = q4_groups(cols, group), total = matrices * rows * groups, blocks = (total + kThreads - 1) / kThreads, most = (int64_t)sm_count() * 16;
+    T81_CUDA_TRY(launch_behind(group_scales_kernel, dim3((unsigned)(blocks < most ? blocks : most)), kThreads, 0, static_cast<cudaStream_t>(stream), static_cast<const uint16_t *>(scales), rows,
+                               groups, total, static_cast<uint16_t *>(out)));
+    return T81B200_OK;
 }

@@ -716,6 +716,28 @@ PyObject *dequantize_q4(PyObject *, PyObject *const *args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// q4_group_scales(scales, matrices, rows, cols, group) -> (matrices, rows, groups)
+PyObject *q4_group_scales(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 5) return PyErr_Format(PyExc_TypeError, "q4_group_scales takes 5 arguments");
+    const Tensor &scales = tensor_of(args[0]);
+    const int64_t matrices = PyLong_AsLongLong(args[1]), rows = PyLong_AsLongLong(args[2]), cols = PyLong_AsLongLong(args[3]), group = PyLong_AsLongLong(args[4]);
+    if (PyErr_Occurred()) return nullptr;
+    TORCH_CHECK_VALUE(matrices >= 0 && rows >= 0 && cols >= 0 && (group == 32 || group == 64 || group == 128) && scales.is_cuda() && scales.scalar_type() == at::kBFloat16 &&
+                          scales.is_contiguous() && scales.numel() == matrices * t81b200_q4_scales(rows, cols, (int)group),
+                      "scales are not those of such matrices");
+    const c10::Device device = scales.device();
+    OnDevice on(device);
+    Tensor out = at::empty({matrices, rows, (cols + group - 1) / group}, scales.options());
+    try {
+        check(t81b200_q4_group_scales(scales.const_data_ptr(), matrices, rows, cols, (int)group, out.mutable_data_ptr(), stream_of(device)));
+    } catch (const LibraryError &e) {
+        return raise_library_error(e.code);
+    }
+    return THPVariable_Wrap(out);
+    END_HANDLE_TH_ERRORS
+}
+
 // linear_q4(codes, scales, rows, k, group, x, bias or None, out_dtype or None, offsets or None, n_experts): x (tokens, k) with unit column
 // stride; with offsets (n_experts + 1 int32) the rows are sorted by expert and the weights hold n_experts matrices, the bias (n_experts, rows).
 PyObject *linear_q4(PyObject *, PyObject *const *args, Py_ssize_t n) {
@@ -919,6 +941,7 @@ PyMethodDef methods[] = {
     {"qat_weight_grad", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(qat_weight_grad)), METH_FASTCALL, nullptr},
     {"quantize_q4", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(quantize_q4)), METH_FASTCALL, nullptr},
     {"dequantize_q4", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(dequantize_q4)), METH_FASTCALL, nullptr},
+    {"q4_group_scales", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(q4_group_scales)), METH_FASTCALL, nullptr},
     {"linear_q4", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(linear_q4)), METH_FASTCALL, nullptr},
     {"sort_by_expert", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(sort_by_expert)), METH_FASTCALL, nullptr},
     {"gather_rows", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(gather_rows)), METH_FASTCALL, nullptr},

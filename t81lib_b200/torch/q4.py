@@ -25,9 +25,9 @@ class Q4Tensor:
             raise ValueError("a Q4Tensor is a 2D matrix or a 3D stack of them")
         if group not in (32, 64, 128):
             raise ValueError(f"groups of 32, 64 or 128 columns, not {group}")
-        matrices = shape[0] if len(shape) == 3 else 1
-        if codes.dtype != torch.uint8 or codes.numel() != matrices * _capi.lib.t81b200_q4_bytes(*shape[-2:]) or scales.dtype != torch.bfloat16 \
-                or scales.numel() != matrices * _capi.lib.t81b200_q4_scales(*shape[-2:], group) or scales.device != codes.device:
+        matrices, tiles = (shape[0] if len(shape) == 3 else 1), (shape[-2] + 15) // 16
+        if codes.dtype != torch.uint8 or codes.numel() != matrices * tiles * ((shape[-1] + 63) // 64) * 512 or scales.dtype != torch.bfloat16 \
+                or scales.numel() != matrices * tiles * ((shape[-1] + group - 1) // group + 1) * 16 or scales.device != codes.device:
             raise ValueError(f"codes and scales do not hold a {tuple(shape)} weight with groups of {group}")
         self.codes, self.scales, self.shape, self.group = codes, scales, shape, group
         self._product = None  # the native call
@@ -50,15 +50,14 @@ class Q4Tensor:
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """The weights that the codes stand for; exact in float32 and bfloat16."""
         matrices = self.shape[0] if len(self.shape) == 3 else 1
-        return ops.dequantize_q4(self.codes, self.scales, self.shape[-2], self.shape[-1], self.group, matrices, dtype).view(self.shape)
+        values = ops.dequantize_q4(self.codes, self.scales, self.shape[-2], self.shape[-1], self.group, matrices, dtype)
+        return values if len(self.shape) == 3 else values[0]
 
     def group_scales(self) -> torch.Tensor:
         """bfloat16 (..., rows, groups)."""
-        rows, cols = self.shape[-2:]
-        groups = (cols + self.group - 1) // self.group
-        s = self.scales.view(*self.shape[:-2], (rows + 15) // 16, groups + 1, 8, 2)[..., :groups, :, :]
-        # row r of a tile lies at [r % 8, r / 8]
-        return s.movedim((-1, -2), (-3, -2)).flatten(-4, -2)[..., :rows, :].contiguous()
+        matrices = self.shape[0] if len(self.shape) == 3 else 1
+        s = _capi.native.q4_group_scales(self.scales, matrices, self.shape[-2], self.shape[-1], self.group)
+        return s if len(self.shape) == 3 else s[0]
 
     def _native_product(self):
         if self._product is None and len(self.shape) == 2 and self.shape.numel() > 0:

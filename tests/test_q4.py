@@ -135,7 +135,8 @@ def test_quantise_strided_and_stacked(dev):
                 on = wide.to(dev).to(dtype).transpose(1, 2)
             q = t81_torch.Q4Tensor.from_float(on, group=64)
             assert q.shape == w.shape
-            assert torch.equal(q.dequantize().cpu().double(), ref.quantize(source, 64)[2])
+            _, scales, values = ref.quantize(source, 64)
+            assert torch.equal(q.dequantize().cpu().double(), values) and torch.equal(q.group_scales().cpu().double(), scales)
 
 
 @pytest.mark.gpu
@@ -186,6 +187,21 @@ def test_product_of_many_rows(dev, rows, cols, tokens):
         q, x, b = _case(gen, dev, rows, cols, tokens, dtype, (32, 64, 128)[i], i == 0)
         _check(q.matmul_input(x, b), x, q, b)
         _check(q.matmul_input(x, None, out_dtype=torch.float32), x, q, None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,cols,tokens", [(300, 2048, 300), (256, 2049, 70), (300, 6144, 200), (513, 8200, 129), (100, 14336, 150), (64, 31000, 40), (40, 40000, 65), (20000, 128, 33)])
+def test_float32_sums_of_long_rows(dev, rows, cols, tokens):
+    """Many float32 rows: accumulators per 2048 columns keep the error below what 2048 columns' worth of cut-off steps and a few roundings make."""
+    gen = torch.Generator(device="cuda").manual_seed(cols)
+    q, x, b = _case(gen, dev, rows, cols, tokens, torch.float32, 64, True)
+    want, magnitude = ref.product(x, q.dequantize().double(), b)
+    y = q.matmul_input(x, b)
+    _check(y, x, q, b)
+    # 128 steps of at most 2^-23 of the sum so far, which is at most some three times the root of the terms' squares, twenty more roundings; the
+    # accumulators' errors are independent of one another
+    rms = (x.double() ** 2 @ (q.dequantize().double() ** 2).t()).sqrt()
+    assert bool(((y.double() - want).abs() <= (128 * 3 + 20 * 5) * 2.0 ** -23 * rms + 2.0 ** -23 * b.double().abs()).all())
 
 
 @pytest.mark.gpu
