@@ -563,15 +563,17 @@ gemm_trit_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
             RawChunk<FMT> words;
             const int slot = raw.stage < RAW_STAGES ? raw.stage : raw.stage - RAW_STAGES;
             read_chunk<FMT>(p, gen_base + raw_off + slot * kRawBytes<FMT>, rt, c, lane, words);
-            __syncwarp();
-            if (lane == 0) mbar_arrive(raw_empty(slot));
             ok = __all_sync(0xffffffffu, mbar_wait(a_empty(a.stage), a.phase ^ 1));
             if (!ok) break;
             expand_chunk<FMT>(words, gen_base + a.stage * A_CHUNK_BYTES + rt * 4096, lane, p.one_mask);
             // generic-proxy writes must be visible to the tensor core's async proxy
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
-            if (lane == 0) mbar_arrive_leader(a_full(a.stage));
+            // The words are handed back only now that they have been used: an arrival overtakes loads of shared memory that are still on their way.
+            if (lane == 0) {
+                mbar_arrive_leader(a_full(a.stage));
+                mbar_arrive(raw_empty(slot));
+            }
             a.advance(p.a_stages);
             a.advance(p.a_stages);
             raw.advance(RAW_BARRIERS);
