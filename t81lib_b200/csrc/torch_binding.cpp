@@ -743,7 +743,7 @@ PyObject *q4_group_scales(PyObject *, PyObject *const *args, Py_ssize_t n) {
 PyObject *linear_q4(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     if (n != 10) return PyErr_Format(PyExc_TypeError, "linear_q4 takes 10 arguments");
-    const Tensor &codes = tensor_of(args[0]), &scales = tensor_of(args[1]), &x = tensor_of(args[5]);
+    const Tensor &codes = tensor_of(args[0]), &scales = tensor_of(args[1]), x = tensor_of(args[5]).resolve_neg();
     const int64_t rows = PyLong_AsLongLong(args[2]), k = PyLong_AsLongLong(args[3]), group = PyLong_AsLongLong(args[4]), experts = PyLong_AsLongLong(args[9]);
     const std::optional<Tensor> bias = optional_tensor(args[6]), offsets = optional_tensor(args[8]);
     if (PyErr_Occurred()) return nullptr;

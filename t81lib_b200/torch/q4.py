@@ -72,6 +72,7 @@ class Q4Tensor:
             raise ValueError("Q4Tensor products expect 2D activations")
         if input.shape[1] != self.shape[1]:
             raise ValueError("rhs dimension does not match the weight's width")
+        _check_type(input)
         if torch.is_grad_enabled() and (input.requires_grad or (bias is not None and bias.requires_grad)):
             return _Q4LinearFunction.apply(self, input, bias, out_dtype)
         product = self._native_product()
@@ -86,6 +87,7 @@ class Q4Tensor:
             raise ValueError("matmul_sorted takes an (experts, rows, cols) stack")
         if rows.ndim != 2 or rows.shape[1] != self.shape[2]:
             raise ValueError("rows do not match the weights' width")
+        _check_type(rows)
         if offsets.numel() != self.shape[0] + 1:
             raise ValueError("offsets must have one entry more than there are experts")
         if torch.is_grad_enabled() and (rows.requires_grad or (bias is not None and bias.requires_grad)):
@@ -94,14 +96,14 @@ class Q4Tensor:
         return ops.experts_q4(self.codes, self.scales, self.shape[1], rows, self.shape[2], self.group, offsets, bias, out_dtype)
 
 
+def _check_type(x: torch.Tensor) -> None:
+    if x.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise ValueError(f"x must be float32, bfloat16 or float16, got {x.dtype}")
+
+
 def _operand(x: torch.Tensor, device: torch.device) -> torch.Tensor:
-    """Activations as the kernels take them: on the weight's device, a type that they read, unit column stride."""
-    from . import _to_device_float
-    x = _to_device_float(x.as_subclass(torch.Tensor))
-    if x.device != device:
-        x = x.to(device)
-    if x.is_neg():
-        x = x.resolve_neg()
+    """Activations as the kernels take them: on the weight's device, unit column stride."""
+    x = x.detach().as_subclass(torch.Tensor).to(device).resolve_neg()
     return x if x.numel() == 0 or ((x.shape[1] == 1 or x.stride(1) == 1) and (x.shape[0] == 1 or x.stride(0) >= x.shape[1])) else x.contiguous()
 
 

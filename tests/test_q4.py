@@ -50,6 +50,9 @@ def test_refusals_need_no_device(lib_built):
         q.matmul_input(torch.zeros(64))
     with pytest.raises(ValueError, match="width"):
         q.matmul_input(torch.zeros(2, 63))
+    for bad in (torch.float64, torch.int32):
+        with pytest.raises(ValueError, match="float32, bfloat16 or float16"):
+            q.matmul_input(torch.zeros(2, 64, dtype=bad))
     with pytest.raises(ValueError, match="stack"):
         q.matmul_sorted(torch.zeros(2, 64), torch.zeros(2, dtype=torch.int32))
 
@@ -236,6 +239,9 @@ def test_strided_and_unaligned_activations(dev, tokens):
                 _check(q.matmul_input(x, b), x, q, b)  # nothing beside the rows is used
             x = torch.randn(cols, tokens, generator=gen, device=dev).to(dtype).t()  # columns apart
             _check(q.matmul_input(x, b), x, q, b)
+            x = torch._neg_view(torch.randn(tokens, cols, generator=gen, device=dev).to(dtype))
+            _check(q.matmul_input(x, b), x, q, b)
+            assert torch.equal(ops.linear_q4(q.codes, q.scales, 200, x, cols, 64), ops.linear_q4(q.codes, q.scales, 200, x.resolve_neg(), cols, 64))
             x = torch.randn(1, cols, generator=gen, device=dev).to(dtype).expand(tokens, cols)  # one row, many times
             _check(q.matmul_input(x, b), x, q, b)
             assert ops.linear_q4(q.codes, q.scales, 200, x.contiguous(), cols, 64).shape == (tokens, 200)
