@@ -219,7 +219,7 @@ T81B200_API int t81b200_elementwise_auto(int op, const float *a, const float *b,
  * epilogue, converter), 5..6 = inside the streaming kernel (producer, consumer), 7 = a wait
  * on the exchange flags of a sharded call, 8 = the streaming kernel found dynamic shared memory
  * starting above the address its tables were laid out for, 9..10 = a wait inside the streaming quantise + pack
- * kernel (producer, consumer); that launch's output is invalid.  The kernels never spin forever:
+ * kernel (producer, consumer); the 4-bit kernels use 1..4 and 6 in the same sense; that launch's output is invalid.  The kernels never spin forever:
  * every wait has an iteration limit after which it records the code, releases its
  * tensor memory and returns.  Reading the word synchronises the device; `reset`
  * non-zero clears it.  No counterpart in the reference (its CUDA path has no

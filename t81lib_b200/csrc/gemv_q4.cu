@@ -400,7 +400,7 @@ int product_q4(const char *name, const uint8_t *codes, const void *scales, const
     if (M < 0 || N < 0 || K < 0 || ldb < K || ldc < M || n_experts < 0) return fail(T81B200_EINVAL, "%s: bad dimensions", name);
     if (!q4_group_ok(group)) return fail(T81B200_EINVAL, "%s: groups of 32, 64 or 128 columns, not %d", name, group);
     if (dtype_size(b_dtype) == 0 || b_dtype < 0 || b_dtype > T81B200_F16 || c_dtype < 0 || c_dtype > T81B200_F16) return fail(T81B200_EINVAL, "%s: unknown dtype", name);
-    if (M >= (1ll << 31) || N >= (1ll << 31) || K >= (1ll << 31) || n_experts > kMostExperts || q4_row_tiles(M) * (n_experts > 0 ? n_experts : 1) >= (1ll << 31))
+    if (M >= (1ll << 31) - 4096 || N >= (1ll << 31) - 4096 || K >= (1ll << 31) - 4096 || n_experts > kMostExperts || q4_row_tiles(M) * (n_experts > 0 ? n_experts : 1) >= (1ll << 31))
         return fail(T81B200_ELIMIT, "%s: dimension too large (at most %d experts)", name, kMostExperts);
     if (int rc = check_device()) return rc;
     if (M == 0 || N == 0) return T81B200_OK;

@@ -60,9 +60,7 @@ class _Q4Module(nn.Module):
         return self
 
     def __getstate__(self):
-        state = super().__getstate__() if hasattr(nn.Module, "__getstate__") else dict(self.__dict__)
-        state["_q4"] = {}  # native calls do not travel
-        return state
+        return {**self.__dict__, "_q4": {}}  # native calls do not travel
 
 
 class Q4Linear(_Q4Module):
