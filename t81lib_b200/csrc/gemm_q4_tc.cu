@@ -620,7 +620,7 @@ double gemm_q4_tc_estimate_us(int64_t M, int64_t N, int64_t K, int planes, int n
     return 5.0 + 1e-3 * ceil(tiles / fit) * (2.0 * (double)((K + CHUNK - 1) / CHUNK) * step_cost(n, planes) + 700.0);
 }
 
-// x: 16-bit rows on 16-byte boundaries, K columns of them, N rows; with three planes three times N, and C is float32.  Arguments are checked by
+// x: 16-bit rows on 16-byte boundaries, K columns of them, N rows; with three planes three times N.  Arguments are checked by
 // the caller.
 int gemm_q4_tc_launch(const uint8_t *codes, const void *scales, const float *bias, void *C, int64_t M, const void *x, bool f16, int planes, int64_t ldx, int c_dtype, int64_t ldc, int64_t N,
                       int64_t K, int group, const int32_t *offsets, int n_experts, cudaStream_t st) {
@@ -685,12 +685,15 @@ int gemm_q4_tc_launch(const uint8_t *codes, const void *scales, const float *bia
     using One = std::integral_constant<int, 1>;
     auto by_experts = [&](auto t, auto pl, auto g, auto ct) { return offsets ? go(t, pl, g, ct, std::true_type{}) : go(t, pl, g, ct, std::false_type{}); };
     auto by_out = [&](auto t, auto g) {
-        if constexpr (std::is_same<decltype(t), __nv_bfloat16>::value)
-            if (planes == 3) return by_experts(t, std::integral_constant<int, 3>{}, g, float{});
+        auto by_planes = [&](auto ct) {
+            if constexpr (std::is_same<decltype(t), __nv_bfloat16>::value)
+                if (planes == 3) return by_experts(t, std::integral_constant<int, 3>{}, g, ct);
+            return by_experts(t, One{}, g, ct);
+        };
         switch (c_dtype) {
-            case T81B200_F32: return by_experts(t, One{}, g, float{});
-            case T81B200_BF16: return by_experts(t, One{}, g, __nv_bfloat16{});
-            default: return by_experts(t, One{}, g, __half{});
+            case T81B200_F32: return by_planes(float{});
+            case T81B200_BF16: return by_planes(__nv_bfloat16{});
+            default: return by_planes(__half{});
         }
     };
     auto by_group = [&](auto t) {

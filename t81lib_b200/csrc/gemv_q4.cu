@@ -426,7 +426,7 @@ int product_q4(const char *name, const uint8_t *codes, const void *scales, const
         p.plane_elems = N * p.ldx;
     }
     const int planes = b_dtype == T81B200_F32 ? 3 : 1;
-    if (K > 0 && (planes == 1 || (c_dtype == T81B200_F32 && 3 * N < (1ll << 31))) && tiles_are_faster(M, N, K, planes, offsets ? n_experts : 0))
+    if (K > 0 && (planes == 1 || 3 * N < (1ll << 31)) && tiles_are_faster(M, N, K, planes, offsets ? n_experts : 0))
         return gemm_q4_tc_launch(codes, scales, bias, C, M, p.x, b_dtype == T81B200_F16, planes, p.ldx, c_dtype, ldc, N, K, group, offsets, n_experts, st);
     if (b_dtype == T81B200_F32) return launch_shape<__nv_bfloat16, 3>(p, group, st);
     return b_dtype == T81B200_BF16 ? launch_shape<__nv_bfloat16, 1>(p, group, st) : launch_shape<__half, 1>(p, group, st);

@@ -208,6 +208,45 @@ def test_float32_sums_of_long_rows(dev, rows, cols, tokens):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,cols,tokens", [(512, 512, 300), (1000, 4100, 70), (33, 130, 9), (300, 6144, 200)])
+def test_float32_rows_with_16_bit_results(dev, rows, cols, tokens):
+    gen = torch.Generator(device="cuda").manual_seed(rows + tokens)
+    for out_dtype in (torch.bfloat16, torch.float16):
+        q, x, b = _case(gen, dev, rows, cols, tokens, torch.float32, 64, True)
+        y = q.matmul_input(x, b, out_dtype=out_dtype)
+        assert y.dtype == out_dtype
+        _check(y, x, q, b)
+        assert torch.equal(y, q.matmul_input(x, b).to(out_dtype))  # the same sums, rounded once
+
+
+@pytest.mark.gpu
+def test_more_elements_than_31_bits_count(dev):
+    """Weights, results and activations of more than 2^31 elements each, at their far ends."""
+    from t81lib_b200 import torch as t81_torch
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    rows, cols = 66001, 32800
+    w = torch.empty(rows, cols, dtype=torch.bfloat16, device=dev).normal_(generator=gen)
+    q = t81_torch.Q4Tensor.from_float(w, group=64)
+    last = t81_torch.Q4Tensor.from_float(w[-17:].contiguous(), group=64)  # 66001 = 16 * 4125 + 1: row tiles begin alike
+    del w
+    for tokens in (3, 40):
+        x = torch.randn(tokens, cols, generator=gen, device=dev).to(torch.bfloat16)
+        y = q.matmul_input(x, out_dtype=torch.float32)
+        _check(y[:, -17:], x, last, None)
+    del q, y
+    q = t81_torch.Q4Tensor.from_float(torch.randn(1003, 64, generator=gen, device=dev), group=64)
+    x = torch.randn(2150000, 64, generator=gen, device=dev).to(torch.bfloat16)
+    y = q.matmul_input(x)
+    _check(y[-300:], x[-300:], q, None)
+    _check(y[1000000:1000300], x[1000000:1000300], q, None)
+    del y
+    wide = torch.zeros(33, 1 << 26, dtype=torch.bfloat16, device=dev)  # rows 2^26 elements apart
+    wide[:, :64] = x[:33]
+    for few in (5, 33):
+        _check(q.matmul_input(wide[-few:, :64]), x[33 - few:33], q, None)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("tokens", [1, 8, 20, 200])
 def test_whole_numbers_come_back_whole(dev, dtype, tokens):

@@ -263,3 +263,32 @@ def test_saved_tensors_that_come_back_otherwise_and_batched_gradients(dev):
             y = r.combine(r.gather(x), w)
         with pytest.raises(ValueError):
             torch.autograd.grad(y, [x, w], v[0])
+
+
+def test_more_elements_than_31_bits_count(dev):
+    from t81lib_b200 import torch as t81_torch
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    tokens, top, width = 70000, 4, 8192  # 2.3e9 elements in the sorted rows
+    ids = torch.randint(0, 9, (tokens, top), generator=gen, device=dev)  # expert 8 takes no part
+    routing = t81_torch.route(ids, 8)
+    x = torch.randn(tokens, width, generator=gen, device=dev).to(torch.bfloat16)
+    rows = routing.gather(x)
+    kept = int(routing.offsets[-1])
+    some = torch.arange(kept - 100, kept, device=dev)
+    assert torch.equal(rows[kept - 100:kept], x[routing.order[some].long() // top]) and bool((rows[-100:] == 0).all())
+    weights = torch.rand(tokens, top, generator=gen, device=dev)
+    at = torch.arange(tokens - 64, tokens, device=dev)
+    share = torch.where(routing.position[at] >= 0, weights[at], torch.zeros_like(weights[at])).double().sum(1, keepdim=True)
+    y = routing.combine(rows, weights)
+    want = share * x[at].double()  # four roundings of fp32 and one of bf16
+    assert bool(((y[at].double() - want).abs() <= want.abs() * (2.0 ** -8 + 2.0 ** -20)).all())
+    rows.requires_grad_(True)
+    weights.requires_grad_(True)
+    g = torch.randn(tokens, width, generator=gen, device=dev).to(torch.bfloat16)
+    grad_rows, grad_weights = torch.autograd.grad(routing.combine(rows, weights), (rows, weights), g)
+    pair = routing.order[some].long()
+    want = weights.detach().flatten()[pair].double().unsqueeze(1) * g[pair // top].double()
+    assert bool(((grad_rows[kept - 100:kept].double() - want).abs() <= want.abs() * (2.0 ** -8 + 2.0 ** -20)).all()) and bool((grad_rows[-100:] == 0).all())
+    dots = (g[at].double() * x[at].double()).sum(1, keepdim=True) * (routing.position[at] >= 0)
+    magnitude = (g[at].double() * x[at].double()).abs().sum(1, keepdim=True)
+    assert bool(((grad_weights[at].double() - dots).abs() <= magnitude * (width / 32 + 6) * 2.0 ** -24).all())
