@@ -110,8 +110,8 @@ def _four_bit_modules(model: nn.Module, patterns: Sequence[str]) -> "list[str]":
     """The modules that the names mean, checked before any is replaced."""
     if isinstance(patterns, str):
         raise TypeError("four_bit takes a sequence of module names")
-    found = []
-    for name, module in model.named_modules():
+    found, seen, matched = [], set(), set()
+    for name, module in model.named_modules(remove_duplicate=False):
         if not name or not _named(name, patterns):
             continue
         if isinstance(module, TernaryLinear) and getattr(module, "_t81_float_released", False):
@@ -122,24 +122,29 @@ def _four_bit_modules(model: nn.Module, patterns: Sequence[str]) -> "list[str]":
                 raise ValueError(f"four_bit: the weights of {name} must be on a CUDA device")
             if any(w.numel() == 0 for w in weights):
                 raise ValueError(f"four_bit: {name} has no weights")
-            found.append(name)
+            matched.add(name)
+            if id(module) not in seen:  # one module may have several names
+                seen.add(id(module))
+                found.append(name)
     for pattern in patterns:
-        if not any(fnmatchcase(name, pattern) for name in found):
+        if not any(fnmatchcase(name, pattern) for name in matched):
             raise ValueError(f"four_bit: no nn.Linear and no stacked experts are named {pattern!r}")
     return found
 
 
 def _to_four_bit(model: nn.Module, names: Sequence[str], group: int, keep_biases_bf16: bool, stats: ConversionStats) -> None:
     for name in names:
-        parent_name, _, leaf = name.rpartition(".")
-        module, parent = model.get_submodule(name), model.get_submodule(parent_name) if parent_name else model
+        module = model.get_submodule(name)
         if isinstance(module, nn.Linear):
             new = Q4Linear.from_linear(module, group)
             if not keep_biases_bf16 and new.bias is not None and new.bias.dtype == torch.bfloat16:
                 new.bias = nn.Parameter(new.bias.detach().to(torch.float32), requires_grad=new.bias.requires_grad)
         else:
             new = Q4Experts.from_float(module.gate_up_proj, module.down_proj, module.act_fn, group).train(module.training)
-        setattr(parent, leaf, new)
+        for parent in list(model.modules()):  # wherever it is registered
+            for leaf, child in list(parent._modules.items()):
+                if child is module:
+                    setattr(parent, leaf, new)
         stats.four_bit += 1
         stats.four_bit_bytes += sum(b.numel() * b.element_size() for b in new.buffers())
 

@@ -177,3 +177,26 @@ def test_converted_model_runs_and_decodes_from_a_graph(dev, tmp_path):
         x.normal_()
         graph.replay()
         assert torch.equal(y, model(x))
+
+
+@pytest.mark.gpu
+def test_a_module_of_two_names_is_replaced_under_both(dev):
+    from t81lib_b200 import convert
+    from t81lib_b200.nn import Q4Linear
+    for pattern in ("first", "second"):
+        model = nn.Module()
+        model.first = model.second = nn.Linear(64, 48).to(dev)
+        stats = convert.convert_module(model, verbose=False, four_bit=[pattern])
+        assert isinstance(model.first, Q4Linear) and model.second is model.first and stats.four_bit == 1 and stats.replaced == 0
+
+
+@pytest.mark.gpu
+def test_pickled_layers(dev):
+    import pickle
+    from t81lib_b200.nn import Q4Linear
+    layer = Q4Linear.from_linear(nn.Linear(64, 48).to(dev)).eval()
+    x = torch.randn(3, 64, device=dev)
+    with torch.no_grad():
+        y = layer(x)
+        held = layer.weight
+        assert torch.equal(pickle.loads(pickle.dumps(layer))(x), y) and layer.weight is held
