@@ -3,7 +3,7 @@
 // Quantise: m = the group's value of largest magnitude (the first of equals), scale s = m / -8 rounded to five significant bits, code =
 // the whole number nearest to w / s, ties to even, held in -8 .. 7.  Eight steps reach from 0 to the largest value and seven the
 // other way.  Five bits for the scale make code * s a bf16 number, and cost little: N(0, 1) weights in groups of 128 come back with
-// a mean square error 0.3 % above that of an unrounded scale.
+// a mean square error 0.15 % above that of an unrounded scale (0.6 % in groups of 32).
 // Bound by memory: a weight is read once, half a byte is written.  A warp holds 16 rows x 128 columns in registers, a lane eight columns
 // of two rows at a time as the format has them: 64 (16-bit) or 128 bytes of a row side by side per load.
 #include "common.cuh"
