@@ -370,6 +370,32 @@ def test_experts(dev, counts, behind, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("experts,most,rows,cols", [(100, 600, 300, 512), (33, 2000, 520, 256), (1024, 90, 264, 192), (7, 3000, 2000, 320), (64, 40, 1400, 1024)])
+def test_experts_of_many_sizes(dev, experts, most, rows, cols):
+    """Tiles of every width, in more rounds than one, experts without rows among them."""
+    from t81lib_b200 import torch as t81_torch
+    gen = torch.Generator(device="cuda").manual_seed(experts)
+    counts = (torch.rand(experts, generator=gen, device=dev) * most).int()
+    counts[torch.rand(experts, generator=gen, device=dev) < 0.2] = 0
+    counts[experts // 2] = most
+    offsets = torch.cat([torch.zeros(1, dtype=torch.int32, device=dev), counts.cumsum(0).int()])
+    total = int(offsets[-1])
+    q = t81_torch.Q4Tensor.from_float(torch.randn(experts, rows, cols, generator=gen, device=dev) * 0.02, group=64)
+    bias = torch.randn(experts, rows, generator=gen, device=dev) * 0.1
+    values = q.dequantize().double()
+    for dtype in (torch.bfloat16, torch.float16, torch.float32):
+        x = torch.randn(total + 5, cols, generator=gen, device=dev).to(dtype)
+        y = q.matmul_sorted(x, offsets, bias)
+        assert bool((y[total:] == 0).all())
+        at = offsets.tolist()
+        for e in range(experts):
+            lo, hi = at[e], at[e + 1]
+            want, magnitude = ref.product(x[lo:hi], values[e], bias[e])
+            off = (y[lo:hi].double() - want).abs()
+            assert bool((off <= ref.tolerance(magnitude + bias[e].double().abs(), want, cols, dtype)).all()), e
+
+
+@pytest.mark.gpu
 def test_experts_refusals_and_bad_offsets(dev):
     from t81lib_b200 import torch as t81_torch
     q = t81_torch.Q4Tensor.from_float(torch.randn(3, 32, 64, device=dev), group=32)
