@@ -202,7 +202,7 @@ gemv_q4_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_const
     if (p.units > 0)
         for (int i = 0; i < S::kCount; ++i) issue();
     const Q4Decode<T> decode;
-    const uint32_t nothing = opaque(0u);
+    const uint32_t zero = unknown_zero();
     Ring at;
     bool ok = true, buffer = false;
     for (; item < items; item += (int)gridDim.x) {
@@ -280,7 +280,7 @@ gemv_q4_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_const
             uint32_t used = 0;
 #pragma unroll
             for (int r = 0; r < RT; ++r) used |= __float_as_uint(sum[r][0][0][0]);
-            if (!__any_sync(0xffffffffu, (used & nothing) != 0u)) issue();
+            if (all_loaded(used, zero)) issue();
             at.advance(S::kCount);
 #pragma unroll
             for (int n = 0; n < NT; ++n) src_x[n] += p.k_warps * (W * 128);

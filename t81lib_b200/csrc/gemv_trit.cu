@@ -493,7 +493,7 @@ gemv_trit_tma_kernel(const __grid_constant__ CUtensorMap map_w, const GemvTmaPar
         int tok_off[TOKB];
 #pragma unroll
         for (int b = 0; b < TOKB; ++b) tok_off[b] = (8 * b + g < p.ntok ? 8 * b + g : 0) * tok_stride + t * 24;
-        const uint32_t lane_off = (uint32_t)((rw * 16 + g) * 64 + t * 16);
+        const uint32_t lane_off = (uint32_t)((rw * 16 + g) * 64 + t * 16), zero = unknown_zero();
         bool ok = true;
         for (int c = kw; c < chunks_cta; c += k_warps) {
             const int st = c % tp.stages;
@@ -503,8 +503,8 @@ gemv_trit_tma_kernel(const __grid_constant__ CUtensorMap map_w, const GemvTmaPar
             const uint8_t *tile = smem_bytes_tma + tp.ring_offset + st * tp.stage_bytes + lane_off;
             const uint4 la = *reinterpret_cast<const uint4 *>(tile);
             const uint4 lb = *reinterpret_cast<const uint4 *>(tile + 8 * 64);
-            __syncwarp();
-            if (lane == 0) mbar_arrive(empty_bar(st));  // the limbs are in registers: the slot can be refilled
+            // the limbs have to be in registers before the slot is refilled: an arrival does not wait for loads that are on their way
+            if (all_loaded(la.x | lb.x, zero) && lane == 0) mbar_arrive(empty_bar(st));
             // activations of this chunk first (their latency hides behind the first decode), then,
             // word by word: decode 4 + 4 trytes, issue the 3 MMAs that consume them.
             uint4 xr[TOKB][PLANES][6];

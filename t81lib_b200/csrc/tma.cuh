@@ -38,6 +38,16 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
     return false;
 }
 
+// Whether the whole warp has in registers what `used` was made of, loads from a ring's slot: always true, but only once they have come.  An
+// arrival that hands the slot back does not wait for loads that are still on their way, and the next copy may overwrite what they read.
+// `zero`: unknown_zero(), so that the vote is not left out.
+__device__ __forceinline__ uint32_t unknown_zero() {
+    uint32_t r;
+    asm volatile("mov.b32 %0, 0;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ bool all_loaded(uint32_t used, uint32_t zero) { return __all_sync(0xffffffffu, (used & zero) == 0u); }
+
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t bar) {
     asm volatile(
         "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
