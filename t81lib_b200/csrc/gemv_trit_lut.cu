@@ -627,7 +627,7 @@ gemv_trit_lut_kernel(const __grid_constant__ CUtensorMap map0, const __grid_cons
                     wd[4 * j] = q.x; wd[4 * j + 1] = q.y; wd[4 * j + 2] = q.z; wd[4 * j + 3] = q.w;
                 }
                 // The codes have to be in registers before the slot is refilled: an arrival does not wait for loads that are on their way.  (Behind the
-                // loads below the vote takes registers that are not there: 16384 x 3072, 16 tokens 9.4 and 12.2 us.)
+                // loads below the vote takes registers that are not there: 14336 x 4096, 4 tokens of float32 10.5 and 11.3 us.)
                 if (all_loaded(wd[0] | wd[4] | wd[8], zero) && lane == 0) mbar_arrive(empty_bar(st));
                 uint4 xr[TOKB][PLANES][6];
 #pragma unroll
