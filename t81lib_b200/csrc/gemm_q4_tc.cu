@@ -10,9 +10,10 @@
 //
 // Weights: 128 columns (a chunk) of 128 rows are 8 KB of codes and up to 1 KB of scales, one TMA load each; a converter warp per 16 rows
 // turns them into operands of 128-byte rows.  A pair of codes is a shift, an AND-OR and one packed FMA, v * s - 24 s on v = 16 + code + 8, which
-// is exact: a code times its scale is a bf16 number.  Beside fp16 activations the scales of a row are first divided by the power of
-// two in the row's largest, which the result is multiplied by: fp16 holds all of a row's weights then but those 2^-20 below its
-// largest, which lose places that the sums do not have.
+// is exact: a code times its scale is a bf16 number.  Beside fp16 activations the scales of a row are first brought to 2^10 .. 2^11 at
+// the largest by a power of two, which the result is divided by: fp16 holds all of a row's weights then whose scale is no less than 2^-30 of that.
+// Where a converter meets a smaller scale, which counts as soon as the activations beside the large ones are small, the CTA
+// goes over its tiles once more at its end and writes the results of such rows from sums in fp32 registers (mend_rows).
 //
 // float32 activations come as three bf16 planes (all 24 bits, stage_planes), each a product of its own with the same expanded weights.  The tensor
 // core cuts an accumulator off at every 16 columns: 2.4e-7 of the result after 1024 columns, 5.6e-7 after 2048, 1.4e-6 after 4096, 7e-6
@@ -65,6 +66,10 @@ struct Q4TcParams {
     int M, N;                   // output features (of an expert), rows of x
     int n_experts, row_tiles;   // 16-row tiles of an expert
     int groups;
+    const uint8_t *codes;       // and x, for rows that fp16 does not hold
+    const void *x;
+    int64_t ldx;
+    int K, group;
     int m_tiles, n_tiles;       // 256-row pair tiles; tiles of bn rows of x (one matrix)
     int bn;                     // most rows of x a tile, a multiple of 32
     int n_atoms, n_chunks;
@@ -159,10 +164,63 @@ __device__ __forceinline__ void load_sums(const Q4TcParams &p, uint32_t taddr, i
         }
 }
 
-// The power of two in a row's largest scale (1 for a row of zeros), as the exponent bits of a float.
+// The power of two in a row's largest scale (1 for a row of zeros), as the exponent bits of a float; 2^-103 at least, the format's smallest.
 __device__ __forceinline__ uint32_t row_exponent(const __nv_bfloat16 *scales, int64_t tile, int groups, int r) {
     const uint32_t bits = (uint32_t)__ldg(reinterpret_cast<const unsigned short *>(scales) + (tile * (groups + 1) + groups) * 16 + 2 * (r & 7) + (r >> 3)) & 0x7F80u;
-    return bits ? bits << 16 : 0x3F800000u;
+    return bits ? max(bits << 16, 0x0C000000u) : 0x3F800000u;
+}
+
+// A row's scales beside fp16 activations are multiplied by 2^(kF16Up - e), 2^e being row_exponent: the largest weight is below 2^14 then, 24 scales below
+// 2^16.  A scale of five bits is held to the last place of every code times it down to 2^-20, which is kF16Span below 2^e.
+constexpr int kF16Up = 10, kF16Span = kF16Up + 20;
+
+// Whether a scale (bf16 bits without the sign) is too small for that beside a row's largest.
+__device__ __forceinline__ bool f16_loses(uint32_t scale, uint32_t exponent) { return scale != 0u && (int)scale < (int)(exponent >> 16) - (kF16Span << 7); }
+
+// Results of a tile's rows with such scales, from the codes, in fp32: a warp per row and four rows of x, a lane sixteen columns of one of eight 64-column
+// tiles at a time, the lanes' sums in a fixed order.  For the few rows that want it, if any: two to three orders slower than the tensor core.
+template <typename CT>
+__device__ __noinline__ void mend_rows(const Q4TcParams &p, int expert, int row0, int tok0, int end, int warp, int lane) {
+    const int64_t col_tiles = q4_col_tiles(p.K);
+    for (int r = warp; r < BM && row0 + r < p.M; r += NUM_THREADS / 32) {
+        const int row = row0 + r, g = row & 7, hi = (row >> 3) & 1, t = lane & 3;
+        const int64_t tile = (int64_t)expert * p.row_tiles + (row >> 4);
+        const unsigned short *scales = reinterpret_cast<const unsigned short *>(p.scales) + tile * (p.groups + 1) * 16 + 2 * g + hi;
+        const uint32_t exponent = row_exponent(p.scales, tile, p.groups, row & 15);
+        bool lost = false;
+        for (int u = lane; u < p.groups; u += 32) lost = lost || f16_loses(scales[(int64_t)u * 16] & 0x7FFFu, exponent);
+        if (!__any_sync(0xffffffffu, lost)) continue;
+        const float bias = p.bias ? p.bias[(int64_t)expert * p.M + row] : 0.0f;
+        for (int tok = tok0; tok < end; tok += 4) {
+            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int64_t c = lane >> 2; c < col_tiles; c += 8) {
+                const uint4 q = *reinterpret_cast<const uint4 *>(p.codes + (tile * col_tiles + c) * kQ4TileBytes + (4 * g + t) * 16);
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const int64_t col = 64 * c + 32 * half + 8 * t;
+                    if (col >= p.K) continue;  // (rows of x are whole pieces of eight)
+                    const float s = __uint_as_float((uint32_t)scales[col / p.group * 16] << 16);
+                    float w[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        w[i] = (float)((int)(((half ? (i < 4 ? q.z : q.w) : (i < 4 ? q.x : q.y)) >> (4 * (2 * ((i >> 1) & 1) + hi) + 16 * (i & 1))) & 15u) - 8) * s;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        if (tok + k >= end) break;
+                        const uint4 v = *reinterpret_cast<const uint4 *>(static_cast<const __half *>(p.x) + (int64_t)(tok + k) * p.ldx + col);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) sum[k] = fmaf(w[i], __half2float(reinterpret_cast<const __half *>(&v)[i]), sum[k]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+#pragma unroll
+                for (int d = 16; d > 0; d >>= 1) sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], d);
+                if (lane == k && tok + k < end) static_cast<CT *>(p.C)[(int64_t)(tok + k) * p.ldc + row] = from_float<CT>(sum[k] + bias);
+            }
+        }
+    }
 }
 
 template <typename T, int PLANES, int GROUP, typename CT, bool EXPERTS>
@@ -187,6 +245,7 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_co
     auto b_full = [&](int s) { return bars + 8u * (2 * A_STAGES + 2 * RAW_MAX + 4 + s); };
     auto b_empty = [&](int s) { return bars + 8u * (2 * A_STAGES + 2 * RAW_MAX + 4 + B_MAX + s); };
     const uint32_t tmem_slot = bars + 8u * (2 * A_STAGES + 2 * RAW_MAX + 4 + 2 * B_MAX);
+    volatile int *const losses = reinterpret_cast<volatile int *>(gen_base + (tmem_slot + 4u - base));  // fp16: a scale of this CTA's rows was too small
 
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
@@ -197,6 +256,7 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_co
         for (int s = 0; s < 2; ++s) { mbar_init(acc_full(s), 1); mbar_init(acc_empty(s), 8); }
         for (int s = 0; s < B_MAX; ++s) { mbar_init(b_full(s), 1); mbar_init(b_empty(s), 1); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        *losses = 0;
         prefetch_map(&map_codes);
         prefetch_map(&map_scales);
         prefetch_map(&map_x.m[0]);
@@ -233,7 +293,7 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_co
     // factor of the sums and bias of a feature
     auto factor_of = [&](const Tile &t, int r) {
         if (!F16 || t.row0 + r >= p.M) return 1.0f;
-        return __uint_as_float(row_exponent(p.scales, (int64_t)t.expert * p.row_tiles + ((t.row0 + r) >> 4), p.groups, r & 15));
+        return __uint_as_float(row_exponent(p.scales, (int64_t)t.expert * p.row_tiles + ((t.row0 + r) >> 4), p.groups, r & 15) - (kF16Up << 23));
     };
     auto bias_of = [&](const Tile &t, int r) { return p.bias && t.row0 + r < p.M ? __ldg(p.bias + (int64_t)t.expert * p.M + t.row0 + r) : 0.0f; };
 
@@ -395,6 +455,15 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_co
         if (group == 1) { a.advance(A_STAGES); raw.advance(p.raw_stages); }
         bool ok = true;
         float shrink[2] = {1.0f, 1.0f};
+        // the smallest scales of the lane's two rows in a tile, bf16 bits plus 0x7FFF as signed 16-bit numbers: zeros are the largest
+        constexpr uint32_t kNone = 0x7FFF7FFFu, kOne = 0x7F000000u + (kF16Up << 23);
+        uint32_t least = kNone;
+        auto look = [&]() {
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+                if (f16_loses((((least >> (16 * r)) & 0xFFFFu) - 0x7FFFu) & 0xFFFFu, kOne - __float_as_uint(shrink[r]))) *losses = 1;
+            least = kNone;
+        };
         // the chunks of this CTA's tiles; `c`: of the tile's, where its rows' powers of two matter
         const int span = c1 - c0;
         int c = group, i = cluster_id;
@@ -403,11 +472,12 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_co
             if constexpr (F16) {
                 for (; c >= span; c -= span, i += n_clusters) fresh = true;
                 if (fresh) {
+                    look();
                     const Tile t = tiles.tile(p, i, half);
                     const int64_t tile = (int64_t)t.expert * p.row_tiles + (t.row0 >> 4) + cw;
 #pragma unroll
                     for (int r = 0; r < 2; ++r)
-                        shrink[r] = t.row0 + cw * 16 < p.M ? __uint_as_float(0x7F000000u - row_exponent(p.scales, tile, p.groups, g + 8 * r)) : 1.0f;  // 2^-e
+                        shrink[r] = t.row0 + cw * 16 < p.M ? __uint_as_float(kOne - row_exponent(p.scales, tile, p.groups, g + 8 * r)) : 1.0f;  // 2^(kF16Up - e)
                     fresh = false;
                 }
                 c += 2;
@@ -421,6 +491,9 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_co
             for (int k = 0; k < 2; ++k) q[k] = *reinterpret_cast<const uint4 *>(src + cw * 1024 + k * 512 + lane * 16);
 #pragma unroll
             for (int u = 0; u < PER; ++u) s[u] = *reinterpret_cast<const uint32_t *>(src + RAW_CODES + (cw * PER + u) * 32 + g * 4);
+            if constexpr (F16)
+#pragma unroll
+                for (int u = 0; u < PER; ++u) least = __vmins2(least, (s[u] & 0x7FFF7FFFu) + 0x7FFF7FFFu);
             // a row's scale twice in a word, and -24 times it
             uint32_t s2[2][PER], n2[2][PER];
 #pragma unroll
@@ -482,6 +555,7 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_co
             a.advance(A_STAGES);
             a.advance(A_STAGES);
         }
+        if constexpr (F16) look();
         if (!ok) give_up(&g_q4_status, STATUS_CONVERTER);
     }
     __syncwarp();
@@ -528,6 +602,12 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_co
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         tmem_free_pair(tmem_base);
     }
+    if constexpr (F16)
+        if (*losses)  // the cluster's results are written: those of rows that fp16 does not hold are written again
+            for (int i = cluster_id; i < total_tiles; i += n_clusters) {
+                const Tile t = tiles.tile(p, i, half);
+                mend_rows<CT>(p, t.expert, t.row0, t.tok, t.end, warp, lane);
+            }
 }
 
 // Time of a 64-deep step at n columns, in ns: 18944 rows of 8192 columns (4096 for wide tiles of three planes), one tile a pair, 34 to 256 rows of
@@ -630,6 +710,7 @@ int gemm_q4_tc_launch(const uint8_t *codes, const void *scales, const float *bia
     p.scales = static_cast<const __nv_bfloat16 *>(scales); p.bias = bias; p.C = C; p.offsets = offsets; p.ldc = ldc;
     p.M = (int)M; p.N = (int)N; p.n_experts = experts;
     p.row_tiles = (int)q4_row_tiles(M); p.groups = (int)q4_groups(K, group);
+    p.codes = codes; p.x = x; p.ldx = ldx; p.K = (int)K; p.group = group;
     p.m_tiles = (int)((M + 255) / 256);
     p.n_atoms = (int)((K + BK - 1) / BK); p.n_chunks = (int)((K + CHUNK - 1) / CHUNK);
     p.splits = 1;

@@ -1,0 +1,95 @@
+"""4-bit weights where types end: scales of one row far apart, activations beside the largest numbers."""
+
+import pytest
+import torch
+
+import _q4_reference as ref
+
+
+@pytest.fixture(scope="module")
+def dev(lib_built):
+    from t81lib_b200 import _capi
+    assert _capi.device_available(), _capi.last_error()
+    yield torch.device("cuda", 0)
+    assert _capi.kernel_status(reset=True) == 0  # no bounded wait of a kernel ran out
+
+
+def _check(y, x, values, bias=None):
+    want, magnitude = ref.product(x, values, bias)
+    if bias is not None:
+        magnitude = magnitude + bias.double().abs()
+    off = (y.double() - want).abs()
+    assert y.shape == want.shape and bool((off <= ref.tolerance(magnitude, want, x.shape[1], y.dtype)).all()), float((off / magnitude).nan_to_num().max())
+
+
+def _far_apart(gen, dev, rows, cols, group, plain):
+    """Weights of which every row but each `plain`-th has groups 2^-16 to 2^-60 below its largest, and activations that are 0 beside the large groups."""
+    w = torch.randn(rows, cols, generator=gen, device=dev)
+    factor = torch.ones(rows, (cols + group - 1) // group, device=dev)
+    for i, e in enumerate((-16, -20, -21, -25, -29, -30, -31, -35, -41, -60)):
+        if i + 1 < factor.shape[1]:
+            factor[:, i + 1] = 2.0 ** e
+    factor[::plain] = 1.0
+    factor[1::plain, 0] = 0.0                     # rows without the large group: the next one is the largest
+    return w * factor.repeat_interleave(group, 1)[:, :cols]
+
+
+def _quiet(x, group):
+    """Activations that meet one small group each, by their row."""
+    groups = (x.shape[1] + group - 1) // group
+    at = torch.arange(x.shape[0], device=x.device) % groups
+    return x * (torch.arange(x.shape[1], device=x.device) // group == at[:, None])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,cols,group,plain", [(2048, 4096, 64, 3), (2000, 4090, 128, 50), (520, 8192, 32, 2), (5000, 1032, 64, 40), (37, 14336, 128, 5)])
+def test_scales_of_a_row_far_apart(dev, rows, cols, group, plain):
+    """float16 holds 40 binades and a row's scales span more: the result does not depend on how many rows of x there are."""
+    from t81lib_b200 import torch as t81_torch
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    q = t81_torch.Q4Tensor.from_float(_far_apart(gen, dev, rows, cols, group, plain), group=group)
+    values = q.dequantize().double()
+    bias = torch.randn(rows, generator=gen, device=dev) * 2.0 ** -40
+    for tokens in (3, 130, 1200):
+        x = torch.randn(tokens, cols, generator=gen, device=dev).half()
+        for each, b in ((x, None), (_quiet(x, group), None), (_quiet(x, group), bias)):
+            _check(q.matmul_input(each, b, out_dtype=torch.float32), each, values, b)
+        y = q.matmul_input(_quiet(x, group))
+        assert y.dtype == torch.float16
+        _check(y, _quiet(x, group), values)
+
+
+@pytest.mark.gpu
+def test_infinite_activations_beside_small_scales(dev):
+    """An infinity beside a weight that float16 would hold as 0 is an infinity of the product's sign."""
+    from t81lib_b200 import torch as t81_torch
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    w = torch.randint(1, 8, (1024, 4096), generator=gen, device=dev).float()
+    w[:, ::64] = -8.0
+    w[:, 64:128] *= 2.0 ** -50
+    q = t81_torch.Q4Tensor.from_float(w, group=64)
+    for tokens in (2, 200):
+        x = torch.randn(tokens, 4096, generator=gen, device=dev).half()
+        x[0, 64], x[1, 70] = float("inf"), float("-inf")
+        y = q.matmul_input(x, out_dtype=torch.float32)
+        assert bool((y[:2] == -float("inf")).all()) and bool(torch.isfinite(y[2:]).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("counts,behind", [([300, 0, 40, 257, 1], 7), ([700] * 9, 0)])
+def test_experts_with_scales_far_apart(dev, counts, behind):
+    from t81lib_b200 import torch as t81_torch
+    gen = torch.Generator(device="cuda").manual_seed(len(counts))
+    rows, cols, group = 1500, 1024, 64
+    w = torch.stack([_far_apart(gen, dev, rows, cols, group, 2 + 20 * e) for e in range(len(counts))])
+    w[0] = torch.randn(rows, cols, generator=gen, device=dev)  # an expert without such rows
+    q = t81_torch.Q4Tensor.from_float(w, group=group)
+    offsets = torch.tensor([0] + torch.tensor(counts).cumsum(0).tolist(), dtype=torch.int32, device=dev)
+    total = sum(counts)
+    x = _quiet(torch.randn(total + behind, cols, generator=gen, device=dev).half(), group)
+    bias = torch.randn(len(counts), rows, generator=gen, device=dev) * 2.0 ** -30
+    y = q.matmul_sorted(x, offsets, bias, out_dtype=torch.float32)
+    values, at = q.dequantize().double(), offsets.tolist()
+    assert not y[total:].any()
+    for e in range(len(counts)):
+        _check(y[at[e]:at[e + 1]], x[at[e]:at[e + 1]], values[e], bias[e])
