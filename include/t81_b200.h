@@ -433,8 +433,8 @@ T81B200_API size_t t81b200_gemm_trit_workspace_bytes(int b_dtype, int layout, in
  *                  exact, sums the tensor cores' fp32 ones (plain fp32 ones where fp16 does not hold a row beside fp16 B, whose scales
  *                  span more than 2^30); fp32 B keeps all 24 bits.
  *   experts_q4:    the same with rows sorted by expert: row p is multiplied by matrix e, offsets[e] <= p < offsets[e + 1]; codes, scales
- *                  and bias (n_experts, M) one expert behind the other; offsets: n_experts + 1 rising numbers on the device,
- *                  from 0.  Rows at or past offsets[n_experts] become 0. */
+ *                  and bias (n_experts, M) one expert behind the other; offsets: n_experts + 1 rising numbers on the device.
+ *                  Rows ahead of offsets[0], and at or past offsets[n_experts], become 0. */
 T81B200_API int64_t t81b200_q4_bytes(int64_t rows, int64_t cols);
 T81B200_API int64_t t81b200_q4_scales(int64_t rows, int64_t cols, int group);
 T81B200_API int t81b200_quantize_q4(const void *w, int w_dtype, int64_t matrices, int64_t rows, int64_t cols, int64_t ld, int64_t matrix_stride, int group, uint8_t *codes,

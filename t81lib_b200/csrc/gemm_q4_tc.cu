@@ -280,13 +280,16 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_co
     const int segments = PLANES == 3 ? (c1 - c0 + p.seg_chunks - 1) / p.seg_chunks : 0;
 
     if constexpr (EXPERTS) {  // rows of no expert: a warp each
-        const int kept = tiles.list.first(p.n_experts);
-        for (int64_t row = (int64_t)kept + blockIdx.x * (NUM_THREADS / 32) + warp; row < p.N; row += (int64_t)gridDim.x * (NUM_THREADS / 32)) {
-            CT *dst = static_cast<CT *>(p.C) + row * p.ldc;
-            if (p.vec && p.M % 8 == 0)
-                for (int i = lane; i < p.M * (int)sizeof(CT) / 16; i += 32) reinterpret_cast<uint4 *>(dst)[i] = make_uint4(0u, 0u, 0u, 0u);
-            else
-                for (int i = lane; i < p.M; i += 32) dst[i] = from_float<CT>(0.0f);
+#pragma unroll 1
+        for (int side = 0; side < 2; ++side) {  // ahead of the first one's and behind the last one's
+            const int to = side ? p.N : tiles.list.first(0);
+            for (int64_t row = (int64_t)(side ? tiles.list.first(p.n_experts) : 0) + blockIdx.x * (NUM_THREADS / 32) + warp; row < to; row += (int64_t)gridDim.x * (NUM_THREADS / 32)) {
+                CT *dst = static_cast<CT *>(p.C) + row * p.ldc;
+                if (p.vec && p.M % 8 == 0)
+                    for (int i = lane; i < p.M / (16 / (int)sizeof(CT)); i += 32) reinterpret_cast<uint4 *>(dst)[i] = make_uint4(0u, 0u, 0u, 0u);
+                else
+                    for (int i = lane; i < p.M; i += 32) dst[i] = from_float<CT>(0.0f);
+            }
         }
         __syncwarp();
     }

@@ -12,8 +12,8 @@
 // float32 activations come as three bf16 planes (all 24 bits, stage_planes), each multiplied exactly; the first has sums of its own, since the
 // tensor core cuts small terms beside large ones off.
 //
-// The same kernel multiplies rows sorted by expert (`offsets`): blocks go through the experts that have rows; rows behind the last
-// expert's become zero.
+// The same kernel multiplies rows sorted by expert (`offsets`): blocks go through the experts that have rows; rows of none, ahead
+// of the first one's or behind the last one's, become zero.
 #include "common.cuh"
 #include "launch_order.cuh"
 #include "q4.cuh"
@@ -163,8 +163,11 @@ gemv_q4_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_const
         items = list.build(reinterpret_cast<int32_t *>(part + 2 * PART), p.offsets, p.n_experts, p.rows, TOK) * p.row_items;
         for (int e = threadIdx.x; e < p.n_experts; e += kThreads)
             for (int q = list.before(e); q < min(list.before(e + 1), kOwners); ++q) owner[q] = (int16_t)e;
-        for (int row = list.first(p.n_experts) + (int)blockIdx.x * kWarps + warp; row < p.rows; row += (int)gridDim.x * kWarps)  // rows of no expert: a warp each
-            for (int i = lane; i < p.M; i += 32) store(p.y, (int64_t)row * p.ldy + i, 0.0f, p.y_dtype);
+        const int ahead = list.first(0), taken = list.first(p.n_experts) - ahead;
+        for (int64_t at = (int64_t)blockIdx.x * kWarps + warp; at < (int64_t)p.rows - taken; at += (int64_t)gridDim.x * kWarps) {  // rows of no expert: a warp each
+            const int64_t row = at < ahead ? at : at + taken;
+            for (int i = lane; i < p.M; i += 32) store(p.y, row * p.ldy + i, 0.0f, p.y_dtype);
+        }
     }
     __syncthreads();
 

@@ -398,8 +398,8 @@ def linear_q4(codes: torch.Tensor, scales: torch.Tensor, M: int, x: torch.Tensor
 def experts_q4(codes: torch.Tensor, scales: torch.Tensor, M: int, x: torch.Tensor, K: int, group: int, offsets: torch.Tensor,
                bias: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """``linear_q4`` for rows sorted by expert: rows ``offsets[e]`` to ``offsets[e + 1] - 1`` are multiplied by matrix ``e`` of the stack
-    (and get row ``e`` of the bias, (experts, M)); rows from ``offsets[-1]`` on come out as 0.  ``offsets``: int32, on the device,
-    rising from 0, as ``sort_by_expert`` gives it."""
+    (and get row ``e`` of the bias, (experts, M)); rows ahead of ``offsets[0]`` and from ``offsets[-1]`` on come out as 0.
+    ``offsets``: int32, on the device, rising, as ``sort_by_expert`` gives it."""
     return _capi.native.linear_q4(codes, scales, M, K, group, x, bias, out_dtype, offsets, offsets.numel() - 1)
 
 

@@ -81,8 +81,8 @@ class Q4Tensor:
 
     def matmul_sorted(self, rows: torch.Tensor, offsets: torch.Tensor, bias: Optional[torch.Tensor] = None,
                       out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
-        """Rows sorted by expert (``Routing.gather``) times the matrix of the expert each belongs to; rows from ``offsets[-1]`` on come out
-        as 0.  ``bias``: (experts, rows of a matrix).  For inference: no gradient is recorded."""
+        """Rows sorted by expert (``Routing.gather``) times the matrix of the expert each belongs to; rows ahead of ``offsets[0]`` and from
+        ``offsets[-1]`` on come out as 0.  ``bias``: (experts, rows of a matrix).  For inference: no gradient is recorded."""
         if len(self.shape) != 3:
             raise ValueError("matmul_sorted takes an (experts, rows, cols) stack")
         if rows.ndim != 2 or rows.shape[1] != self.shape[2]:

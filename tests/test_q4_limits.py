@@ -93,3 +93,23 @@ def test_experts_with_scales_far_apart(dev, counts, behind):
     assert not y[total:].any()
     for e in range(len(counts)):
         _check(y[at[e]:at[e + 1]], x[at[e]:at[e + 1]], values[e], bias[e])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("offsets,total", [([4, 5, 5, 9], 10), ([300, 500, 700, 1100], 1200), ([7, 7, 7, 7], 7), ([2500, 2500, 2500, 2500], 2500), ([3, 900, 1000, 1500], 1500)])
+def test_rows_ahead_of_the_first_expert(dev, offsets, total, dtype):
+    """Slices of a sorted batch: rows that belong to an expert that is not there come out as 0, like the ones behind the last."""
+    from t81lib_b200 import torch as t81_torch
+    gen = torch.Generator(device="cuda").manual_seed(total)
+    for rows, cols in ((70, 200), (1000, 1024), (1001, 256)):
+        q = t81_torch.Q4Tensor.from_float(torch.randn(3, rows, cols, generator=gen, device=dev) * 0.02, group=64)
+        x = torch.randn(total, cols, generator=gen, device=dev).to(dtype)
+        x[:offsets[0]], x[offsets[-1]:] = float("nan"), float("nan")
+        torch.full((total, rows), float("nan"), device=dev, dtype=dtype)  # what the result's memory may hold
+        y = q.matmul_sorted(x, torch.tensor(offsets, dtype=torch.int32, device=dev))
+        assert not y[:offsets[0]].any() and not y[offsets[-1]:].any()
+        values = q.dequantize().double()
+        for e in range(3):
+            lo, hi = offsets[e], offsets[e + 1]
+            _check(y[lo:hi], x[lo:hi], values[e])
