@@ -128,6 +128,9 @@ struct ProductObject {
 
 bool plain_tensor(PyObject *o) { return THPVariable_CheckExact(o); }
 
+// Whether a forward-mode derivative rides on the tensor (torch.autograd.forward_ad), which requires_grad does not tell.
+bool has_tangent(const Tensor &t) { return t._fw_grad(0).defined(); }
+
 PyObject *product_call(PyObject *self, PyObject *const *args, size_t nargsf, PyObject *kwnames) {
     HANDLE_TH_ERRORS
     auto *p = reinterpret_cast<ProductObject *>(self);
@@ -604,12 +607,12 @@ PyObject *q4_product_call(PyObject *self, PyObject *const *args, size_t nargsf, 
     Rows rows;
     if (x.device() != device || x.layout() != at::kStrided || x.is_neg() || !as_rows(x, p->k, rows)) Py_RETURN_NONE;
     const bool grad = at::GradMode::is_enabled();
-    if (grad && x.requires_grad()) Py_RETURN_NONE;
+    if ((grad && x.requires_grad()) || has_tangent(x)) Py_RETURN_NONE;
     const float *bias = nullptr;
     if (n > 1 && args[1] != Py_None) {
         if (!plain_tensor(args[1])) Py_RETURN_NONE;
         const Tensor &b = THPVariable_Unpack(args[1]);
-        if ((grad && b.requires_grad()) || !float_vector(b, device, p->rows)) Py_RETURN_NONE;
+        if ((grad && b.requires_grad()) || has_tangent(b) || !float_vector(b, device, p->rows)) Py_RETURN_NONE;
         bias = b.const_data_ptr<float>();
     }
     at::ScalarType out_type = x.scalar_type();
@@ -930,6 +933,15 @@ PyObject *combine_rows(PyObject *, PyObject *const *args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// has_tangent(*tensors): whether one of them (None counts as none) carries a forward-mode derivative.
+PyObject *any_tangent(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    for (Py_ssize_t i = 0; i < n; ++i)
+        if (args[i] != Py_None && has_tangent(tensor_of(args[i]))) Py_RETURN_TRUE;
+    Py_RETURN_FALSE;
+    END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef methods[] = {
     {"quantize_pack", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(quantize_pack)), METH_FASTCALL, nullptr},
     {"tensor_body", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(tensor_body)), METH_FASTCALL, nullptr},
@@ -939,6 +951,7 @@ PyMethodDef methods[] = {
     {"qat_linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(qat_linear)), METH_FASTCALL, nullptr},
     {"linear_t2", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(linear_t2)), METH_FASTCALL, nullptr},
     {"qat_weight_grad", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(qat_weight_grad)), METH_FASTCALL, nullptr},
+    {"has_tangent", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(any_tangent)), METH_FASTCALL, nullptr},
     {"quantize_q4", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(quantize_q4)), METH_FASTCALL, nullptr},
     {"dequantize_q4", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(dequantize_q4)), METH_FASTCALL, nullptr},
     {"q4_group_scales", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(q4_group_scales)), METH_FASTCALL, nullptr},

@@ -113,3 +113,32 @@ def test_rows_ahead_of_the_first_expert(dev, offsets, total, dtype):
         for e in range(3):
             lo, hi = offsets[e], offsets[e + 1]
             _check(y[lo:hi], x[lo:hi], values[e])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_is_refused(dev, grad):
+    """A tangent of the activations or the bias is not dropped without a word, whatever path a call takes."""
+    import torch.autograd.forward_ad as fwd
+    from t81lib_b200 import torch as t81_torch
+    from t81lib_b200.nn import Q4Experts, Q4Linear
+    layer = Q4Linear.from_linear(torch.nn.Linear(64, 48, bias=False, device=dev), group=32)
+    stack = t81_torch.Q4Tensor.from_float(torch.randn(2, 48, 64, device=dev), group=32)
+    block = Q4Experts.from_float(torch.randn(2, 64, 48, device=dev), torch.randn(2, 48, 32, device=dev), group=32)
+    offsets = torch.tensor([0, 1, 4], dtype=torch.int32, device=dev)
+    x, bias = torch.randn(4, 64, device=dev), torch.randn(48, device=dev)
+    ids, weights = torch.zeros(4, 1, dtype=torch.int64, device=dev), torch.ones(4, 1, device=dev)
+    with torch.set_grad_enabled(grad), fwd.dual_level():
+        dual, dual_bias = fwd.make_dual(x, torch.ones_like(x)), fwd.make_dual(bias, torch.ones_like(bias))
+        assert layer(x).shape == (4, 48) and layer.weight.matmul_input(x, bias).shape == (4, 48)
+        for call in (lambda: layer(dual), lambda: layer(dual.half()), lambda: layer.weight.matmul_input(dual), lambda: layer.weight.matmul_input(dual.t().contiguous().t()),
+                     lambda: layer.weight.matmul_input(x, dual_bias), lambda: layer.weight.matmul_input(dual.cpu()),
+                     lambda: stack.matmul_sorted(dual, offsets), lambda: stack.matmul_sorted(x, offsets, dual_bias.expand(2, 48)),
+                     lambda: layer(dual.requires_grad_(True) if grad else dual)):
+            with pytest.raises(NotImplementedError, match="forward|jvp"):
+                call()
+        with pytest.raises(RuntimeError, match="jvp"):
+            block(fwd.make_dual(torch.randn(4, 48, device=dev), torch.ones(4, 48, device=dev)), ids, weights)
+        with pytest.raises(RuntimeError, match="jvp"):
+            t81_torch.route(ids, 2).combine(x, fwd.make_dual(weights, torch.ones_like(weights)))
+        assert layer(x).shape == (4, 48)
