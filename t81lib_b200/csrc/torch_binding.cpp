@@ -145,12 +145,12 @@ PyObject *product_call(PyObject *self, PyObject *const *args, size_t nargsf, PyO
     Rows rows;
     if (x.device() != device || x.layout() != at::kStrided || !as_rows(x, p->k, rows)) Py_RETURN_NONE;
     const bool grad = at::GradMode::is_enabled();
-    if (grad && x.requires_grad()) Py_RETURN_NONE;
+    if ((grad && x.requires_grad()) || has_tangent(x)) Py_RETURN_NONE;
     const float *bias = nullptr;
     if (n > 1 && args[1] != Py_None) {
         if (!plain_tensor(args[1])) Py_RETURN_NONE;
         const Tensor &b = THPVariable_Unpack(args[1]);
-        if ((grad && b.requires_grad()) || !float_vector(b, device, p->rows)) Py_RETURN_NONE;
+        if ((grad && b.requires_grad()) || has_tangent(b) || !float_vector(b, device, p->rows)) Py_RETURN_NONE;
         bias = b.const_data_ptr<float>();
     }
     at::ScalarType out_type = x.scalar_type();

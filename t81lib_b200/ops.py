@@ -376,6 +376,12 @@ def qat_weight_grad(grad: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, s
     return _capi.native.qat_weight_grad(grad, x, weight, scale)
 
 
+def refuse_tangents(*tensors: Optional[torch.Tensor]) -> None:
+    """Forward-mode derivatives (torch.autograd.forward_ad) would be lost in a native call."""
+    if _capi.native.has_tangent(*tensors):
+        raise NotImplementedError("products from packed weights have no forward-mode derivatives")
+
+
 def quantize_q4(w: torch.Tensor, group: int = 128) -> Tuple[torch.Tensor, torch.Tensor]:
     """A (rows, cols) matrix or a (matrices, rows, cols) stack of them -> 4-bit codes and group scales in the products' order:
     ``(codes uint8, scales bfloat16)``, both flat.  ``group``: 32, 64 or 128 columns that share a scale."""

@@ -199,6 +199,7 @@ class TernaryTensor(torch.Tensor):
             # inference fast path: no autograd node, no device shuffling — one kernel call
             if input.shape[1] != self._k_actual:
                 raise ValueError("rhs dimension does not match ternary weight width")
+            ops.refuse_tangents(input, bias)
             # the weight in the decode-stream layout (made once): a quarter fewer bytes to stream, and two instructions per pair
             # of trits to expand
             product = self._native_product() if DECODE_STREAM_LAYOUT and self._rows > 0 and self._k_actual > 0 else None

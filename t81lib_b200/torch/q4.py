@@ -79,7 +79,7 @@ class Q4Tensor:
         y = product(input, bias, out_dtype) if product is not None else None
         if y is not None:
             return y
-        refuse_tangents(input, bias)
+        ops.refuse_tangents(input, bias)
         return _multiply(self, input, bias, out_dtype)
 
     def matmul_sorted(self, rows: torch.Tensor, offsets: torch.Tensor, bias: Optional[torch.Tensor] = None,
@@ -95,15 +95,9 @@ class Q4Tensor:
             raise ValueError("offsets must have one entry more than there are experts")
         if torch.is_grad_enabled() and (rows.requires_grad or (bias is not None and bias.requires_grad)):
             raise NotImplementedError("experts in 4 bits record no gradients: call them under torch.no_grad()")
-        refuse_tangents(rows, bias)
+        ops.refuse_tangents(rows, bias)
         rows, bias = _operand(rows, self.device), _bias(bias, self.device)
         return ops.experts_q4(self.codes, self.scales, self.shape[1], rows, self.shape[2], self.group, offsets, bias, out_dtype)
-
-
-def refuse_tangents(*tensors: Optional[torch.Tensor]) -> None:
-    """Forward-mode derivatives (torch.autograd.forward_ad) would be lost in a native call."""
-    if _capi.native.has_tangent(*tensors):
-        raise NotImplementedError("products from packed weights have no forward-mode derivatives")
 
 
 def _check_type(x: torch.Tensor) -> None:
