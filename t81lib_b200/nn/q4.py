@@ -16,7 +16,10 @@ from .. import torch as t81_torch
 
 
 class _Q4Module(nn.Module):
-    """Holds Q4Tensors as pairs of buffers (``<name>_codes``, ``<name>_scales``)."""
+    """Holds Q4Tensors as pairs of buffers (``<name>_codes``, ``<name>_scales``).  The buffers' lengths tell rows and columns only up to whole
+    tiles, so the state dict has the weights' shapes beside them (``_extra_state``, int64)."""
+
+    _version = 2  # 1: without the shapes
 
     # the float weight is gone: what saves models asks for this
     _t81_float_released = True
@@ -58,6 +61,23 @@ class _Q4Module(nn.Module):
             if now.dtype != torch.bfloat16:
                 self._buffers[name] = b.to(now.device)
         return self
+
+    def get_extra_state(self) -> torch.Tensor:
+        return torch.tensor([n for shape in self._q4_shapes.values() for n in shape], dtype=torch.int64)
+
+    def set_extra_state(self, state: torch.Tensor) -> None:
+        pass  # looked at before anything is loaded
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs) -> None:
+        key = prefix + "_extra_state"
+        held = state_dict.get(key)
+        if held is not None and held.tolist() != self.get_extra_state().tolist():
+            error_msgs.append(f"size mismatch for {prefix}{'/'.join(self._q4_shapes)}: the state holds 4-bit weights of other sizes, {held.tolist()}, "
+                              f"than this module's, {self.get_extra_state().tolist()}.")
+            return
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
+        if held is None and local_metadata.get("version", 1) < 2 and key in missing_keys:
+            missing_keys.remove(key)
 
     def __getstate__(self):
         return {**self.__dict__, "_q4": {}}  # native calls do not travel

@@ -1,0 +1,62 @@
+"""What 4-bit layers and tensors keep of themselves: state dicts, copies, the names a model was converted by."""
+
+import copy
+import io
+import pickle
+from collections import OrderedDict
+
+import pytest
+import torch
+from torch import nn
+
+
+def _filled(module, seed):
+    """Codes and scales that tell modules apart."""
+    gen = torch.Generator().manual_seed(seed)
+    for b in module.buffers():
+        b.copy_(torch.randint(0, 255, b.shape, generator=gen).to(b.dtype))
+    return module
+
+
+def test_state_of_another_size_is_refused(lib_built):
+    """Rows and columns that round up to the same tiles: the buffers are as long, the weights are not the same."""
+    from t81lib_b200.nn import Q4Experts, Q4Linear
+    pairs = [(lambda: Q4Linear(4096, 300, bias=False), lambda: Q4Linear(4090, 295, bias=False)), (lambda: Q4Linear(64, 48), lambda: Q4Linear(50, 48)),
+             (lambda: Q4Experts(3, 100, 40, group=32), lambda: Q4Experts(3, 100, 39, group=32)), (lambda: Q4Experts(3, 96, 40), lambda: Q4Experts(3, 90, 40))]
+    for one, other in pairs:
+        target, source = _filled(one(), 1), _filled(other(), 2)
+        assert [b.shape for b in target.buffers()] == [b.shape for b in source.buffers()]
+        before = {k: v.clone() for k, v in target.state_dict().items()}
+        for strict in (True, False):
+            for assign in (True, False):
+                with pytest.raises(RuntimeError, match="size mismatch"):
+                    target.load_state_dict(source.state_dict(), strict=strict, assign=assign)
+                with pytest.raises(RuntimeError, match="size mismatch"):
+                    nn.Sequential(target).load_state_dict(nn.Sequential(source).state_dict(), strict=strict, assign=assign)
+        assert all(torch.equal(v, before[k]) for k, v in target.state_dict().items())  # nothing was loaded
+
+
+def test_state_comes_back(lib_built):
+    from t81lib_b200.nn import Q4Experts, Q4Linear
+    for make in (lambda: nn.Sequential(Q4Linear(100, 40, group=32), Q4Linear(40, 7, bias=False)), lambda: Q4Experts(3, 100, 40, group=32)):
+        source = _filled(make(), 3)
+        file = io.BytesIO()
+        torch.save(source.state_dict(), file)
+        file.seek(0)
+        state = torch.load(file, weights_only=True)
+        assert all(isinstance(v, torch.Tensor) for v in state.values())  # formats that hold tensors alone take it
+        target = _filled(make(), 4)
+        assert str(target.load_state_dict(state)) == "<All keys matched successfully>"
+        for target_of in (lambda s: s, lambda s: dict(s), lambda s: OrderedDict((k, v) for k, v in s.items())):
+            target = _filled(make(), 4)
+            target.load_state_dict(target_of(state))
+            assert all(torch.equal(a, b) for a, b in zip(target.buffers(), source.buffers()))
+        # states without the shapes, as they were once
+        bare = OrderedDict((k, v) for k, v in state.items() if not k.endswith("_extra_state"))
+        target = _filled(make(), 4)
+        target.load_state_dict(bare)
+        assert all(torch.equal(a, b) for a, b in zip(target.buffers(), source.buffers()))
+        # of this version they belong to it
+        bare._metadata = state._metadata
+        with pytest.raises(RuntimeError, match="_extra_state"):
+            make().load_state_dict(bare)
