@@ -132,8 +132,8 @@ def _four_bit_modules(model: nn.Module, patterns: Sequence[str]) -> "list[str]":
     return found
 
 
-def _to_four_bit(model: nn.Module, names: Sequence[str], group: int, keep_biases_bf16: bool, stats: ConversionStats) -> None:
-    for name in names:
+def _to_four_bit(model: nn.Module, patterns: Sequence[str], group: int, keep_biases_bf16: bool, stats: ConversionStats) -> None:
+    for name in _four_bit_modules(model, patterns):
         module = model.get_submodule(name)
         if isinstance(module, nn.Linear):
             new = Q4Linear.from_linear(module, group)
@@ -147,6 +147,11 @@ def _to_four_bit(model: nn.Module, names: Sequence[str], group: int, keep_biases
                     setattr(parent, leaf, new)
         stats.four_bit += 1
         stats.four_bit_bytes += sum(b.numel() * b.element_size() for b in new.buffers())
+    # added to what earlier calls replaced: saved names make all of it again
+    calls = [*getattr(model, "_t81_four_bit_calls", ()), [list(patterns), group]]
+    model._t81_four_bit_calls = calls
+    model._t81_four_bit = list(dict.fromkeys(pattern for names, _ in calls for pattern in names))
+    model._t81_q4_group = group
 
 
 def _walk_and_replace(module: nn.Module, threshold: float, keep_biases_bf16: bool, rule: str, pack_now: bool,
@@ -201,14 +206,12 @@ def convert_module(model: nn.Module, threshold: float = 0.45, keep_biases_bf16: 
 
     ``four_bit`` names modules (``"lm_head"``, ``"layers.*.mlp.experts"``) that go to 4-bit weights with a scale per ``q4_group``
     columns instead: each ``nn.Linear`` and each module of stacked experts so named, whose weights must be on a CUDA device and whose
-    float weights are given up."""
+    float weights are given up.  Later calls may name more, in groups of another size too."""
     stats = ConversionStats()
     if q4_group not in (32, 64, 128):
         raise ValueError(f"groups of 32, 64 or 128 columns, not {q4_group}")
     if four_bit:
-        _to_four_bit(model, _four_bit_modules(model, four_bit), q4_group, keep_biases_bf16, stats)
-        setattr(model, "_t81_four_bit", list(four_bit))
-        setattr(model, "_t81_q4_group", q4_group)
+        _to_four_bit(model, four_bit, q4_group, keep_biases_bf16, stats)
     _walk_and_replace(model, threshold, keep_biases_bf16, rule, pack_now, release_float, stats)
     setattr(model, "_t81_threshold", threshold)
     setattr(model, "_t81_keep_biases_bf16", keep_biases_bf16)
@@ -276,6 +279,9 @@ def save_pretrained_t81(model: nn.Module, save_directory, *, threshold: Optional
     }
     if getattr(model, "_t81_four_bit", None):
         metadata |= {"four_bit": model._t81_four_bit, "q4_group": model._t81_q4_group}
+        calls = getattr(model, "_t81_four_bit_calls", ())
+        if len({group for _, group in calls}) > 1:
+            metadata["four_bit_calls"] = calls
     with _metadata_path(directory).open("w", encoding="utf-8") as handle:
         json.dump(metadata, handle)
 
@@ -302,8 +308,12 @@ def from_pretrained_t81(cls, pretrained_model_name_or_path, *model_args: Any, th
     else:
         model = cls.from_pretrained(pretrained_model_name_or_path, *model_args, trust_remote_code=trust_remote_code,
                                     device_map=device_map, torch_dtype=torch_dtype, **model_kwargs)
-    convert_module(model, threshold, keep_biases_bf16, rule=metadata.get("rule", "fixed"), verbose=False,
-                   four_bit=metadata.get("four_bit", ()), q4_group=metadata.get("q4_group", 128))
+    four_bit, group = metadata.get("four_bit", ()), metadata.get("q4_group", 128)
+    if "four_bit_calls" in metadata:  # groups of several sizes: call by call, as they were made
+        *earlier, (four_bit, group) = metadata["four_bit_calls"]
+        for names, size in earlier:
+            _to_four_bit(model, names, size, keep_biases_bf16, ConversionStats())
+    convert_module(model, threshold, keep_biases_bf16, rule=metadata.get("rule", "fixed"), verbose=False, four_bit=four_bit, q4_group=group)
     return model
 
 

@@ -60,3 +60,42 @@ def test_state_comes_back(lib_built):
         bare._metadata = state._metadata
         with pytest.raises(RuntimeError, match="_extra_state"):
             make().load_state_dict(bare)
+
+
+class Model(nn.Module):
+    def __init__(self):
+        super().__init__()
+        self.first, self.second, self.third, self.last = (nn.Linear(96, 96) for _ in range(4))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("groups", [(64, 64), (128, 32), (32, 32, 128)])
+def test_converted_in_several_calls(lib_built, tmp_path, groups):
+    """Names of every call are kept: a model loaded by them has the 4-bit weights of all."""
+    from t81lib_b200 import convert
+    from t81lib_b200.nn import Linear, Q4Linear
+    names = ["first", "thi*", "second"][:len(groups)]
+    torch.manual_seed(0)
+    floats = Model().state_dict()
+    model = Model().cuda()
+    model.load_state_dict(floats)
+    for name, group in zip(names, groups):
+        convert.convert_module(model, rule="absmean", verbose=False, four_bit=[name], q4_group=group)
+    convert.save_pretrained_t81(model, tmp_path, call_save_pretrained=False)
+
+    def loader(path):
+        again = Model()
+        again.load_state_dict(floats)
+        return again.cuda()
+
+    again = convert.from_pretrained_t81(None, tmp_path, loader=loader)
+    x = torch.randn(3, 96, device="cuda")
+    for leaf in ("first", "second", "third", "last"):
+        one, other = getattr(model, leaf).eval(), getattr(again, leaf).eval()
+        assert type(one) is type(other) and isinstance(one, Linear if leaf == "last" or (leaf == "second" and len(groups) == 2) else Q4Linear)
+        assert not isinstance(one, Q4Linear) or one.group == other.group
+        with torch.no_grad():
+            assert torch.equal(one(x), other(x))
+    # and saved once more the names are the same
+    convert.save_pretrained_t81(again, tmp_path / "again", call_save_pretrained=False)
+    assert convert.read_metadata(tmp_path / "again") == convert.read_metadata(tmp_path)
