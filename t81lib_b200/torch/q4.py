@@ -30,7 +30,14 @@ class Q4Tensor:
                 or scales.numel() != matrices * tiles * ((shape[-1] + group - 1) // group + 1) * 16 or scales.device != codes.device:
             raise ValueError(f"codes and scales do not hold a {tuple(shape)} weight with groups of {group}")
         self.codes, self.scales, self.shape, self.group = codes, scales, shape, group
-        self._product = None  # the native call
+
+    def __setattr__(self, name: str, value) -> None:
+        object.__setattr__(self, name, value)
+        if name != "_product":
+            object.__setattr__(self, "_product", None)  # the native call; it holds what it was made of
+
+    def __reduce__(self):
+        return type(self), (self.codes, self.scales, tuple(self.shape), self.group)  # native calls do not travel
 
     @classmethod
     def from_float(cls, source: torch.Tensor, group: int = 128) -> "Q4Tensor":

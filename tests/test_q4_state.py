@@ -99,3 +99,33 @@ def test_converted_in_several_calls(lib_built, tmp_path, groups):
     # and saved once more the names are the same
     convert.save_pretrained_t81(again, tmp_path / "again", call_save_pretrained=False)
     assert convert.read_metadata(tmp_path / "again") == convert.read_metadata(tmp_path)
+
+
+def test_copies_of_a_tensor(lib_built):
+    from t81lib_b200.torch import Q4Tensor
+    codes, scales = torch.randint(0, 255, (512,)).to(torch.uint8), torch.rand(32).to(torch.bfloat16)
+    q = Q4Tensor(codes, scales, (16, 64), 64)
+    for again in (copy.deepcopy(q), pickle.loads(pickle.dumps(q)), copy.copy(q)):
+        assert again.shape == q.shape and isinstance(again.shape, torch.Size) and again.group == 64
+        assert torch.equal(again.codes, codes) and torch.equal(again.scales, scales)
+    assert copy.copy(q).codes is codes and copy.deepcopy(q).codes is not codes
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [2, 40])
+def test_copies_and_new_weights_after_a_product(lib_built, tokens):
+    from t81lib_b200.torch import Q4Tensor
+    torch.manual_seed(tokens)
+    q, other = (Q4Tensor.from_float(torch.randn(48, 96, device="cuda"), group=32) for _ in range(2))
+    x = torch.randn(tokens, 96, device="cuda")
+    y, want = q.matmul_input(x), other.matmul_input(x)
+    assert torch.equal(copy.deepcopy(q).matmul_input(x), y) and torch.equal(pickle.loads(pickle.dumps(q)).matmul_input(x), y)
+    file = io.BytesIO()
+    torch.save({"head": q}, file)
+    file.seek(0)
+    assert torch.equal(torch.load(file, weights_only=False)["head"].matmul_input(x), y)
+    q.codes, q.scales = other.codes, other.scales  # what was multiplied by is not kept
+    assert torch.equal(q.matmul_input(x), want) and torch.equal(q.dequantize(), other.dequantize())
+    q.codes = other.codes[:-1]
+    with pytest.raises(ValueError, match="do not hold"):
+        q.matmul_input(x)
