@@ -35,6 +35,7 @@ EXPORTS = (
 )
 TQ1_0, TQ2_0 = 0, 1
 T2_MAX_TOKENS = 128  # T81B200_T2_MAX_ROWS
+MOST_EXPERTS = 1024  # of sort_by_expert and experts_q4
 MAX_GROUP = 3       # T81B200_MAX_GROUP
 EW_WHERE, EW_CLAMP, EW_LERP, EW_ADDCMUL = 0, 1, 2, 3
 

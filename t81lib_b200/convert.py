@@ -32,6 +32,7 @@ from torch import nn
 
 from .nn import Linear as TernaryLinear
 from .nn import Q4Experts, Q4Linear
+from . import _capi
 from . import torch as t81_torch
 
 _METADATA_FILENAME = "t81_metadata.json"
@@ -118,6 +119,8 @@ def _four_bit_modules(model: nn.Module, patterns: Sequence[str]) -> "list[str]":
             raise ValueError(f"four_bit: the float weight of {name} was released")
         if isinstance(module, nn.Linear) or _holds_experts(module):
             weights = [module.weight] if isinstance(module, nn.Linear) else [module.gate_up_proj, module.down_proj]
+            if weights[0].ndim == 3 and weights[0].shape[0] > _capi.MOST_EXPERTS:
+                raise ValueError(f"four_bit: {name} has {weights[0].shape[0]} experts, more than {_capi.MOST_EXPERTS}")
             if any(w.is_meta or not w.is_cuda for w in weights):
                 raise ValueError(f"four_bit: the weights of {name} must be on a CUDA device")
             if any(w.numel() == 0 for w in weights):

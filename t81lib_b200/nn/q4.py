@@ -83,6 +83,11 @@ class _Q4Module(nn.Module):
         return {**self.__dict__, "_q4": {}}  # native calls do not travel
 
 
+def _check_experts(n: int) -> None:
+    if n > _capi.MOST_EXPERTS:
+        raise ValueError(f"{n} experts: a mixture in 4 bits has at most {_capi.MOST_EXPERTS}")
+
+
 class Q4Linear(_Q4Module):
     """``nn.Linear`` with a 4-bit weight: ``x @ W.T + bias`` for 1 to any number of tokens, float32, bfloat16 or float16."""
 
@@ -140,6 +145,7 @@ class Q4Experts(_Q4Module):
                  device: Optional[torch.device] = None) -> None:
         """Empty experts, for ``load_state_dict``."""
         super().__init__(group)
+        _check_experts(n_experts)
         self.n_experts, self.hidden, self.ffn, self.act_fn = n_experts, hidden, ffn, act_fn
         self._hold("gate_up", None, (n_experts, 2 * ffn, hidden), device)
         self._hold("down", None, (n_experts, hidden, ffn), device)
@@ -150,6 +156,7 @@ class Q4Experts(_Q4Module):
         """``gate_up_proj`` (experts, 2 ffn, hidden): the gate's rows, then the up projection's; ``down_proj`` (experts, hidden, ffn)."""
         if gate_up_proj.ndim != 3 or down_proj.ndim != 3 or gate_up_proj.shape != (down_proj.shape[0], 2 * down_proj.shape[2], down_proj.shape[1]):
             raise ValueError(f"experts must be (experts, 2 ffn, hidden) and (experts, hidden, ffn), not {tuple(gate_up_proj.shape)} and {tuple(down_proj.shape)}")
+        _check_experts(down_proj.shape[0])
         layer = cls.__new__(cls)
         _Q4Module.__init__(layer, group)
         layer.n_experts, layer.hidden, layer.ffn = down_proj.shape

@@ -129,3 +129,27 @@ def test_copies_and_new_weights_after_a_product(lib_built, tokens):
     q.codes = other.codes[:-1]
     with pytest.raises(ValueError, match="do not hold"):
         q.matmul_input(x)
+
+
+class Experts(nn.Module):
+    def __init__(self, experts):
+        super().__init__()
+        self.gate_up_proj, self.down_proj = nn.Parameter(torch.zeros(experts, 4, 3)), nn.Parameter(torch.zeros(experts, 3, 2))
+        self.act_fn = nn.SiLU()
+
+
+def test_more_experts_than_the_routing_takes(lib_built):
+    """Refused before a float weight is given up for experts that no call could run."""
+    from t81lib_b200 import convert
+    from t81lib_b200.nn import Q4Experts
+    assert Q4Experts(1024, 3, 2).n_experts == 1024
+    with pytest.raises(ValueError, match="at most 1024"):
+        Q4Experts(1025, 3, 2)
+    many = Experts(1025)
+    with pytest.raises(ValueError, match="at most 1024"):
+        Q4Experts.from_float(many.gate_up_proj, many.down_proj)
+    model = nn.Module()
+    model.first, model.second = nn.Linear(4, 4), many
+    with pytest.raises(ValueError, match="second has 1025 experts"):
+        convert.convert_module(model, four_bit=["second"])
+    assert model.second is many and type(model.first) is nn.Linear
