@@ -430,8 +430,7 @@ T81B200_API size_t t81b200_gemm_trit_workspace_bytes(int b_dtype, int layout, in
  *   dequantize_q4: (matrices, rows, cols) contiguous, exact in fp32 and bf16.  q4_group_scales: (matrices, rows, groups) bf16, contiguous.
  *   linear_q4:     C (N, M) = B (N, K) W^T + bias, W (M, K); B as it is where its type is 16-bit, its rows lie on 16-byte boundaries and
  *                  K % 8 == 0, else through the workspace (linear_q4_workspace_bytes for this very B, 16-byte aligned).  Products are
- *                  exact, sums the tensor cores' fp32 ones (plain fp32 ones where fp16 does not hold a row beside fp16 B, whose scales
- *                  span more than 2^30); fp32 B keeps all 24 bits.
+ *                  exact, sums the tensor cores' fp32 ones; fp32 B keeps all 24 bits.
  *   experts_q4:    the same with rows sorted by expert: row p is multiplied by matrix e, offsets[e] <= p < offsets[e + 1]; codes, scales
  *                  and bias (n_experts, M) one expert behind the other; offsets: n_experts + 1 rising numbers on the device.
  *                  Rows ahead of offsets[0], and at or past offsets[n_experts], become 0. */

@@ -177,49 +177,103 @@ constexpr int kF16Up = 10, kF16Span = kF16Up + 20;
 // Whether a scale (bf16 bits without the sign) is too small for that beside a row's largest.
 __device__ __forceinline__ bool f16_loses(uint32_t scale, uint32_t exponent) { return scale != 0u && (int)scale < (int)(exponent >> 16) - (kF16Span << 7); }
 
-// Results of a tile's rows with such scales, from the codes, in fp32: a warp per row and four rows of x, a lane sixteen columns of one of eight 64-column
-// tiles at a time, the lanes' sums in a fixed order.  For the few rows that want it, if any: two to three orders slower than the tensor core.
+// Results of a tile's rows with such scales, once more as the streaming kernel computes them: codes as whole numbers times fp16, the scale on the fp32
+// sum.  16 rows and 16 rows of x at a time; a CTA's warps share the columns, and their sums meet in `part` in warp order.  For the
+// few rows that want it, if any: 4096 x 14336, 64 rows of x 27 us, 79 with one such row, 430 where all are.
+constexpr int MEND_WARPS = NUM_THREADS / 32, MEND_TOK = 16;
 template <typename CT>
-__device__ __noinline__ void mend_rows(const Q4TcParams &p, int expert, int row0, int tok0, int end, int warp, int lane) {
-    const int64_t col_tiles = q4_col_tiles(p.K);
-    for (int r = warp; r < BM && row0 + r < p.M; r += NUM_THREADS / 32) {
-        const int row = row0 + r, g = row & 7, hi = (row >> 3) & 1, t = lane & 3;
-        const int64_t tile = (int64_t)expert * p.row_tiles + (row >> 4);
-        const unsigned short *scales = reinterpret_cast<const unsigned short *>(p.scales) + tile * (p.groups + 1) * 16 + 2 * g + hi;
-        const uint32_t exponent = row_exponent(p.scales, tile, p.groups, row & 15);
-        bool lost = false;
-        for (int u = lane; u < p.groups; u += 32) lost = lost || f16_loses(scales[(int64_t)u * 16] & 0x7FFFu, exponent);
-        if (!__any_sync(0xffffffffu, lost)) continue;
-        const float bias = p.bias ? p.bias[(int64_t)expert * p.M + row] : 0.0f;
-        for (int tok = tok0; tok < end; tok += 4) {
-            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            for (int64_t c = lane >> 2; c < col_tiles; c += 8) {
-                const uint4 q = *reinterpret_cast<const uint4 *>(p.codes + (tile * col_tiles + c) * kQ4TileBytes + (4 * g + t) * 16);
+__device__ void mend_rows(const Q4TcParams &p, float (*part)[MEND_TOK][17], uint32_t *rows, int expert, int row0, int tok0, int end) {
+    const int warp = (int)threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, col_tiles = (int)q4_col_tiles(p.K), halves_per_group = p.group / 32;
+    const int64_t first_tile = (int64_t)expert * p.row_tiles + (row0 >> 4);
+    if (threadIdx.x < BM / 32) rows[threadIdx.x] = 0u;
+    __syncthreads();
+    for (int tile16 = warp >> 1; tile16 < BM / 16 && row0 + 16 * tile16 < p.M; tile16 += MEND_WARPS / 2) {  // two warps each, a lane two rows of every eighth group
+        const int64_t tile = first_tile + tile16;
+        const int r = lane & 7;
+        const uint32_t *scales = reinterpret_cast<const uint32_t *>(p.scales + tile * (p.groups + 1) * 16) + r;
+        const uint32_t lower = row_exponent(p.scales, tile, p.groups, r), upper = row_exponent(p.scales, tile, p.groups, r + 8);
+        uint32_t lost = 0u;
+#pragma unroll 4
+        for (int u = 4 * (warp & 1) + (lane >> 3); u < p.groups; u += 8) {
+            const uint32_t pair = scales[(int64_t)u * 8];
+            lost |= (f16_loses(pair & 0x7FFFu, lower) ? 1u : 0u) | (f16_loses(pair >> 16 & 0x7FFFu, upper) ? 256u : 0u);
+        }
+        if (lost) atomicOr(rows + (tile16 >> 1), lost << (r + 16 * (tile16 & 1)));
+    }
+    __syncthreads();
+    const Q4Decode<__half> decode;
+    for (int tile16 = 0; tile16 < BM / 16; ++tile16) {
+        const uint32_t mine = rows[tile16 >> 1] >> (16 * (tile16 & 1)) & 0xFFFFu;
+        if (mine == 0u) continue;
+        const int64_t tile = first_tile + tile16;
+        const uint8_t *codes = p.codes + tile * col_tiles * kQ4TileBytes + lane * 16;
+        const __nv_bfloat16 *scales = p.scales + tile * (p.groups + 1) * 16 + 2 * g;
+        for (int tok = tok0; tok < end; tok += MEND_TOK) {
+            float sum[MEND_TOK / 8][4] = {};
+            for (int c = warp; c < col_tiles; c += MEND_WARPS) {
+                const uint4 q = *reinterpret_cast<const uint4 *>(codes + (int64_t)c * kQ4TileBytes);
+                const uint32_t words[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const int64_t col = 64 * c + 32 * half + 8 * t;
-                    if (col >= p.K) continue;  // (rows of x are whole pieces of eight)
-                    const float s = __uint_as_float((uint32_t)scales[col / p.group * 16] << 16);
-                    float w[8];
+                for (int half = 0; half < 2; ++half) {  // (rows of x are whole pieces of eight, zeros from K on)
+                    const int64_t col = 64 * (int64_t)c + 32 * half;
+                    const uint32_t s = col < p.K ? *reinterpret_cast<const uint32_t *>(scales + (int64_t)((2 * c + half) / halves_per_group) * 16) : 0u;
+                    uint4 x[MEND_TOK / 8];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        w[i] = (float)((int)(((half ? (i < 4 ? q.z : q.w) : (i < 4 ? q.x : q.y)) >> (4 * (2 * ((i >> 1) & 1) + hi) + 16 * (i & 1))) & 15u) - 8) * s;
+                    for (int n = 0; n < MEND_TOK / 8; ++n) {
+                        const __half *src = static_cast<const __half *>(p.x) + (int64_t)min(tok + 8 * n + g, end - 1) * p.ldx + col + 8 * t;
+                        x[n] = col + 8 * t < p.K ? *reinterpret_cast<const uint4 *>(src) : make_uint4(0u, 0u, 0u, 0u);
+                    }
+                    uint32_t a[2][4];
+                    q4_fragments(decode, words[2 * half], a[0]);
+                    q4_fragments(decode, words[2 * half + 1], a[1]);
+                    const float lo = __uint_as_float(s << 16), hi = __uint_as_float(s & 0xFFFF0000u);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        if (tok + k >= end) break;
-                        const uint4 v = *reinterpret_cast<const uint4 *>(static_cast<const __half *>(p.x) + (int64_t)(tok + k) * p.ldx + col);
+                    for (int n = 0; n < MEND_TOK / 8; ++n) {
+                        float d[4];
+                        mma_16816<__half, false>(d, a[0], x[n].x, x[n].y);
+                        mma_16816<__half, true>(d, a[1], x[n].z, x[n].w);
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) sum[k] = fmaf(w[i], __half2float(reinterpret_cast<const __half *>(&v)[i]), sum[k]);
+                        for (int k = 0; k < 4; ++k) sum[n][k] = fmaf(d[k], k < 2 ? lo : hi, sum[n][k]);
                     }
                 }
             }
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
+            for (int n = 0; n < MEND_TOK / 8; ++n)
 #pragma unroll
-                for (int d = 16; d > 0; d >>= 1) sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], d);
-                if (lane == k && tok + k < end) static_cast<CT *>(p.C)[(int64_t)(tok + k) * p.ldc + row] = from_float<CT>(sum[k] + bias);
+                for (int k = 0; k < 4; ++k) part[warp][8 * n + 2 * t + (k & 1)][g + 8 * (k >> 1)] = sum[n][k];
+            __syncthreads();
+            for (int i = threadIdx.x; i < 16 * MEND_TOK; i += NUM_THREADS) {
+                const int r = i & 15, row = row0 + 16 * tile16 + r, at = tok + (i >> 4);
+                if (!(mine >> r & 1u) || at >= end) continue;
+                float v = p.bias ? p.bias[(int64_t)expert * p.M + row] : 0.0f;
+                for (int w = 0; w < MEND_WARPS; ++w) v += part[w][i >> 4][r];
+                static_cast<CT *>(p.C)[(int64_t)at * p.ldc + row] = from_float<CT>(v);
             }
+            __syncthreads();
         }
+    }
+    __syncthreads();  // `rows` is the next tile's
+}
+
+// The barriers' place in a CTA's shared memory, behind the rings and what the epilogue stages; the list of experts lies behind them.
+__device__ __forceinline__ uint32_t barriers_at(const Q4TcParams &p, int planes, int group) {
+    return A_STAGES * A_CHUNK_BYTES + (uint32_t)p.b_stages * (uint32_t)(planes * p.bn * BK) + (uint32_t)p.raw_stages * (RAW_CODES + 8 * (CHUNK / group) * 32) + (uint32_t)p.out_bytes;
+}
+
+// The same for every tile of a CTA, in whose shared memory nothing is awaited any more.
+template <typename CT, bool EXPERTS>
+__device__ __noinline__ void mend_tiles(const Q4TcParams &p) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *const memory = smem_raw + (((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw));
+    TileList<EXPERTS> tiles;
+    int total = p.m_tiles * p.n_tiles;
+    if constexpr (EXPERTS) {
+        tiles.list.at = reinterpret_cast<int2 *>(memory + barriers_at(p, 1, p.group) + BARRIER_BYTES);
+        total = tiles.list.before(p.n_experts) * p.m_tiles;
+    }
+    for (int i = (int)blockIdx.x / (2 * p.splits); i < total; i += (int)gridDim.x / (2 * p.splits)) {
+        const Tile t = tiles.tile(p, i, (int)(blockIdx.x & 1u));
+        mend_rows<CT>(p, reinterpret_cast<float (*)[MEND_TOK][17]>(memory + 16), reinterpret_cast<uint32_t *>(memory), t.expert, t.row0, t.tok, t.end);
     }
 }
 
@@ -606,11 +660,8 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_co
         tmem_free_pair(tmem_base);
     }
     if constexpr (F16)
-        if (*losses)  // the cluster's results are written: those of rows that fp16 does not hold are written again
-            for (int i = cluster_id; i < total_tiles; i += n_clusters) {
-                const Tile t = tiles.tile(p, i, half);
-                mend_rows<CT>(p, t.expert, t.row0, t.tok, t.end, warp, lane);
-            }
+        if (__builtin_expect(*losses, 0))  // the cluster's results are written: those of rows that fp16 does not hold are written again
+            mend_tiles<CT, EXPERTS>(p);
 }
 
 // Time of a 64-deep step at n columns, in ns: 18944 rows of 8192 columns (4096 for wide tiles of three planes), one tile a pair, 34 to 256 rows of

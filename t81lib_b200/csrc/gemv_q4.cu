@@ -57,33 +57,6 @@ struct Q4Params {
     int k_warps;                    // warps that share a row tile's units
 };
 
-// c = a b, or (ADD) c += a b.
-template <typename T, bool ADD> __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-#define T81_MMA(TYPE)                                                                                                                                  \
-    if constexpr (ADD)                                                                                                                                 \
-        asm("mma.sync.aligned.m16n8k16.row.col.f32." TYPE "." TYPE ".f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"              \
-            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])                                                                                           \
-            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));                                                                           \
-    else                                                                                                                                               \
-        asm("mma.sync.aligned.m16n8k16.row.col.f32." TYPE "." TYPE ".f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"          \
-            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])                                                                                           \
-            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f))
-    if constexpr (std::is_same<T, __half>::value) {
-        T81_MMA("f16");
-    } else {
-        T81_MMA("bf16");
-    }
-#undef T81_MMA
-}
-
-template <typename T>
-__device__ __forceinline__ void fragments(const Q4Decode<T> &decode, uint32_t w, uint32_t (&a)[4]) {
-    a[0] = decode.code(decode.template biased<0>(w));
-    a[1] = decode.code(decode.template biased<1>(w));
-    a[2] = decode.code(decode.template biased<2>(w));
-    a[3] = decode.code(decode.template biased<3>(w));
-}
-
 // Where a warp is: a block's share of the row tiles (of an expert), and a piece of at most TOK rows of x.  Items go through the shares of one
 // piece before those of the next, and a block takes every gridDim.x-th.
 template <int TOK> struct Walk {
@@ -261,7 +234,7 @@ gemv_q4_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_const
 #pragma unroll
                         for (int r = 0; r < RT; ++r) {
                             uint32_t a[4];
-                            fragments<T>(decode, word[r][j], a);
+                            q4_fragments(decode, word[r][j], a);
                             if (j % (GROUP / 16) == 0) products<T, PLANES, NT, true>(c[r], a, x, j & 1);
                             else products<T, PLANES, NT, false>(c[r], a, x, j & 1);
                         }

@@ -16,6 +16,8 @@
 
 #include "common.cuh"
 
+#include <type_traits>
+
 namespace t81b200 {
 
 constexpr int kQ4TileBytes = 512;
@@ -71,6 +73,33 @@ template <> struct Q4Decode<__half> {
         return d;
     }
 };
+
+// c = a b, or (ADD) c += a b.
+template <typename T, bool ADD> __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+#define T81_MMA(TYPE)                                                                                                                                  \
+    if constexpr (ADD)                                                                                                                                 \
+        asm("mma.sync.aligned.m16n8k16.row.col.f32." TYPE "." TYPE ".f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"              \
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])                                                                                           \
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));                                                                           \
+    else                                                                                                                                               \
+        asm("mma.sync.aligned.m16n8k16.row.col.f32." TYPE "." TYPE ".f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"          \
+            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])                                                                                           \
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f))
+    if constexpr (std::is_same<T, __half>::value) {
+        T81_MMA("f16");
+    } else {
+        T81_MMA("bf16");
+    }
+#undef T81_MMA
+}
+
+template <typename T>
+__device__ __forceinline__ void q4_fragments(const Q4Decode<T> &decode, uint32_t w, uint32_t (&a)[4]) {
+    a[0] = decode.code(decode.template biased<0>(w));
+    a[1] = decode.code(decode.template biased<1>(w));
+    a[2] = decode.code(decode.template biased<2>(w));
+    a[3] = decode.code(decode.template biased<3>(w));
+}
 
 // Rows sorted by expert as a list of pieces of at most `width` rows: in shared memory, made by every block from the experts' first rows.
 struct ExpertList {
