@@ -6,8 +6,9 @@
 // SM were 16 KB, and 65536 x 4096 with 8 tokens took 69 us).  A warp waits for and refills its own stages only.
 // A lane's 16 bytes of a tile are the A fragments of four mma.sync m16n8k16, the codes as exact numbers -8 .. 7, and its eight columns of an
 // activation row are the B fragments of two of them, read where the row lies (L1 holds the few rows that an SM's warps share).
-// Sums of a group are scaled and added in fp32.  A block's warps take the units of its rows in turn and their sums meet in shared
-// memory, in warp order: results do not depend on the schedule.
+// Sums of a group are scaled and added in fp32.  Beside bf16, whose numbers reach as far as fp32's, the codes are 2^-10 of what they are up to
+// the last step: 128 times 8 times the largest number stays finite, and so does a result that should be.  A block's warps take the units of
+// its rows in turn and their sums meet in shared memory, in warp order: results do not depend on the schedule.
 //
 // float32 activations come as three bf16 planes (all 24 bits, stage_planes), each multiplied exactly; the first has sums of its own, since the
 // tensor core cuts small terms beside large ones off.
@@ -56,6 +57,8 @@ struct Q4Params {
     int row_tiles, row_items;       // 16-row tiles, and blocks' shares of them (RT * k_split-wise rows)
     int k_warps;                    // warps that share a row tile's units
 };
+
+template <typename T> constexpr int kDown = std::is_same<T, __nv_bfloat16>::value ? 10 : 0;
 
 // Where a warp is: a block's share of the row tiles (of an expert), and a piece of at most TOK rows of x.  Items go through the shares of one
 // piece before those of the next, and a block takes every gridDim.x-th.
@@ -177,7 +180,7 @@ gemv_q4_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_const
     };
     if (p.units > 0)
         for (int i = 0; i < S::kCount; ++i) issue();
-    const Q4Decode<T> decode;
+    const Q4Decode<T, kDown<T>> decode;
     const uint32_t zero = unknown_zero();
     Ring at;
     bool ok = true, buffer = false;
@@ -279,6 +282,7 @@ gemv_q4_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_const
             if (row >= p.M) continue;
             float v = 0.0f;
             for (int w = 0; w < p.k_warps; ++w) v += part[((share * p.k_warps + w) * TOK + tok) * WIDTH + r];
+            v *= (float)(1 << kDown<T>);
             if (p.bias) v += p.bias[use.expert * p.bias_stride + row];
             store(p.y, (int64_t)(use.tok + tok) * p.ldy + row, v, p.y_dtype);
         }

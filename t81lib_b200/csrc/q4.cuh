@@ -43,11 +43,12 @@ template <uint32_t B> __device__ __forceinline__ uint32_t and_or(uint32_t a, uin
     return d;
 }
 
-template <typename T> struct Q4Decode;
-template <> struct Q4Decode<__nv_bfloat16> {
-    static constexpr uint32_t mask = 0x00780078u;
+// DOWN (bf16): the constants, and so the codes, times 2^-DOWN.
+template <typename T, int DOWN = 0> struct Q4Decode;
+template <int DOWN> struct Q4Decode<__nv_bfloat16, DOWN> {
+    static constexpr uint32_t mask = 0x00780078u, down = (uint32_t)DOWN * 0x00800080u;
     uint32_t sixteen, minus24;
-    __device__ __forceinline__ Q4Decode() : sixteen(opaque(0x41804180u)), minus24(opaque(0xC1C0C1C0u)) {}
+    __device__ __forceinline__ Q4Decode() : sixteen(opaque(0x41804180u - down)), minus24(opaque(0xC1C0C1C0u - down)) {}
     template <int R> __device__ __forceinline__ uint32_t biased(uint32_t w) const { return and_or<mask>(R == 0 ? w << 3 : w >> (4 * R - 3), sixteen); }
     __device__ __forceinline__ uint32_t code(uint32_t v) const {
         uint32_t d;
@@ -57,7 +58,7 @@ template <> struct Q4Decode<__nv_bfloat16> {
     // (v - 24) s for n = -24 s (7 bits): one rounding, of an exact result
     static __device__ __forceinline__ uint32_t scaled(uint32_t v, uint32_t s, uint32_t n) { return fma_bf16x2(v, s, n); }
 };
-template <> struct Q4Decode<__half> {
+template <> struct Q4Decode<__half, 0> {
     static constexpr uint32_t mask = 0x03C003C0u;
     uint32_t sixteen, minus24;
     __device__ __forceinline__ Q4Decode() : sixteen(opaque(0x4C004C00u)), minus24(opaque(0xCE00CE00u)) {}
@@ -93,8 +94,8 @@ template <typename T, bool ADD> __device__ __forceinline__ void mma_16816(float 
 #undef T81_MMA
 }
 
-template <typename T>
-__device__ __forceinline__ void q4_fragments(const Q4Decode<T> &decode, uint32_t w, uint32_t (&a)[4]) {
+template <typename Decode>
+__device__ __forceinline__ void q4_fragments(const Decode &decode, uint32_t w, uint32_t (&a)[4]) {
     a[0] = decode.code(decode.template biased<0>(w));
     a[1] = decode.code(decode.template biased<1>(w));
     a[2] = decode.code(decode.template biased<2>(w));

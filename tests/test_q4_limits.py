@@ -142,3 +142,41 @@ def test_forward_mode_is_refused(dev, grad):
         with pytest.raises(RuntimeError, match="jvp"):
             t81_torch.route(ids, 2).combine(x, fwd.make_dual(weights, torch.ones_like(weights)))
         assert layer(x).shape == (4, 48)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("largest", [2.0 ** 119, 3.3e38])
+def test_the_largest_activations(dev, dtype, largest):
+    """Activations beside the end of their type: results that are numbers come out as those, however many rows there are."""
+    from t81lib_b200 import torch as t81_torch
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    for rows, cols, group in ((300, 512, 128), (2048, 4096, 32), (100, 1032, 64)):
+        q = t81_torch.Q4Tensor.from_float(torch.randn(rows, cols, generator=gen, device=dev) * 2.0 ** -20, group=group)
+        values = q.dequantize().double()
+        for tokens in (1, 8, 12, 200):
+            x = (torch.rand(tokens, cols, generator=gen, device=dev) * 2 - 1).to(dtype) * largest
+            x[0] = largest
+            x[tokens // 2] = -largest
+            assert bool(torch.isfinite(x).all())
+            y = q.matmul_input(x)
+            assert bool(torch.isfinite(y).all())
+            _check(y, x, values)
+            stack = t81_torch.Q4Tensor(q.codes, q.scales, (1, rows, cols), group)
+            _check(stack.matmul_sorted(x, torch.tensor([0, tokens], dtype=torch.int32, device=dev)), x, values)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_results_near_the_smallest_numbers(dev, dtype):
+    """The smallest scales there are and small activations: off by at most 2^-135, the last place of float32 brought up by the sums' 2^10, 16 times."""
+    from t81lib_b200 import torch as t81_torch
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    q = t81_torch.Q4Tensor.from_float(torch.randn(300, 512, generator=gen, device=dev) * 2.0 ** -96, group=64)
+    values = q.dequantize().double()
+    for tokens in (3, 12, 200):
+        for factor in (1.0, 2.0 ** -16, 2.0 ** -24):
+            x = torch.randn(tokens, 512, generator=gen, device=dev).to(dtype) * factor
+            want, magnitude = ref.product(x, values)
+            off = (q.matmul_input(x, out_dtype=torch.float32).double() - want).abs()
+            assert bool((off <= ref.tolerance(magnitude, want, 512, torch.float32) + 2.0 ** -135).all()), float(off.max())
