@@ -446,7 +446,7 @@ T81B200_API int t81b200_linear_q4(const uint8_t *codes, const void *scales, cons
 T81B200_API int t81b200_experts_q4(const uint8_t *codes, const void *scales, const float *bias, void *C, int64_t M, const void *B, int b_dtype, int64_t ldb, int c_dtype, int64_t ldc,
                                    int64_t N, int64_t K, int group, const int32_t *offsets, int n_experts, void *workspace, size_t workspace_bytes, void *stream);
 
-/* Rows of a mixture of experts.  n = tokens * top (token, slot) pairs, flat index token * top + slot, n < 2^31.  No counterpart in the
+/* Rows of a mixture of experts.  n = tokens * top (token, slot) pairs, flat index token * top + slot, n < 2^31 (the sort: 2^31 - 2^19).  No counterpart in the
  * reference.
  *   sort_by_expert: ids (n int32 or int64, id_bytes 4 or 8) to order (n), position (n) and offsets (n_experts + 1): order[p] is the flat
  *       index of sorted row p, pairs of one expert in their order, -1 past the last; position is the inverse, -1 for ids outside

