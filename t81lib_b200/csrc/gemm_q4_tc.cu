@@ -534,7 +534,7 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_co
                     const int64_t tile = (int64_t)t.expert * p.row_tiles + (t.row0 >> 4) + cw;
 #pragma unroll
                     for (int r = 0; r < 2; ++r)
-                        shrink[r] = t.row0 + cw * 16 < p.M ? __uint_as_float(kOne - row_exponent(p.scales, tile, p.groups, g + 8 * r)) : 1.0f;  // 2^(kF16Up - e)
+                        shrink[r] = t.row0 + cw * 16 < p.M ? __uint_as_float(kOne - row_exponent(p.scales, tile, p.groups, g + 8 * r)) : 0x1p100f;  // 2^(kF16Up - e); rows past M lose nothing
                     fresh = false;
                 }
                 c += 2;
