@@ -10,7 +10,7 @@
 // Words 0, 1 are columns 0 .. 31 and words 2, 3 columns 32 .. 63, so that no multiply mixes two groups, and a lane's eight columns of either
 // half are 16 bytes of an activation row or of an operand tile.  Scales of tile row T and group u: 16 bf16 numbers at
 // (T * (groups + 1) + u) * 16, row r of the tile at 2 (r % 8) + r / 8: a lane's two rows are one word.  Behind the groups' come the
-// rows' largest magnitudes of a scale: kernels that hold weights in fp16 divide a row by the power of two in it.
+// rows' largest magnitudes of a scale: kernels that hold weights in fp16 bring a row into its range by the power of two in it.
 // Rows and columns past the matrix have code 0 (bits 8) and scale 0.
 #pragma once
 
