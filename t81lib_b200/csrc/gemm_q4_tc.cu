@@ -179,10 +179,10 @@ __device__ __forceinline__ bool f16_loses(uint32_t scale, uint32_t exponent) { r
 
 // Results of a tile's rows with such scales, once more as the streaming kernel computes them: codes as whole numbers times fp16, the scale on the fp32
 // sum.  16 rows and 16 rows of x at a time; a CTA's warps share the columns, and their sums meet in `part` in warp order.  For the
-// few rows that want it, if any: 4096 x 14336, 64 rows of x 27 us, 79 with one such row, 430 where all are.
+// few rows that want it, if any: 4096 x 14336, 64 rows of x 27 us, 76 with one such row, 406 where all are.
 constexpr int MEND_WARPS = NUM_THREADS / 32, MEND_TOK = 16;
 template <typename CT>
-__device__ void mend_rows(const Q4TcParams &p, float (*part)[MEND_TOK][17], uint32_t *rows, int expert, int row0, int tok0, int end) {
+__device__ __noinline__ void mend_rows(const Q4TcParams &p, float (*part)[MEND_TOK][17], uint32_t *rows, int expert, int row0, int tok0, int end) {
     const int warp = (int)threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, col_tiles = (int)q4_col_tiles(p.K), halves_per_group = p.group / 32;
     const int64_t first_tile = (int64_t)expert * p.row_tiles + (row0 >> 4);
     if (threadIdx.x < BM / 32) rows[threadIdx.x] = 0u;
@@ -255,23 +255,17 @@ __device__ void mend_rows(const Q4TcParams &p, float (*part)[MEND_TOK][17], uint
     __syncthreads();  // `rows` is the next tile's
 }
 
-// The barriers' place in a CTA's shared memory, behind the rings and what the epilogue stages; the list of experts lies behind them.
-__device__ __forceinline__ uint32_t barriers_at(const Q4TcParams &p, int planes, int group) {
-    return A_STAGES * A_CHUNK_BYTES + (uint32_t)p.b_stages * (uint32_t)(planes * p.bn * BK) + (uint32_t)p.raw_stages * (RAW_CODES + 8 * (CHUNK / group) * 32) + (uint32_t)p.out_bytes;
-}
-
-// The same for every tile of a CTA, in whose shared memory nothing is awaited any more.
-template <typename CT, bool EXPERTS>
-__device__ __noinline__ void mend_tiles(const Q4TcParams &p) {
+// The same for every tile of a CTA that multiplies experts' rows.  `memory`: its shared memory, in which nothing is awaited any more; the list of experts lies
+// behind the rings, what the epilogue stages and the barriers.
+template <typename CT>
+__device__ __noinline__ void mend_experts(const Q4TcParams &p) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t *const memory = smem_raw + (((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw));
-    TileList<EXPERTS> tiles;
-    int total = p.m_tiles * p.n_tiles;
-    if constexpr (EXPERTS) {
-        tiles.list.at = reinterpret_cast<int2 *>(memory + barriers_at(p, 1, p.group) + BARRIER_BYTES);
-        total = tiles.list.before(p.n_experts) * p.m_tiles;
-    }
-    for (int i = (int)blockIdx.x / (2 * p.splits); i < total; i += (int)gridDim.x / (2 * p.splits)) {
+    const uint32_t raw_bytes = RAW_CODES + 8 * (CHUNK / p.group) * 32;
+    TileList<true> tiles;
+    tiles.list.at = reinterpret_cast<int2 *>(memory + A_STAGES * A_CHUNK_BYTES + p.b_stages * (p.bn * BK) + p.raw_stages * raw_bytes + p.out_bytes + BARRIER_BYTES);
+    const int total = tiles.list.before(p.n_experts) * p.m_tiles;
+    for (int i = (int)blockIdx.x / 2; i < total; i += (int)gridDim.x / 2) {
         const Tile t = tiles.tile(p, i, (int)(blockIdx.x & 1u));
         mend_rows<CT>(p, reinterpret_cast<float (*)[MEND_TOK][17]>(memory + 16), reinterpret_cast<uint32_t *>(memory), t.expert, t.row0, t.tok, t.end);
     }
@@ -660,8 +654,16 @@ gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_co
         tmem_free_pair(tmem_base);
     }
     if constexpr (F16)
-        if (__builtin_expect(*losses, 0))  // the cluster's results are written: those of rows that fp16 does not hold are written again
-            mend_tiles<CT, EXPERTS>(p);
+        if (*losses) {  // the cluster's results are written: those of rows that fp16 does not hold are written again
+            // Two forms, because the registers that the call leaves to the rest of the kernel differ (us, without such rows, loop here and there: 32 experts of 2048 x
+            // 4096, 2048 tokens 135 and 131; 4096 x 14336, 64 rows 27.6 and 28.1).
+            if constexpr (EXPERTS) mend_experts<CT>(p);
+            else
+                for (int i = cluster_id; i < total_tiles; i += n_clusters) {
+                    const Tile t = tiles.tile(p, i, half);
+                    mend_rows<CT>(p, reinterpret_cast<float (*)[MEND_TOK][17]>(gen_base + 16), reinterpret_cast<uint32_t *>(gen_base), 0, t.row0, t.tok, t.end);
+                }
+        }
 }
 
 // Time of a 64-deep step at n columns, in ns: 18944 rows of 8192 columns (4096 for wide tiles of three planes), one tile a pair, 34 to 256 rows of
